@@ -29,6 +29,15 @@ class BqError(RuntimeError):
 _i64, _i32, _vp = C.c_int64, C.c_int, C.c_void_p
 _h = C.c_uint64
 
+class Kv4Pool(C.Structure):
+    """bq_kv4_pool of include/b200q.h."""
+    _fields_ = [("pages", _vp), ("tables", _vp), ("lens", _vp), ("refs", _vp), ("work", _vp), ("n_pages", _i64),
+                ("max_seqs", C.c_int32), ("max_pages", C.c_int32), ("layers", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("page", C.c_int32)]
+
+
+_pool = C.POINTER(Kv4Pool)
+
 # name -> (restype, argtypes); must list every symbol that include/b200q.h declares
 PROTOTYPES = {
     "bq_init": (_i32, [_i32]),
@@ -87,6 +96,17 @@ PROTOTYPES = {
     "bq_ep_layout_selftest": (_i32, [_vp, _i32, _i32, _i32, _vp, _vp]),
     "bq_ep_recv_view": (_i32, [_h, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_i64)]),
     "bq_ep_combine": (_i32, [_h, _vp, _vp, _vp, _i64, _i32, _vp, _i32, _vp]),
+    "bq_kv4_page_bytes": (_i64, [_pool]),
+    "bq_kv4_work_bytes": (_i64, [_pool]),
+    "bq_kv4_extend": (_i32, [_pool, _vp, _vp, _i64, _vp, _vp]),
+    "bq_kv4_fork": (_i32, [_pool, _vp, _vp, _i64, _vp]),
+    "bq_kv4_free": (_i32, [_pool, _vp, _i64, _vp]),
+    "bq_kv4_compact": (_i32, [_pool, _pool, _vp]),
+    "bq_kv4_append": (_i32, [_pool, _i32, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "bq_kv4_rope_append": (_i32, [_pool, _i32, _vp, _vp, _i32, C.c_float, _i32, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "bq_kv4_gather": (_i32, [_pool, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "bq_kv4_attention_work_bytes": (_i64, [_pool, _i32, _i32]),
+    "bq_kv4_attention": (_i32, [_pool, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
     "bq_qlinear_push": (_i32, [_h, _vp, _i32, _i64, _h, _vp]),
     "bq_allreduce": (_i32, [_h, _vp, _vp, _i64, _vp]),
     "bq_allreduce_add_rmsnorm": (_i32, [_h, _vp, _vp, _vp, _vp, _i64, _i64, C.c_float, _i32, _vp]),

@@ -332,6 +332,72 @@ int bq_ep_recv_view(bq_ep_t ep, void** xrecv_bf16, const int32_t** local_offsets
 int bq_ep_combine(bq_ep_t ep, const float* out_rows, const int32_t* inv, const float* w, int64_t T,
                   int top_k, void* y, int y_dtype, void* stream);
 
+/* ---- paged 4-bit KV cache (no counterpart in the reference; the specification's 4-bit format - "4-bit codes in
+ *      groups of 32 with an fp16 scale per group", groups along head_dim - applied to the keys and values that decode
+ *      attention streams) -------------------------------------------------------------------------------------------
+ * All memory is the caller's; the struct only says where it is and is read during the call.  A page holds `page`
+ * positions of every layer and KV head.  Sequences are rows ("slots") of the page table; pages may be shared between
+ * sequences and are counted.  A pool starts with lens = 0, refs = 0 and tables = -1; the pages need no initial value.
+ * Bytes of pages: [n_pages][layers][kv_heads][page / 16][576 * head_dim / 32]; a block of 16 positions holds K codes,
+ * K scales, V codes, V scales.  With G = d / 32, i = d % 32 / 16, e = d % 16 the code (+ 8) of K at position r, dimension
+ * d is the low (e < 8) or high nibble of byte G * 256 + ((r % 8) * 4 + e % 8 / 2) * 8 + 4 i + r / 8 + 2 * (e % 2), that of V
+ * the low or high nibble (by e again) of byte G * 256 + ((e % 8) * 4 + r % 8 / 2) * 8 + 4 i + r / 8 + 2 * (r % 2); scale of K
+ * number r * head_dim / 32 + G, of V number G * 16 + r % 8 / 2 * 4 + r / 8 * 2 + r % 2.
+ * Limits: head_dim a multiple of 32 up to 256, page a power of two from 16 to 4096, max_seqs <= 8192, max_pages * page
+ * <= 2^30, n_pages < 2^30; pages, refs and work 16-byte aligned.  The CUDA device must be the one bq_init() selected.  */
+typedef struct {
+  void* pages;         /* n_pages * bq_kv4_page_bytes() bytes                                                       */
+  int32_t* tables;     /* [max_seqs][max_pages] page numbers, -1 behind a sequence's last page                      */
+  int32_t* lens;       /* [max_seqs] positions of every sequence                                                    */
+  int32_t* refs;       /* [n_pages] sequences that hold a page, 0 = free                                            */
+  int32_t* work;       /* bq_kv4_work_bytes() of scratch for extend, fork and compact; contents do not matter       */
+  int64_t n_pages;
+  int32_t max_seqs, max_pages, layers, kv_heads, head_dim, page;
+} bq_kv4_pool;
+int64_t bq_kv4_page_bytes(const bq_kv4_pool* p);
+int64_t bq_kv4_work_bytes(const bq_kv4_pool* p);
+/* Batch calls below take, in DEVICE memory: slots int32[B] (NULL: slot b), starts int32[B + 1], ascending (NULL: one row per
+ * sequence): sequence b owns rows starts[b] .. starts[b + 1] - 1 of the n_rows token rows, and pos int32[B]: the position
+ * of its first row.  Rows that belong to no sequence are neither read nor written.  A sequence with pos < 0 takes no part.
+ * A slot, row range or position outside the pool records BQ_ERR_ARG in the status word and is treated like pos < 0.       */
+/* Makes room for each sequence's new rows: lens += rows, pages are given out lowest number first in batch order, and a
+ * partly filled last page that other sequences hold too is replaced by a copy (every layer).  pos_out[b] = the length
+ * before the call, or -1 if the sequence was refused and is unchanged: no pages left, longer than max_pages allows, or its
+ * slot already named earlier in the batch (the last two record BQ_ERR_ARG).                                              */
+int bq_kv4_extend(const bq_kv4_pool* p, const int32_t* slots, const int32_t* starts, int64_t B, int32_t* pos_out,
+                  void* stream);
+/* Sequence dst[i] becomes a copy of sequence src[i], all as if at once: it holds the same pages (each counted once more)
+ * and gives up those it held.  A dst that occurs twice takes the last pair.                                             */
+int bq_kv4_fork(const bq_kv4_pool* p, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+/* Empties sequences; a page nobody holds any more is free.  A slot may occur twice.                                     */
+int bq_kv4_free(const bq_kv4_pool* p, const int32_t* slots, int64_t n, void* stream);
+/* Fills pool `to` (same shape but for n_pages, its own memory) with the pages that are held, in ascending order from 0, and
+ * with the tables, lengths and counts that go with them; `p` is unchanged, and so are the bytes of free pages of `to`.  If
+ * `to` has too few pages BQ_ERR_STATE is recorded and `to` is unchanged.                                                 */
+int bq_kv4_compact(const bq_kv4_pool* p, const bq_kv4_pool* to, void* stream);
+/* Quantises rows k, v (n_rows rows of kv_heads * head_dim elements, ldk / ldv elements apart, both even, aligned to two
+ * elements) into the pages of `layer`: scale = fp16(min(absmax * fp32(1/7), 65504)), code = clip(rint(x / scale), +-7)
+ * (bq_quantize divides by 7, which differs in the last bit now and then); a NaN makes its group NaN.  Pages are written whether or not other sequences hold them: call
+ * bq_kv4_extend first, once for all layers.                                                                              */
+int bq_kv4_append(const bq_kv4_pool* p, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int dtype,
+                  const int32_t* slots, const int32_t* pos, const int32_t* starts, int64_t B, int64_t n_rows, void* stream);
+/* bq_rope_kv_append for this cache: qkv fp32 [n_rows, (Hq + 2 * kv_heads) * head_dim]; every row is rotated by its own
+ * position, q -> q_out [n_rows, Hq, head_dim] in dtype; k and v are rounded to dtype and then quantised.                  */
+int bq_kv4_rope_append(const bq_kv4_pool* p, int layer, const float* qkv, void* q_out, int Hq, float rope_base, int dtype,
+                       const int32_t* slots, const int32_t* pos, const int32_t* starts, int64_t B, int64_t n_rows,
+                       void* stream);
+/* The reverse: k, v [n_rows, kv_heads, head_dim] = code * scale (exact in fp32) of the positions the rows stand for.      */
+int bq_kv4_gather(const bq_kv4_pool* p, int layer, void* k, void* v, int dtype, const int32_t* slots, const int32_t* pos,
+                  const int32_t* starts, int64_t B, int64_t n_rows, void* stream);
+/* out[n_rows, Hq, head_dim] = softmax(q . K^T / sqrt(head_dim)) . V over positions 0 .. own position of every row
+ * (causal), grouped-query heads.  Rows of q are ldq elements apart.  Rows of a sequence with pos < 0 are set to zero.
+ * work: bq_kv4_attention_work_bytes() of device scratch, 16-byte aligned, contents do not matter; calls that may
+ * overlap on the device need scratch of their own.                                                                       */
+int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype);
+int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq, void* out, int Hq, int dtype,
+                     const int32_t* slots, const int32_t* pos, const int32_t* starts, int64_t B, int64_t n_rows, void* work,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,419 @@
+"""Paged 4-bit KV cache on the GPU: rows in and out bit for bit, page bookkeeping against a restatement, attention against
+64 bits."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4 as okv
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def ints(x):
+    return torch.tensor(list(x), dtype=torch.int32, device="cuda")
+
+
+def starts_of(rows):
+    return ints(np.concatenate([[0], np.cumsum(rows)]))
+
+
+def make(layers=1, heads=1, D=64, n_pages=32, max_seqs=8, max_pages=16, page=16):
+    from chadslab_b200 import PagedKV4
+    return PagedKV4(layers, heads, D, n_pages=n_pages, max_seqs=max_seqs, max_pages=max_pages, page=page)
+
+
+def rows(rng, n, heads, D, dtype, scale=1.0):
+    x = torch.from_numpy(rng.normal(0, scale, (n, heads, D)).astype(np.float32)).cuda().to(DT[dtype])
+    return x
+
+
+def num(t):
+    return t.float().cpu().numpy()
+
+
+def status():
+    from chadslab_b200 import _lib
+    return _lib.lib().bq_status_poll()
+
+
+def fill(kv, layer, lens, rng, dtype="bf16", vscale=1.0):
+    """Sequences 0 .. len(lens) - 1 of the given lengths, in one call -> what the cache holds of each, in 64 bits."""
+    starts = starts_of(lens)
+    k, v = rows(rng, sum(lens), kv.kv_heads, kv.head_dim, dtype), rows(rng, sum(lens), kv.kv_heads, kv.head_dim, dtype, vscale)
+    pos = kv.extend(ints(range(len(lens))), starts)
+    assert pos.cpu().tolist() == [0] * len(lens)
+    kv.append(layer, k, v, None, pos, starts)
+    at = np.concatenate([[0], np.cumsum(lens)])
+    K, V = okv.held(num(k)), okv.held(num(v))
+    return [(K[at[b]:at[b + 1]], V[at[b]:at[b + 1]]) for b in range(len(lens))]
+
+
+def shuffle(kv, rng):
+    """Gives and takes back pages so that later sequences get theirs out of order."""
+    n = kv.n_pages
+    perm = torch.from_numpy(rng.permutation(n)).cuda()
+    kv.pages.random_(0, 256)                     # free pages hold anything: NaN and infinite scales among it
+    kv.pages.copy_(kv.pages[perm])
+
+
+# ---- rows --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,heads,page", [(32, 1, 16), (64, 2, 32), (96, 3, 16), (128, 4, 64), (256, 5, 16)])
+def test_append_bytes_and_gather(cuda_lib, D, heads, page, dtype):
+    rng = np.random.default_rng(D + heads)
+    kv = make(2, heads, D, n_pages=24, page=page, max_pages=8)
+    kv.pages.fill_(0xA5)
+    lens = [page + 3, 16, 0, 1, 31]
+    starts = starts_of(lens)
+    k, v = rows(rng, sum(lens), heads, D, dtype), rows(rng, sum(lens), heads, D, dtype, 3.0)
+    k[0, 0, :32] = 0.0                           # a group of zeros
+    v[1, heads - 1, :32] = 1e30                  # one whose scale saturates
+    pos = kv.extend(None, starts, batch=len(lens))
+    kv.append(1, k, v, None, pos, starts)
+    gk, gv = kv.gather(1, None, pos, starts, rows=sum(lens))
+    wk, wv = okv.held(num(k)).astype(np.float32), okv.held(num(v)).astype(np.float32)
+    assert np.array_equal(num(gk), wk) and np.array_equal(num(gv), wv)
+    bk, bv = kv.gather(1, None, pos, starts, rows=sum(lens), dtype=torch.bfloat16)
+    assert torch.equal(bk, gk.bfloat16()) and torch.equal(bv, gv.bfloat16())
+    # the bytes: whole blocks as documented, layer 0 and free pages untouched
+    pages = kv.pages.view(kv.n_pages, 2, heads, page // 16, -1).cpu().numpy()
+    assert (pages[:, 0] == 0xA5).all() and (pages[kv.refs.cpu().numpy() == 0] == 0xA5).all()
+    table, at = kv.tables.cpu().numpy(), np.concatenate([[0], np.cumsum(lens)])
+    for b, n in enumerate(lens):
+        for p in range(0, n - 15, 16):
+            for h in range(heads):
+                want = okv.block_bytes(num(k)[at[b] + p:at[b] + p + 16, h], num(v)[at[b] + p:at[b] + p + 16, h])
+                assert np.array_equal(pages[table[b, p // page], 1, h, p % page // 16], want)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_append_in_steps_equals_append_at_once(cuda_lib, dtype):
+    """Row by row, in odd pieces and at once: the same bytes; a piece leaves its neighbours' bytes alone."""
+    rng = np.random.default_rng(1)
+    D, heads, total = 96, 2, 53
+    k, v = rows(rng, total, heads, D, dtype), rows(rng, total, heads, D, dtype)
+    got = []
+    for pieces in ([total], [1] * total, [5, 16, 1, 20, 11], [15, 2, 36]):
+        kv = make(1, heads, D, page=32)
+        kv.pages.zero_()
+        at = 0
+        for n in pieces:
+            pos = kv.extend([3], [0, n])
+            assert pos.tolist() == [at]
+            # every other piece comes as a strided slice of a wider buffer
+            wide = torch.zeros((n, 2 * heads + 1, D), dtype=k.dtype, device="cuda")
+            wide[:, :heads], wide[:, heads:2 * heads] = k[at:at + n], v[at:at + n]
+            kv.append(0, wide[:, :heads], wide[:, heads:2 * heads], [3], pos, [0, n])
+            at += n
+        got.append(kv.pages.clone())
+    for g in got[1:]:
+        assert torch.equal(got[0], g)
+
+
+def test_nan_and_infinity_in_rows(cuda_lib):
+    kv = make(1, 1, 64)
+    k = torch.ones((3, 1, 64), device="cuda")
+    k[1, 0, 5], k[2, 0, 40] = float("nan"), float("inf")
+    pos = kv.extend([0], [0, 3])
+    kv.append(0, k, k, [0], pos, [0, 3])
+    for g in kv.gather(0, [0], pos, [0, 3], rows=3):
+        g = num(g)[:, 0]
+        assert np.array_equal(g[0], okv.held(num(k)[0, 0]))
+        assert np.isnan(g[1, :32]).all() and not np.isnan(g[1, 32:]).any()      # the group of the NaN
+        assert g[2, 40] == 7 * 65504.0 and (g[2, 32:40] == 0).all()               # saturates; the rest of the group vanishes
+    # a row that cannot see them is not touched by them
+    q = torch.ones((3, 2, 64), device="cuda")
+    o = num(kv.attention(0, q, [0], pos, [0, 3]))
+    assert np.allclose(o[0], okv.held(num(k)[0, 0]), rtol=1e-5) and np.isnan(o[1]).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rowcounts", [[1, 1, 1], [17, 0, 33, 2]])
+def test_rope_append_is_rotation_then_append(cuda_lib, dtype, rowcounts):
+    """Same q and same cache as bq_rope_kv_append (dense cache) followed by append."""
+    from chadslab_b200 import _lib
+    rng = np.random.default_rng(4)
+    Hq, Hkv, D, base = 4, 2, 64, 10000.0
+    B, T = len(rowcounts), sum(rowcounts)
+    kv, ref = make(1, Hkv, D), make(1, Hkv, D)
+    kv.pages.zero_(), ref.pages.zero_()
+    before = [7, 16, 0, 30][:B]
+    for p in (kv, ref):
+        p.extend(None, starts_of(before), batch=B)
+    qkv = torch.from_numpy(rng.normal(0, 1, (T, (Hq + 2 * Hkv) * D)).astype(np.float32)).cuda()
+    starts = starts_of(rowcounts)
+    pos = kv.extend(None, starts, batch=B)
+    assert torch.equal(pos, ref.extend(None, starts, batch=B))
+    one = all(n == 1 for n in rowcounts)
+    q = kv.rope_append(0, qkv, Hq, base, None, pos, None if one else starts, dtype=DT[dtype])
+    S = 128
+    wq = torch.empty((T, Hq, D), dtype=DT[dtype], device="cuda")
+    wk, wv = (torch.zeros((T, Hkv, D), dtype=DT[dtype], device="cuda") for _ in range(2))
+    row = 0
+    for b, n in enumerate(rowcounts):
+        for i in range(n):
+            p = torch.tensor([before[b] + i], dtype=torch.int64, device="cuda")
+            kc, vc = (torch.zeros((1, S, Hkv, D), dtype=DT[dtype], device="cuda") for _ in range(2))
+            _lib.check(_lib.lib().bq_rope_kv_append(qkv[row].data_ptr(), p.data_ptr(), wq[row].data_ptr(), kc.data_ptr(), vc.data_ptr(), 1, Hq,
+                                                    Hkv, D, S, base, 0 if dtype == "f32" else 1, torch.cuda.current_stream().cuda_stream))
+            wk[row], wv[row] = kc[0, before[b] + i], vc[0, before[b] + i]
+            row += 1
+    ref.append(0, wk, wv, None, pos, starts)
+    assert torch.equal(q, wq) and torch.equal(kv.pages, ref.pages) and status() == 0
+
+
+# ---- pages -------------------------------------------------------------------------------------------------------------
+def same(kv, model):
+    assert np.array_equal(kv.tables.cpu().numpy(), model.tables)
+    assert np.array_equal(kv.lens.cpu().numpy(), model.lens)
+    assert np.array_equal(kv.refs.cpu().numpy(), model.refs)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_page_bookkeeping_against_restatement(cuda_lib, seed):
+    rng = np.random.default_rng(seed)
+    n_pages, seqs, most, page = [(20, 6, 5, 16), (300, 33, 9, 32), (17000, 40, 600, 16), (50, 12, 12, 64)][seed]
+    kv = make(2, 1, 32, n_pages=n_pages, max_seqs=seqs, max_pages=most, page=page)
+    model = okv.Pool(n_pages, seqs, most, page)
+    kv.pages.random_(0, 256)
+    for _ in range(60):
+        what = rng.integers(0, 5)
+        slots = rng.permutation(seqs)[:rng.integers(1, seqs + 1)].tolist()
+        if what <= 1:
+            n = [int(rng.choice([0, 1, 1, 2, page - 1, page, 3 * page + 1, most * page // 2])) for _ in slots]
+            before = kv.pages.clone()
+            pos = kv.extend(slots, np.concatenate([[0], np.cumsum(n)]).tolist())
+            want, copies = model.extend(slots, n)
+            assert pos.tolist() == want
+            for a, b in copies:
+                before[b] = before[a]
+            assert torch.equal(before, kv.pages)               # the copies are made, nothing else is written
+        elif what == 2:
+            dst = rng.integers(0, seqs, len(slots)).tolist()   # destinations may repeat and may be sources
+            kv.fork(slots, dst)
+            model.fork(slots, dst)
+        elif what == 3:
+            slots = slots[:max(1, len(slots) // 3)]
+            kv.free(slots + slots[:2])                         # the same slot twice
+            model.free(slots)
+        else:
+            live = int((model.refs > 0).sum())
+            room = live + int(rng.integers(1, 5))
+            to = make(2, 1, 32, n_pages=room, max_seqs=seqs, max_pages=most, page=page)
+            to.pages.fill_(7)
+            kv.compact(to)
+            moved, old = model.compact(room)
+            same(to, moved)
+            assert torch.equal(to.pages[:live], kv.pages[torch.from_numpy(old).cuda()]) and (to.pages[live:] == 7).all()
+        same(kv, model)
+    assert status() in (0, -1)           # -1: a sequence would have outgrown its table
+
+
+def test_extend_refusals(cuda_lib):
+    kv = make(1, 1, 32, n_pages=4, max_seqs=4, max_pages=3, page=16)
+    assert kv.extend([0, 1, 2], [0, 20, 40, 60]).tolist() == [0, 0, -1]      # 2 + 2 pages; none are left
+    assert kv.refs.tolist() == [1, 1, 1, 1] and kv.lens.tolist() == [20, 20, 0, 0] and status() == 0
+    assert kv.extend([1, 3, 0], [0, 12, 13, 13]).tolist() == [20, -1, 20] and status() == 0    # what needs no page is served
+    assert kv.extend([0, 0], [0, 1, 2]).tolist() == [20, -1] and status() == -1               # twice in one batch
+    assert kv.extend([0, 9, -1], [0, 1, 2, 3]).tolist() == [21, -1, -1] and status() == -1    # no such slot
+    assert kv.extend([0], [0, 40]).tolist() == [-1] and status() == -1                        # longer than the table
+    small = make(1, 1, 32, n_pages=3, max_seqs=4, max_pages=3, page=16)
+    kv.compact(small)
+    assert status() == -4 and small.lens.tolist() == [0] * 4 and small.refs.tolist() == [0] * 3
+    kv.free([7])
+    assert status() == -1
+    kv.fork([0, 9], [1, 2])
+    assert status() == -1 and kv.lens.tolist() == [22, 22, 0, 0] and kv.refs.tolist() == [2, 2, 0, 0]
+    # an append or attention that names a place outside the pool takes no part
+    k = torch.ones((2, 1, 32), device="cuda")
+    kept = kv.pages.clone()
+    kv.append(0, k, k, [9, 0], [0, 48])
+    assert torch.equal(kept, kv.pages) and status() == -1
+    kv.append(0, k, k, [3, 2], [0, 0])                                        # sequences without pages
+    assert torch.equal(kept, kv.pages) and status() == -1
+    o = kv.attention(0, torch.ones((2, 1, 32), device="cuda"), [9, 0], [3, -1])
+    assert (o == 0).all() and status() == -1
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------------
+def bound(o, mag, size, V, dtype):
+    """Per element.  fp32: queries and weights are held in 22 bits or more (2^-22 relative to every product), sums in fp32.
+    A score's sum has D products in at most 16 dependent additions on any path (a matrix instruction's 16 products count as
+    two, groups of 32 are added one after the other, lanes pairwise), each off by up to 2^-24 of the sum of |q k|: the
+    score is off by at most (2^-22 + 16 * 2^-24) * sum |q k| / sqrt(D), which moves every weight by that share, numerator
+    and denominator; exp2 and the division add a few 2^-23.  bf16: weights (times a scale) are rounded to fp16 twice
+    (2^-11 each) and the result once (2^-8 of itself).  Weights far below the largest, which is held as 2^11 or more, are
+    lost: a weight, and its product with a scale, is off by up to 2^-25 (fp32: the 2^-36 of its second half), times a code
+    of at most 7 or a value."""
+    lost = len(V) * 2.0 ** (-36 if dtype == "bf16" else -47) * (7.0 + np.abs(V).max())
+    score = 2.0 * size * (2.0 ** -22 + 16 * 2.0 ** -24)
+    if dtype == "f32":
+        return (2.0 ** -20 + score) * mag + lost
+    return (2 * 2.0 ** -11 + 2.0 ** -20 + score) * mag * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(o) + lost
+
+
+def check(kv, layer, data, lens, new, Hq, dtype, rng, q_scale=1.5, strided=False):
+    """Attention of the last new[b] rows of every sequence against 64 bits."""
+    T, D = sum(new), kv.head_dim
+    q = rows(rng, T, Hq, D, dtype, q_scale)
+    if strided:
+        wide = torch.zeros((T, Hq + 3, D), dtype=q.dtype, device="cuda")
+        wide[:, :Hq] = q
+        q = wide[:, :Hq]
+    pos = [n - m for n, m in zip(lens, new)]
+    one = all(m == 1 for m in new)
+    out = kv.attention(layer, q, ints(range(len(lens))), ints(pos), None if one else starts_of(new))
+    at = np.concatenate([[0], np.cumsum(new)])
+    for b in range(len(lens)):
+        if new[b] == 0:
+            continue
+        o, mag, size = okv.attention(num(q)[at[b]:at[b + 1]], data[b][0], data[b][1], pos[b])
+        err = np.abs(num(out)[at[b]:at[b + 1]] - o)
+        tol = bound(o, mag, size, data[b][1], dtype)
+        assert (err <= tol).all(), f"sequence {b} (len {lens[b]}): {np.nanmax(err / np.maximum(tol, 1e-300)):.2f} x the bound"
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,Hkv,rep", [(32, 2, 1), (32, 1, 16), (64, 2, 1), (64, 1, 4), (64, 3, 8), (96, 2, 3), (128, 2, 1), (128, 2, 2),
+                                       (128, 1, 4), (128, 2, 8), (128, 1, 16), (128, 1, 5), (160, 2, 2), (192, 1, 1), (224, 1, 6), (256, 2, 1),
+                                       (256, 1, 2), (256, 1, 3), (256, 1, 8), (256, 1, 17)])
+def test_decode_attention(cuda_lib, D, Hkv, rep, dtype):
+    rng = np.random.default_rng(D * 100 + Hkv * 10 + rep)
+    kv = make(2, Hkv, D, n_pages=150, max_seqs=9, max_pages=40, page=16)
+    shuffle(kv, rng)
+    lens = [1, 2, 15, 16, 17, 63, 65, 300, 129]
+    data = fill(kv, 1, lens, rng, dtype)
+    check(kv, 1, data, lens, [1] * len(lens), Hkv * rep, dtype, rng)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,Hkv,rep,page", [(64, 1, 2, 64), (128, 2, 4, 32), (256, 1, 1, 128), (256, 1, 8, 16), (96, 2, 1, 64)])
+def test_chunk_attention(cuda_lib, D, Hkv, rep, page, dtype):
+    """Chunks behind context, whole prompts, single tokens and sequences without rows in one batch."""
+    rng = np.random.default_rng(D + rep)
+    lens, new = [70, 33, 200, 5, 64, 1], [17, 33, 1, 0, 30, 1]
+    kv = make(1, Hkv, D, n_pages=64, max_pages=16, page=page)
+    shuffle(kv, rng)
+    data = fill(kv, 0, lens, rng, dtype)
+    check(kv, 0, data, lens, new, Hkv * rep, dtype, rng, strided=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,Hkv,rep", [(64, 1, 1), (128, 1, 8), (256, 2, 1)])
+def test_long_context_attention(cuda_lib, D, Hkv, rep, dtype):
+    rng = np.random.default_rng(9)
+    lens = [20011, 3, 4097]
+    kv = make(1, Hkv, D, n_pages=400, max_seqs=4, max_pages=320, page=64)
+    shuffle(kv, rng)
+    data = fill(kv, 0, lens, rng, dtype)
+    check(kv, 0, data, lens, [1, 1, 1], Hkv * rep, dtype, rng)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("q_scale,vscale", [(12.0, 1.0), (1e-3, 1e-3), (3.0, 2000.0), (1e4, 1.0), (0.0, 50.0)])
+def test_attention_ranges(cuda_lib, q_scale, vscale, dtype):
+    """Peaked and flat weights, values far below and above one (whose scales leave the range that fp16 weights have)."""
+    rng = np.random.default_rng(11)
+    lens = [700, 40]
+    kv = make(1, 2, 128, n_pages=64, max_pages=60, page=16)
+    shuffle(kv, rng)
+    data = fill(kv, 0, lens, rng, dtype, vscale)
+    check(kv, 0, data, lens, [1, 1], 4, dtype, rng, q_scale)
+
+
+def test_attention_rows_of_nobody(cuda_lib):
+    """Rows behind the last sequence stay as they were, rows of a refused sequence are zero."""
+    rng = np.random.default_rng(2)
+    kv = make(1, 2, 64)
+    fill(kv, 0, [20, 9, 30], rng)
+    q = rows(rng, 9, 4, 64, "bf16")
+    out = torch.full((9, 4, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    kv.attention(0, q, [0, 1, 2], [18, -1, 27], [0, 2, 4, 7], out=out)
+    o = num(out)
+    assert (o[7:] == 5).all() and (o[2:4] == 0).all() and np.isfinite(o).all() and (o[:2] != 5).any() and (o[4:7] != 5).any()
+    assert kv.attention(0, q[:0], [], []).shape == (0, 4, 64)
+
+
+def test_calls_repeat_bit_for_bit_and_streams(cuda_lib):
+    rng = np.random.default_rng(3)
+    kv = make(1, 2, 128, n_pages=200, max_pages=100, page=16)
+    fill(kv, 0, [1500, 800], rng)
+    q = rows(rng, 2, 8, 128, "bf16")
+    slots, pos = ints([0, 1]), ints([1499, 799])
+    ref = kv.attention(0, q, slots, pos)
+    torch.cuda.synchronize()
+    outs = []
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:                            # at the same time on several streams: every call has scratch of its own
+        with torch.cuda.stream(s):
+            outs += [kv.attention(0, q, slots, pos) for _ in range(5)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(ref, o) for o in outs)
+
+
+def test_serving_run_in_a_graph(cuda_lib):
+    """Prompts, a fork of one of them, decode steps replayed from a captured graph, one sequence leaves, the pool is
+    compacted: at every step what 64 bits say."""
+    rng = np.random.default_rng(5)
+    L, Hkv, rep, D, steps = 2, 2, 2, 64, 20
+    kv = make(L, Hkv, D, n_pages=40, max_seqs=4, max_pages=8, page=16)
+    shuffle(kv, rng)
+    lens = [19, 40]
+    starts = starts_of(lens)
+    pos = kv.extend([0, 1], starts)
+    hist = [[None, None] for _ in range(L)]
+    K = [[[] for _ in range(3)] for _ in range(L)]
+    V = [[[] for _ in range(3)] for _ in range(L)]
+    for l in range(L):
+        k, v = rows(rng, sum(lens), Hkv, D, "bf16"), rows(rng, sum(lens), Hkv, D, "bf16")
+        kv.append(l, k, v, [0, 1], pos, starts)
+        for b, (a, e) in enumerate(((0, 19), (19, 59))):
+            K[l][b], V[l][b] = list(okv.held(num(k)[a:e])), list(okv.held(num(v)[a:e]))
+    kv.fork([0], [2])
+    for l in range(L):
+        K[l][2], V[l][2] = list(K[l][0]), list(V[l][0])
+    lens = [19, 40, 19]
+    slots = ints([0, 1, 2])
+    k, v = (torch.zeros((L, 3, Hkv, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q, out = (torch.zeros((L, 3, Hkv * rep, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+
+    def step():
+        at = kv.extend(slots)
+        for l in range(L):
+            kv.append(l, k[l], v[l], slots, at)
+            kv.attention(l, q[l], slots, at, out=out[l])
+
+    keep = [t.clone() for t in (kv.tables, kv.lens, kv.refs)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for t, s in zip((kv.tables, kv.lens, kv.refs), keep):
+        t.copy_(s)
+    for i in range(steps):
+        for t in (k, v, q):
+            t.copy_(torch.from_numpy(rng.normal(0, 1, tuple(t.shape)).astype(np.float32)))
+        graph.replay()
+        for l in range(L):
+            for b in range(3):
+                K[l][b].append(okv.held(num(k[l, b])))
+                V[l][b].append(okv.held(num(v[l, b])))
+                o, mag, size = okv.attention(num(q[l, b])[None], np.array(K[l][b]), np.array(V[l][b]), lens[b] + i)
+                assert (np.abs(num(out[l, b])[None] - o) <= bound(o, mag, size, np.array(V[l][b]), "bf16")).all(), (i, l, b)
+    assert kv.lens.tolist()[:3] == [n + steps for n in lens]
+    kv.free([1])
+    small = make(L, Hkv, D, n_pages=7, max_seqs=4, max_pages=8, page=16)
+    kv.compact(small)
+    assert small.lens.tolist() == [39, 0, 39, 0] and status() == 0
+    q1 = q[1, [0, 2]].contiguous()
+    a, b = (p.attention(1, q1, [0, 2], [38, 38]) for p in (kv, small))
+    assert torch.equal(a, b)
