@@ -9,8 +9,8 @@
 //   K tile: row = position (g, g + 8), k = dimension.   r0 = (g, low k), r1 = (g, high k), r2 = (g + 8, low), r3 = (g + 8, high)
 //   V tile: row = dimension (g, g + 8), k = position.   r0 = (g, low k), r1 = (g + 8, low k), r2 = (g, high), r3 = (g + 8, high)
 // In both the nibbles of one position fill whole bytes, so that appending a position never reads what is there.
-// A nibble n = code + 8 in bits 0-3 (r0, r2) is the fp16 subnormal n * 2^-24, in bits 4-7 (r1, r3) n * 2^-20: masking a word
-// IS the conversion to fp16.
+// A nibble n = code + 8 in bits 0-3 (r0, r2) is the fp16 subnormal n * 2^-24, in bits 4-7 (r1, r3) n * 2^-20, and with the
+// exponent of 1024 or-ed in 1024 + n or 1024 + 16 n.
 #pragma once
 #include "common.cuh"
 

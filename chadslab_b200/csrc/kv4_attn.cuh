@@ -1,0 +1,764 @@
+// Attention over the paged 4-bit KV cache on the warp-level tensor path (mma.sync m16n8k16, fp16 in, fp32 accumulate).
+//   o[i, h] = sum_p softmax_p(q[i, h] . K[p] / sqrt(D)) V[p],   p <= position of row i
+//
+// Bound: HBM.  A position costs 1.125 D bytes per KV head; the kernel streams them once per column tile, a column being
+// one (row, query head) of the KV head, and everything else stays in registers and shared memory.
+//
+// Codes to operands.  The codes lie in fragment order (kv4.cuh): a lane's 32-bit word is its whole A fragment of a 16 x 16
+// tile, one mask (and a shift for half of them) away from four pairs of codes.
+//   * Values, and keys of fp32 rows: w & 0x000F000F | 0x6400.. is a pair of fp16 numbers 1024 + n (n = code + 8), w &
+//     0x00F000F0 | 0x6400.. a pair 1024 + 16 n; one packed subtraction leaves the code, or 16 times the code, exactly.
+//   * Keys of bf16 rows: w & 0x000F000F IS a pair of fp16 subnormals n * 2^-24, w & 0x00F000F0 a pair n * 2^-20, and the +8 is
+//     taken off by starting the accumulator at -8 * sum q: five integer instructions for eight codes and nothing else.  The
+//     matrix unit aligns products by their exponents, which for a subnormal lie above its leading bit: a sum is good to about
+//     2^-17 of its largest term instead of 2^-24 (measured: fp32 rows lost their last bits to it).  A score needs no more
+//     for a bf16 result; for the values the start would be many times the result of a long context.
+// What carries 16 times as much (the high half of a tile's dimensions for keys, rows 8-15 for values) meets q / 16, or is
+// divided by 16 at the end.  A key group's scale multiplies its sum in fp32; the scale of (position, group) of the values
+// multiplies the weight before it becomes the B operand.
+// q is scaled per column by a power of two so that fp16 holds it exactly (bf16 has 8 bits); fp32 rows take two columns, the
+// value and its remainder times 2^11 (22 bits), and so do their weights.
+//
+// Few columns (one query head per KV head: one).  m16n8k16 has 8 columns, so NC < 8 columns leave room for 8 / NC groups side
+// by side: column n = group * NC + c of the B operand is zero outside its group's dimensions, one accumulator tile then holds
+// 8 / NC groups' sums, each still apart for its scale; weights times scales of 8 / NC groups share one B fragment likewise.
+//
+// Softmax runs in the exp2 domain with a reference R per column that lags behind the maximum: weights are 2^(s - R), R = max -
+// A, and R moves only when a weight would exceed 2^(A + 4) (A = 11: weights up to 2^15, 2^-24 is the smallest fp16).  A
+// drops when weight * scale overflows, i.e. for values far above one.
+//
+// Work.  The 64-position tiles of all (sequence, KV head, column tile) segments form one list that is cut into equal runs,
+// one per resident CTA: ragged batches and few long sequences fill the machine alike.  A warp takes every fourth block of 16
+// positions through its own ring of bulk copies (no barrier between warps inside a segment).  A segment that lies in one
+// run is finished there; one that is cut leaves partial states in the caller's scratch, which a second kernel merges in run
+// order.  Every result has one order of additions: repeated calls give the same bits.
+#pragma once
+#include "kv4.cuh"
+
+namespace bq {
+
+constexpr int KA_WARPS = 4;
+constexpr int KA_THREADS = KA_WARPS * 32;
+constexpr int KA_TILE = KA_WARPS * KV4_ROWS;          // positions of a tile: a block per warp
+constexpr int KA_MIN_TILES = 2;                       // a run is at least this long: its prologue and merge cost about a tile
+constexpr uint64_t KA_WAIT_NS = 2000000000ull;        // bound of the wait for a copy
+
+struct KaArgs {
+  Kv4View v;
+  const void* q;
+  void* out;
+  float* part;                                        // [runs][2][HC * (D + 2)]
+  int64_t ldq, n_rows;
+  const int32_t *slots, *pos, *starts;
+  int* status;
+  int B, Hq, rep;
+  int width, sl;                                      // columns of a tile; columns per (row, head): 1, or 2 for fp32 rows
+};
+
+// ---- the list of tiles ---------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int ka_col_tiles(const KaArgs& a, const Kv4Seq& s) {
+  return s.n > 0 && s.pos >= 0 ? (int)(((int64_t)s.n * a.rep * a.sl + a.width - 1) / a.width) : 0;
+}
+__device__ __forceinline__ int ka_end(const KaArgs& a, const Kv4Seq& s, int ct) {      // positions that column tile ct sees
+  const int rows = (int)((((int64_t)ct + 1) * a.width - 1) / (a.rep * a.sl)) + 1;
+  return s.pos + (rows < s.n ? rows : s.n);
+}
+__device__ __forceinline__ int ka_tiles(const KaArgs& a, const Kv4Seq& s, int ct) { return (ka_end(a, s, ct) + KA_TILE - 1) / KA_TILE; }
+__device__ __forceinline__ int64_t ka_head_tiles(const KaArgs& a, const Kv4Seq& s) {   // of one KV head of a sequence
+  const int cts = ka_col_tiles(a, s);
+  int64_t n = 0;
+  for (int ct = 0; ct < cts; ++ct) n += ka_tiles(a, s, ct);
+  return n;
+}
+__device__ __forceinline__ Kv4Seq ka_seq(const KaArgs& a, int b) { return kv4_seq(a.v, a.slots, a.pos, a.starts, b, a.n_rows, a.status); }
+
+struct KaPlace { int b, h, ct, tile; };               // a tile of the list
+struct KaScan {
+  int64_t part[KA_WARPS], total, per;
+  int64_t rem;
+  int b;
+};
+// inclusive sum of v over the CTA (all threads), *total = the sum of all
+__device__ __forceinline__ int64_t ka_scan(int64_t v, KaScan* sc, int64_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += o;
+  }
+  __syncthreads();
+  if (lane == 31) sc->part[warp] = v;
+  __syncthreads();
+  int64_t t = 0;
+#pragma unroll
+  for (int w = 0; w < KA_WARPS; ++w) {
+    if (w < warp) v += sc->part[w];
+    t += sc->part[w];
+  }
+  *total = t;
+  return v;
+}
+// Length of the list and of a run, and the place of the first tile of run `run` (false: the list ends before it).
+static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc, KaPlace* at, int64_t* total, int64_t* per) {
+  int64_t sum = 0, mine = 0, upto = 0, chunk;
+  for (int b0 = 0; b0 < a.B; b0 += KA_THREADS) {
+    const int b = b0 + (int)threadIdx.x;
+    mine = b < a.B ? ka_head_tiles(a, ka_seq(a, b)) * a.v.Hkv : 0;
+    upto = ka_scan(mine, sc, &chunk);
+    sum += chunk;
+  }
+  *total = sum;
+  *per = (sum + runs - 1) / runs;
+  if (*per < KA_MIN_TILES) *per = KA_MIN_TILES;
+  const int64_t lo = (int64_t)run * *per;
+  if (lo >= sum) return false;
+  int64_t before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += KA_THREADS) {
+    if (a.B > KA_THREADS) {                           // otherwise the sums of the loop above are still there
+      const int b = b0 + (int)threadIdx.x;
+      mine = b < a.B ? ka_head_tiles(a, ka_seq(a, b)) * a.v.Hkv : 0;
+      upto = ka_scan(mine, sc, &chunk);
+    }
+    const int64_t from = before + upto - mine;
+    if (lo >= from && lo < from + mine) { sc->b = b0 + (int)threadIdx.x; sc->rem = lo - from; }
+    before += chunk;
+    if (lo < before) break;
+  }
+  __syncthreads();
+  at->b = sc->b;
+  int64_t rem = sc->rem;
+  const Kv4Seq s = ka_seq(a, at->b);
+  const int64_t head = ka_head_tiles(a, s);
+  at->h = (int)(rem / head);
+  rem -= at->h * head;
+  int ct = 0;
+  for (int n; rem >= (n = ka_tiles(a, s, ct)); ++ct) rem -= n;
+  at->ct = ct;
+  at->tile = (int)rem;
+  return true;
+}
+
+// ---- copies ----------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t ka_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ka_bar_init(uint32_t bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void ka_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ bool ka_bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+static __device__ __noinline__ bool ka_bar_wait_long(uint32_t bar, uint32_t parity) {
+  uint64_t t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  do {
+    for (int i = 0; i < 1024; ++i)
+      if (ka_bar_test(bar, parity)) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  } while (t - t0 < KA_WAIT_NS);
+  return false;
+}
+// lane 0 polls, the warp follows
+__device__ __forceinline__ bool ka_bar_wait(uint32_t bar, uint32_t parity, int lane) {
+  bool ok = true;
+  if (lane == 0 && !ka_bar_test(bar, parity)) ok = ka_bar_wait_long(bar, parity);
+  return __shfl_sync(0xffffffffu, ok, 0);
+}
+
+// ---- arithmetic --------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void ka_mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t ka_transpose(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ka_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t ka_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 ka_half2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
+__device__ __forceinline__ uint32_t ka_pack(float lo, float hi) { return ka_bits(__floats2half2_rn(lo, hi)); }
+__device__ __forceinline__ uint32_t ka_mul2(uint32_t a, uint32_t b) { return ka_bits(__hmul2(ka_half2(a), ka_half2(b))); }
+__device__ __forceinline__ uint32_t ka_sub2(uint32_t a, uint32_t b) { return ka_bits(__hsub2(ka_half2(a), ka_half2(b))); }
+// codes of the low / high nibble of bytes 0 and 2 as fp16, the latter times 16: 1032 = 0x6408, 1152 = 0x6480
+__device__ __forceinline__ uint32_t ka_code(uint32_t w) { return ka_sub2(lop3_and_or(w, 0x000F000Fu, 0x64006400u), 0x64086408u); }
+__device__ __forceinline__ uint32_t ka_code16(uint32_t w) { return ka_sub2(lop3_and_or(w, 0x00F000F0u, 0x64006400u), 0x64806480u); }
+__device__ __forceinline__ float2 ka_q2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 ka_q2(const __nv_bfloat16* p) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+constexpr float KA_LO = 1.0f / 2048.0f;               // weight of the second column of an fp32 row
+
+// ---- variants ------------------------------------------------------------------------------------------------------------------
+template <typename T, int NG, int NC, int NT> struct KaCfg {
+  static_assert(NC == 8 || NT == 1, "several column tiles need full ones");
+  static constexpr int SL = sizeof(T) == 4 ? 2 : 1;
+  static constexpr int D = NG * GROUP;
+  static constexpr int GP = 8 / NC;                   // groups side by side in a fragment
+  static_assert(NG % GP == 0, "whole fragments");
+  static constexpr int NF = NG / GP;
+  static constexpr int W = NC * NT;                   // columns of a tile
+  static constexpr int HC = W / SL;
+  static_assert(W % SL == 0, "an fp32 row takes two columns");
+  static constexpr bool SUBNORMAL = SL == 1;          // keys as fp16 subnormals
+  static constexpr int BLK = kv4_block_bytes(D);
+  static constexpr int OSTR = D + 4;                  // row pitch of the merge buffer: a quad's columns hit different banks
+  // resident CTAs: what the accumulators (8 NG NT registers) and q (4 NG NT) leave of 64 K registers
+  static constexpr int CTAS = NG * NT <= 4 ? 4 : NG * NT <= 8 ? 3 : 2;
+  static constexpr int FIXED = HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + (int)sizeof(KaScan) + 512;
+  static constexpr int FIT = (233472 / CTAS - 1024 - FIXED) / (KA_WARPS * (BLK + 8));
+  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+  static_assert(STAGES >= 2, "the ring needs two stages");
+  static constexpr int SMEM = KA_WARPS * STAGES * (BLK + 8) + FIXED;
+};
+
+template <typename T, int NG, int NC, int NT>
+__global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_attention_kernel(const __grid_constant__ KaArgs a) {
+  using C = KaCfg<T, NG, NC, NT>;
+  constexpr int D = C::D, SL = C::SL, GP = C::GP, NF = C::NF, W = C::W, HC = C::HC, S = C::STAGES;
+  extern __shared__ __align__(128) uint8_t smem[];
+  // [warps][S][BLK] ring | [warps][S] barriers | merge buffer | reference and sum of every warp and column | scan
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + KA_WARPS * S * C::BLK);
+  float* s_o = reinterpret_cast<float*>(bars + KA_WARPS * S);
+  float* s_ref = s_o + HC * C::OSTR;
+  float* s_sum = s_ref + KA_WARPS * W;
+  KaScan* scan = reinterpret_cast<KaScan*>(s_sum + KA_WARPS * W);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * S * C::BLK;
+  const uint32_t bar0 = ka_smem(bars + warp * S);
+  if (lane < S) ka_bar_init(bar0 + lane * 8);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  pdl_launch_dependents();
+  pdl_wait();
+  __syncthreads();
+
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {          // rows of refused sequences are zero
+    const Kv4Seq s = ka_seq(a, b);
+    if (s.pos >= 0) continue;
+    T* o = static_cast<T*>(a.out) + (int64_t)s.row0 * a.Hq * D;
+    for (int64_t e = threadIdx.x; e < (int64_t)s.n * a.Hq * D; e += KA_THREADS) o[e] = from_float<T>(0.0f);
+  }
+
+  KaPlace at;
+  int64_t total, per;
+  if (!ka_locate(a, gridDim.x, blockIdx.x, scan, &at, &total, &per)) return;
+  const int64_t lo = (int64_t)blockIdx.x * per;
+  int64_t left = total - lo < per ? total - lo : per;          // tiles of this run that are still to do
+
+  Kv4Seq seq = ka_seq(a, at.b);
+  int end = ka_end(a, seq, at.ct), tiles = (end + KA_TILE - 1) / KA_TILE;
+  int cts = ka_col_tiles(a, seq);
+  uint32_t issued = 0, taken = 0;                              // blocks of this warp's ring so far
+  bool dead = false;
+  // block i of this warp in the current piece is tile first + i; the piece has `mine` of them
+  auto issue = [&](const int32_t* row, int h, int tile) {
+    const uint32_t st = issued % S;
+    if (lane == 0) {
+      const uint8_t* src = a.v.block(row, tile * KA_WARPS + warp, h);
+      if (!src) {                                              // no such page: recorded, the result is undefined
+        *(volatile int*)a.status = (int)BQ_ERR_ARG;
+        src = a.v.pages;
+      }
+      ka_bulk_load(ka_smem(ring + st * C::BLK), src, C::BLK, bar0 + st * 8);
+    }
+    ++issued;
+  };
+  int first = at.tile;
+  int last = (int)(tiles - first < left ? tiles : first + left);         // this piece: tiles first .. last - 1
+  const int32_t* row = a.v.tables + (int64_t)seq.slot * a.v.max_pages;
+  auto my_blocks = [&]() {
+    const int full = (end - warp * KV4_ROWS + KA_TILE - 1) / KA_TILE;    // tiles in which this warp has a block
+    const int n = (full < last ? full : last) - first;
+    return n > 0 ? n : 0;
+  };
+  int mine = my_blocks(), ahead = 0;                           // blocks of this piece: all, and requested
+  for (; ahead < S && ahead < mine; ++ahead) issue(row, at.h, first + ahead);
+
+  while (true) {
+    // ---- the columns: q as B fragments ------------------------------------------------------------------------------------
+    uint32_t bq[NT][2 * NG][2];
+    float start[NT][NF][2], kappa[NT][2];
+    int vis[NT][2];
+    const int cols = seq.n * a.rep * SL;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = NC < 8 ? g % NC : nt * 8 + g, gi = NC < 8 ? g / NC : 0;
+      const int col = at.ct * W + c, rh = col / SL, i = rh / a.rep;
+      const bool ok = col < cols;
+      const T* qp = static_cast<const T*>(a.q) + (ok ? (int64_t)(seq.row0 + i) * a.ldq + (int64_t)(at.h * a.rep + rh % a.rep) * D : 0) + 2 * t;
+      float big = 0.0f;
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = ok ? ka_q2(qp + (f * GP + gi) * 32 + k * 8) : make_float2(0.0f, 0.0f);
+          big = fmaxf(big, fmaxf(fabsf(x.x), fabsf(x.y)));
+        }
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1)
+        if (off < 4 || off >= 4 * NC) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+      int k2 = 13 - ((int)(__float_as_uint(big) >> 23) - 127);          // big * 2^k2 is in [2^13, 2^14)
+      k2 = k2 > 100 ? 100 : k2 < -100 ? -100 : k2;
+      const float up = __uint_as_float((uint32_t)(127 + k2) << 23);
+      const bool second = SL == 2 && (col & 1);
+      float sum[NF];
+#pragma unroll
+      for (int f = 0; f < NF; ++f) sum[f] = 0.0f;
+#pragma unroll
+      for (int G = 0; G < NG; ++G) {
+        const int f = G / GP;
+        const bool here = NC == 8 || G % GP == gi;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // k = 2 * tile + (high k): the high half meets codes that carry 16 times as much
+          float2 x = ok && here ? ka_q2(qp + G * 32 + k * 8) : make_float2(0.0f, 0.0f);
+          const float m = (k & 1) ? up * 0.0625f : up;
+          x.x *= m; x.y *= m;
+          if (second) {
+            x.x = (x.x - __half2float(__float2half_rn(x.x))) * 2048.0f;
+            x.y = (x.y - __half2float(__float2half_rn(x.y))) * 2048.0f;
+          }
+          const __half2 hx = __floats2half2_rn(x.x, x.y);
+          bq[nt][2 * G + (k >> 1)][k & 1] = ka_bits(hx);
+          const float2 back = __half22float2(hx);
+          sum[f] += (back.x + back.y) * ((k & 1) ? 16.0f : 1.0f);
+        }
+      }
+      // what the accumulator layout needs of columns 2t and 2t + 1
+      const float kap = __uint_as_float((uint32_t)(127 - k2) << 23) * ((C::SUBNORMAL ? 16777216.0f : 1.0f) * 1.4426950408889634f) * rsqrtf((float)D);
+      const int see = ok ? seq.pos + i : 0x7FFFFFFF;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        kappa[nt][j] = __shfl_sync(0xffffffffu, kap, (2 * t + j) * 4);
+        vis[nt][j] = __shfl_sync(0xffffffffu, see, (2 * t + j) * 4);
+      }
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        float z = sum[f];
+        z += __shfl_xor_sync(0xffffffffu, z, 1);
+        z += __shfl_xor_sync(0xffffffffu, z, 2);
+        z *= C::SUBNORMAL ? -8.0f / 16777216.0f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) start[nt][f][j] = __shfl_sync(0xffffffffu, z, (2 * t + j) * 4);
+      }
+    }
+    const int all_see = seq.pos + (int)((int64_t)at.ct * W / (a.rep * SL));        // every column sees positions up to here
+
+    // ---- the positions ----------------------------------------------------------------------------------------------------
+    float acc[NT][2 * NG][4], ref[NT][2], l[NT][2];
+    float A = 11.0f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nt][i][j] = 0.0f;
+      ref[nt][0] = ref[nt][1] = -3.0e38f;
+      l[nt][0] = l[nt][1] = 0.0f;
+    }
+    for (int i = 0; i < mine; ++i) {
+      const uint32_t st = taken % S;
+      const uint8_t* blk = ring + st * C::BLK;
+      if (!ka_bar_wait(bar0 + st * 8, (taken / S) & 1u, lane) && !dead) {
+        dead = true;                                           // a copy did not arrive: record it and go on with what is there
+        *(volatile int*)a.status = (int)BQ_ERR_TIMEOUT;
+      }
+      ++taken;
+      const int p0 = ((first + i) * KA_WARPS + warp) * KV4_ROWS;
+      // scores
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        float c[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          c[nt][0] = c[nt][2] = start[nt][f][0];
+          c[nt][1] = c[nt][3] = start[nt][f][1];
+        }
+#pragma unroll
+        for (int gi = 0; gi < GP; ++gi) {
+          const int G = f * GP + gi;
+          const uint2 w2 = *reinterpret_cast<const uint2*>(blk + G * 256 + lane * 8);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w = h ? w2.y : w2.x, u = w >> 8;
+            uint32_t r0, r1, r2, r3;
+            if (C::SUBNORMAL) {
+              r0 = w & 0x000F000Fu; r1 = w & 0x00F000F0u; r2 = u & 0x000F000Fu; r3 = u & 0x00F000F0u;
+            } else {
+              r0 = ka_code(w); r1 = ka_code16(w); r2 = ka_code(u); r3 = ka_code16(u);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) ka_mma(c[nt], r0, r2, r1, r3, bq[nt][2 * G + h][0], bq[nt][2 * G + h][1]);
+          }
+        }
+        const __half* ks = reinterpret_cast<const __half*>(blk + kv4_kscale_off(D));
+        const int Ga = NC == 8 ? f : NC == 4 ? f * 2 + (t >> 1) : NC == 2 ? f * 4 + t : f * 8 + 2 * t;      // group of column 2t
+        const float k0 = __half2float(ks[g * NG + Ga]), k1 = __half2float(ks[(g + 8) * NG + Ga]);
+        const float k0b = NC == 1 ? __half2float(ks[g * NG + Ga + 1]) : k0, k1b = NC == 1 ? __half2float(ks[(g + 8) * NG + Ga + 1]) : k1;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          s[nt][0] += k0 * c[nt][0];
+          s[nt][1] += k0b * c[nt][1];
+          s[nt][2] += k1 * c[nt][2];
+          s[nt][3] += k1b * c[nt][3];
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (NC == 1) {
+          s[nt][0] += s[nt][1];
+          s[nt][2] += s[nt][3];
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 1);
+            s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 2);
+            s[nt][j + 1] = s[nt][j];
+          }
+        } else if (NC < 8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (NC == 2) s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 1);
+            s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 2);
+          }
+        }
+        if (SL == 2) {
+          s[nt][0] = s[nt][1] = s[nt][0] + s[nt][1] * KA_LO;
+          s[nt][2] = s[nt][3] = s[nt][2] + s[nt][3] * KA_LO;
+        }
+      }
+      const bool masked = p0 + KV4_ROWS - 1 > all_see;         // positions past the end, or past a column's own
+      if (masked) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (p0 + g + (j >> 1) * 8 > vis[nt][j & 1]) s[nt][j] = -INFINITY;
+      }
+      // weights; wv = weight * scale of the values, the B fragments of the second product
+      float p[NT][4];
+      uint32_t wv[NT][NF][2];
+#pragma unroll 1
+      for (int tries = 0; tries < 8; ++tries) {
+        bool over = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            p[nt][j] = fmaf(s[nt][j], kappa[nt][j & 1], -ref[nt][j & 1]);
+            over |= p[nt][j] > A + 4.0f;
+          }
+        if (__any_sync(0xffffffffu, over)) {                   // the reference moves up to the maximum so far
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float m = fmaxf(s[nt][j], s[nt][j + 2]) * kappa[nt][j];
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              const float r = fmaxf(ref[nt][j], m - A), corr = ka_exp2(ref[nt][j] - r);
+              ref[nt][j] = r;
+              l[nt][j] *= corr;
+#pragma unroll
+              for (int x = 0; x < 2 * NG; ++x) { acc[nt][x][j] *= corr; acc[nt][x][j + 2] *= corr; }
+              p[nt][j] = fmaf(s[nt][j], kappa[nt][j], -r);
+              p[nt][j + 2] = fmaf(s[nt][j + 2], kappa[nt][j], -r);
+            }
+        }
+        __half2 top = __floats2half2_rn(0.0f, 0.0f);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[nt][j] = ka_exp2(p[nt][j]);
+          uint32_t m0, m1;                                     // rows g, g + 8: columns 2t, 2t + 1
+          if (SL == 1) {
+            m0 = ka_pack(p[nt][0], p[nt][1]);
+            m1 = ka_pack(p[nt][2], p[nt][3]);
+          } else {
+            const float h0 = __half2float(__float2half_rn(p[nt][0])), h1 = __half2float(__float2half_rn(p[nt][2]));
+            m0 = ka_pack(h0, (p[nt][0] - h0) * 2048.0f);
+            m1 = ka_pack(h1, (p[nt][2] - h1) * 2048.0f);
+          }
+          m0 = ka_transpose(m0);                               // column g: positions 2t, 2t + 1
+          m1 = ka_transpose(m1);                               //           positions 2t + 8, 2t + 9
+          if (SL == 1) {
+            const uint32_t live0 = masked ? __hne2_mask(ka_half2(m0), __floats2half2_rn(0.0f, 0.0f)) : 0xFFFFFFFFu;
+            const uint32_t live1 = masked ? __hne2_mask(ka_half2(m1), __floats2half2_rn(0.0f, 0.0f)) : 0xFFFFFFFFu;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+              const int G = f * GP + (NC < 8 ? g / NC : 0);
+              const uint2 vs = *reinterpret_cast<const uint2*>(blk + kv4_vscale_off(D) + G * 32 + t * 8);
+              // a scale behind the last position can be anything: no weight, no product
+              wv[nt][f][0] = ka_mul2(m0, vs.x) & live0;
+              wv[nt][f][1] = ka_mul2(m1, vs.y) & live1;
+              top = __hmax2(top, __hmax2(ka_half2(wv[nt][f][0]), ka_half2(wv[nt][f][1])));
+            }
+          } else {
+            // the partner lane holds the other half of the same weight: 22 bits times the scale, split again
+            const uint32_t o0 = __shfl_xor_sync(0xffffffffu, m0, 4), o1 = __shfl_xor_sync(0xffffffffu, m1, 4);
+            const bool odd = g & 1;
+            const float2 a0 = __half22float2(ka_half2(odd ? o0 : m0)), b0 = __half22float2(ka_half2(odd ? m0 : o0));
+            const float2 a1 = __half22float2(ka_half2(odd ? o1 : m1)), b1 = __half22float2(ka_half2(odd ? m1 : o1));
+            const float w4[4] = {a0.x + b0.x * KA_LO, a0.y + b0.y * KA_LO, a1.x + b1.x * KA_LO, a1.y + b1.y * KA_LO};
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+              const int G = f * GP + (NC < 8 ? g / NC : 0);
+              const uint2 vs = *reinterpret_cast<const uint2*>(blk + kv4_vscale_off(D) + G * 32 + t * 8);
+              const float2 va = __half22float2(ka_half2(vs.x)), vb = __half22float2(ka_half2(vs.y));
+              const float v4[4] = {va.x, va.y, vb.x, vb.y};
+              float z[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                z[j] = w4[j] == 0.0f ? 0.0f : w4[j] * v4[j];
+                const float h = __half2float(__float2half_rn(z[j]));
+                if (h > 60000.0f) top = __floats2half2_rn(65504.0f, 65504.0f);
+                z[j] = odd ? (z[j] - h) * 2048.0f : h;
+              }
+              wv[nt][f][0] = ka_pack(z[0], z[1]);
+              wv[nt][f][1] = ka_pack(z[2], z[3]);
+            }
+          }
+        }
+        if (!__any_sync(0xffffffffu, fmaxf(__low2float(top), __high2float(top)) > 60000.0f)) break;
+        // a weight times its scale leaves fp16: all weights become 16 times smaller
+        A -= 4.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            ref[nt][j] += 4.0f;
+            l[nt][j] *= 0.0625f;
+#pragma unroll
+            for (int x = 0; x < 2 * NG; ++x) { acc[nt][x][j] *= 0.0625f; acc[nt][x][j + 2] *= 0.0625f; }
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        l[nt][0] += p[nt][0] + p[nt][2];
+        l[nt][1] += p[nt][1] + p[nt][3];
+      }
+      // values
+#pragma unroll
+      for (int G = 0; G < NG; ++G) {
+        const uint2 w2 = *reinterpret_cast<const uint2*>(blk + kv4_v_off(D) + G * 256 + lane * 8);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w = h ? w2.y : w2.x, u = w >> 8;
+          const uint32_t r0 = ka_code(w), r1 = ka_code16(w), r2 = ka_code(u), r3 = ka_code16(u);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) ka_mma(acc[nt][2 * G + h], r0, r1, r2, r3, wv[nt][G / GP][0], wv[nt][G / GP][1]);
+        }
+      }
+      __syncwarp();                                            // the stage has been read by every lane
+      if (ahead < mine) { issue(row, at.h, first + ahead); ++ahead; }
+    }
+
+    // ---- where this run goes next: its first copies travel while this piece is merged ------------------------------------------
+    const KaPlace was = at;
+    const Kv4Seq was_seq = seq;
+    const bool begins = first == 0, ends = last == tiles;
+    left -= last - first;
+    if (left > 0) {
+      if (++at.ct >= cts) {
+        at.ct = 0;
+        if (++at.h >= a.v.Hkv) {
+          at.h = 0;
+          cts = 0;
+          while (cts == 0 && ++at.b < a.B) {                   // left > 0: there is one
+            seq = ka_seq(a, at.b);
+            cts = ka_col_tiles(a, seq);
+          }
+          if (cts == 0) left = 0;                              // (unless the batch changed under the call)
+          row = a.v.tables + (int64_t)seq.slot * a.v.max_pages;
+        }
+      }
+    }
+    if (left > 0) {
+      end = ka_end(a, seq, at.ct);
+      tiles = (end + KA_TILE - 1) / KA_TILE;
+      first = 0;
+      last = (int)(tiles < left ? tiles : left);
+      mine = my_blocks();
+      for (ahead = 0; ahead < S && ahead < mine; ++ahead) issue(row, at.h, ahead);
+    }
+
+    // ---- the four warps' states become one ---------------------------------------------------------------------------------------
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float z = l[nt][j];
+        z += __shfl_xor_sync(0xffffffffu, z, 4);
+        z += __shfl_xor_sync(0xffffffffu, z, 8);
+        z += __shfl_xor_sync(0xffffffffu, z, 16);
+        const int n = 2 * t + j;
+        if (g == 0 && n < NC) {
+          s_ref[warp * W + nt * 8 + n] = ref[nt][j];
+          s_sum[warp * W + nt * 8 + n] = z;
+        }
+      }
+    __syncthreads();
+    float corr[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int c = nt * 8 + (NC < 8 ? (2 * t + j) % NC : 2 * t + j);
+        float r = s_ref[c];
+#pragma unroll
+        for (int w = 1; w < KA_WARPS; ++w) r = fmaxf(r, s_ref[w * W + c]);
+        corr[nt][j] = ka_exp2(ref[nt][j] - r) * (SL == 2 && j ? KA_LO : 1.0f);
+      }
+#pragma unroll 1
+    for (int w = 0; w < KA_WARPS; ++w) {                       // one after the other: one order of additions
+      if (warp == w) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int G = 0; G < NG; ++G) {
+            const int n0 = 2 * t;                              // this lane's columns n0, n0 + 1; group G % GP owns NC of them
+            if (NC < 8 && (NC == 1 ? (n0 >> 1) != (G % GP) >> 1 : n0 / NC != G % GP)) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float* x = acc[nt][2 * G + h];
+              const int d = (2 * G + h) * 16 + g;
+              if (SL == 2) {
+                float* o = s_o + (nt * 4 + (NC < 8 ? n0 % NC : n0) / 2) * C::OSTR + d;
+                const float y0 = x[0] * corr[nt][0] + x[1] * corr[nt][1], y1 = (x[2] * corr[nt][0] + x[3] * corr[nt][1]) * 0.0625f;
+                o[0] = w ? o[0] + y0 : y0;
+                o[8] = w ? o[8] + y1 : y1;
+              } else if (NC == 1) {
+                float* o = s_o + d;
+                const float y0 = (G & 1 ? x[1] : x[0]) * corr[nt][0], y1 = (G & 1 ? x[3] : x[2]) * (corr[nt][0] * 0.0625f);
+                o[0] = w ? o[0] + y0 : y0;
+                o[8] = w ? o[8] + y1 : y1;
+              } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  float* o = s_o + (nt * 8 + (NC < 8 ? n0 % NC : n0) + j) * C::OSTR + d;
+                  const float y0 = x[j] * corr[nt][j], y1 = x[j + 2] * (corr[nt][j] * 0.0625f);
+                  o[0] = w ? o[0] + y0 : y0;
+                  o[8] = w ? o[8] + y1 : y1;
+                }
+              }
+            }
+          }
+      }
+      __syncthreads();
+    }
+    float* part = a.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * (HC * (D + 2));
+    const int heads = was_seq.n * a.rep;                       // (row, head) pairs of the sequence
+    for (int e = threadIdx.x; e < HC * D; e += KA_THREADS) {
+      const int hc = e / D, d = e % D, c = hc * SL;
+      float r = s_ref[c], z = 0.0f;
+#pragma unroll
+      for (int w = 1; w < KA_WARPS; ++w) r = fmaxf(r, s_ref[w * W + c]);
+#pragma unroll
+      for (int w = 0; w < KA_WARPS; ++w) z += s_sum[w * W + c] * ka_exp2(s_ref[w * W + c] - r);
+      const float o = s_o[hc * C::OSTR + d];
+      if (begins && ends) {
+        const int rh = was.ct * HC + hc;
+        if (rh < heads)
+          static_cast<T*>(a.out)[((int64_t)(was_seq.row0 + rh / a.rep) * a.Hq + was.h * a.rep + rh % a.rep) * D + d] = from_float<T>(o / z);
+      } else {
+        part[e] = o;
+        if (d == 0) { part[HC * D + 2 * hc] = r; part[HC * D + 2 * hc + 1] = z; }
+      }
+    }
+    if (left <= 0) break;
+    __syncthreads();                                           // the merge buffers are free again
+  }
+  if (dead) {                                                  // do not leave with copies in flight
+    for (; taken < issued; ++taken) ka_bar_wait(bar0 + taken % S * 8, (taken / S) & 1u, lane);
+  }
+}
+
+// Segments that were cut: one CTA row per run boundary; the first boundary inside a segment merges its pieces in run order.
+// grid: (runs, (row, head) pairs of a tile)
+template <typename T>
+__global__ void __launch_bounds__(KA_THREADS) kv4_attention_merge_kernel(const __grid_constant__ KaArgs a, int runs) {
+  __shared__ KaScan scan;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int run = blockIdx.x + 1, HC = a.width / a.sl, hc = blockIdx.y, D = a.v.D;
+  KaPlace at;
+  int64_t total, per;
+  if (!ka_locate(a, runs, run, &scan, &at, &total, &per)) return;
+  if (at.tile == 0 || at.tile > per) return;                   // not inside a segment / an earlier boundary is inside it too
+  const Kv4Seq seq = ka_seq(a, at.b);
+  const int64_t begin = run * per - at.tile, stop = begin + ka_tiles(a, seq, at.ct);
+  const int rh = at.ct * HC + hc;
+  if (rh >= seq.n * a.rep) return;
+  const int last = (int)((stop - 1) / per);                    // the segment lies in runs run - 1 .. last
+  const int64_t slot = (int64_t)HC * (D + 2);
+  const float* p0 = a.part + ((int64_t)(run - 1) * 2 + 1) * slot;
+  float r = p0[HC * D + 2 * hc];
+  for (int k = run; k <= last; ++k) r = fmaxf(r, a.part[(int64_t)k * 2 * slot + HC * D + 2 * hc]);
+  T* out = static_cast<T*>(a.out) + ((int64_t)(seq.row0 + rh / a.rep) * a.Hq + at.h * a.rep + rh % a.rep) * D;
+  for (int d = threadIdx.x; d < D; d += KA_THREADS) {
+    const float f0 = ka_exp2(p0[HC * D + 2 * hc] - r);
+    float z = p0[HC * D + 2 * hc + 1] * f0, o = p0[hc * D + d] * f0;
+    for (int k = run; k <= last; ++k) {
+      const float* p = a.part + (int64_t)k * 2 * slot;
+      const float f = ka_exp2(p[HC * D + 2 * hc] - r);
+      z += p[HC * D + 2 * hc + 1] * f;
+      o += p[hc * D + d] * f;
+    }
+    out[d] = from_float<T>(o / z);
+  }
+}
+
+// most runs of any variant, and most floats of a run's two partial states
+constexpr int KA_MAX_CTAS = 4, KA_MAX_WIDTH = 16;
+
+template <typename T, int NG, int NC, int NT>
+int ka_launch(KaArgs a, cudaStream_t s) {
+  using C = KaCfg<T, NG, NC, NT>;
+  static bool sized = false;
+  if (!sized) {
+    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    sized = true;
+  }
+  a.width = C::W;
+  a.sl = C::SL;
+  // a list cannot be longer than the tables allow
+  const double most = (double)a.B * a.v.Hkv * (double)((((int64_t)a.v.max_pages << a.v.page_log2) + KA_TILE - 1) / KA_TILE) *
+                      (double)((a.n_rows * a.rep * C::SL + C::W - 1) / C::W);
+  int64_t runs = (int64_t)sm_count() * C::CTAS;
+  if ((double)runs * KA_MIN_TILES > most) runs = ((int64_t)most + KA_MIN_TILES - 1) / KA_MIN_TILES;
+  BQ_CUDA(launch_chain(kv4_attention_kernel<T, NG, NC, NT>, dim3((unsigned)runs), dim3(KA_THREADS), C::SMEM, s, 1, a));
+  count_launch();
+  if (runs > 1) {
+    BQ_CUDA(launch_chain(kv4_attention_merge_kernel<T>, dim3((unsigned)(runs - 1), (unsigned)C::HC), dim3(KA_THREADS), 0, s, 1, a, (int)runs));
+    count_launch();
+  }
+  BQ_CUDA(cudaGetLastError());
+  return BQ_OK;
+}
+
+// one per head_dim (kv4_attn_*.cu): picks the variant for `cols` columns per sequence
+template <typename T, int NG> int ka_pick(const KaArgs& a, int64_t cols, cudaStream_t s);
+
+}  // namespace bq

@@ -245,12 +245,14 @@ def bound(o, mag, size, V, dtype):
     A score's sum has D products in at most 16 dependent additions on any path (a matrix instruction's 16 products count as
     two, groups of 32 are added one after the other, lanes pairwise), each off by up to 2^-24 of the sum of |q k|: the
     score is off by at most (2^-22 + 16 * 2^-24) * sum |q k| / sqrt(D), which moves every weight by that share, numerator
-    and denominator; exp2 and the division add a few 2^-23.  bf16: weights (times a scale) are rounded to fp16 twice
-    (2^-11 each) and the result once (2^-8 of itself).  Weights far below the largest, which is held as 2^11 or more, are
+    and denominator; exp2 and the division add a few 2^-23.  bf16: a key's
+    code is a subnormal fp16 n * 2^-24 with n < 16, whose products the matrix unit aligns as if they had their exponent's
+    whole 2^-14: up to 2^6 times coarser, i.e. 16 * 2^-18 in place of 16 * 2^-24; weights (times a scale) are rounded to
+    fp16 twice (2^-11 each) and the result once (2^-8 of itself).  Weights far below the largest, which is held as 2^11 or more, are
     lost: a weight, and its product with a scale, is off by up to 2^-25 (fp32: the 2^-36 of its second half), times a code
     of at most 7 or a value."""
     lost = len(V) * 2.0 ** (-36 if dtype == "bf16" else -47) * (7.0 + np.abs(V).max())
-    score = 2.0 * size * (2.0 ** -22 + 16 * 2.0 ** -24)
+    score = 2.0 * size * (2.0 ** -22 + 16 * 2.0 ** (-24 if dtype == "f32" else -18))
     if dtype == "f32":
         return (2.0 ** -20 + score) * mag + lost
     return (2 * 2.0 ** -11 + 2.0 ** -20 + score) * mag * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(o) + lost
