@@ -27,9 +27,9 @@
 // A, and R moves only when a weight would exceed 2^(A + 4) (A = 11: weights up to 2^15, 2^-24 is the smallest fp16).  A
 // drops when weight * scale overflows, i.e. for values far above one.
 //
-// Work.  The 64-position tiles of all (sequence, KV head, column tile) segments form one list that is cut into equal runs,
-// one per resident CTA: ragged batches and few long sequences fill the machine alike.  A warp takes every fourth block of 16
-// positions through its own ring of bulk copies (no barrier between warps inside a segment).  A segment that lies in one
+// Work.  The tiles (128 positions, or 64 where two steps of 32 per warp do not fit into shared memory) of all (sequence, KV head, column tile) segments form one list that is cut into equal runs,
+// one per resident CTA: ragged batches and few long sequences fill the machine alike.  A warp takes 32 (16) positions of every
+// tile through its own ring of bulk copies (no barrier between warps inside a segment).  A segment that lies in one
 // run is finished there; one that is cut leaves partial states in the caller's scratch, which a second kernel merges in run
 // order.  Every result has one order of additions: repeated calls give the same bits.
 #pragma once
@@ -39,8 +39,7 @@ namespace bq {
 
 constexpr int KA_WARPS = 4;
 constexpr int KA_THREADS = KA_WARPS * 32;
-constexpr int KA_TILE = KA_WARPS * KV4_ROWS;          // positions of a tile: a block per warp
-constexpr int KA_MIN_TILES = 2;                       // a run is at least this long: its prologue and merge cost about a tile
+constexpr int KA_MIN_TILES = 1;                       // a run is at least this long
 constexpr uint64_t KA_WAIT_NS = 2000000000ull;        // bound of the wait for a copy
 
 struct KaArgs {
@@ -53,6 +52,7 @@ struct KaArgs {
   int* status;
   int B, Hq, rep;
   int width, sl;                                      // columns of a tile; columns per (row, head): 1, or 2 for fp32 rows
+  int tile;                                           // positions of a tile: 16 or 32 per warp
 };
 
 // ---- the list of tiles ---------------------------------------------------------------------------------------------------
@@ -63,7 +63,7 @@ __device__ __forceinline__ int ka_end(const KaArgs& a, const Kv4Seq& s, int ct) 
   const int rows = (int)((((int64_t)ct + 1) * a.width - 1) / (a.rep * a.sl)) + 1;
   return s.pos + (rows < s.n ? rows : s.n);
 }
-__device__ __forceinline__ int ka_tiles(const KaArgs& a, const Kv4Seq& s, int ct) { return (ka_end(a, s, ct) + KA_TILE - 1) / KA_TILE; }
+__device__ __forceinline__ int ka_tiles(const KaArgs& a, const Kv4Seq& s, int ct) { return (ka_end(a, s, ct) + a.tile - 1) / a.tile; }
 __device__ __forceinline__ int64_t ka_head_tiles(const KaArgs& a, const Kv4Seq& s) {   // of one KV head of a sequence
   const int cts = ka_col_tiles(a, s);
   int64_t n = 0;
@@ -141,8 +141,10 @@ static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc,
 // ---- copies ----------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t ka_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ka_bar_init(uint32_t bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void ka_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+__device__ __forceinline__ void ka_bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ka_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
                "r"(bar)
                : "memory");
@@ -168,11 +170,12 @@ static __device__ __noinline__ bool ka_bar_wait_long(uint32_t bar, uint32_t pari
   } while (t - t0 < KA_WAIT_NS);
   return false;
 }
-// lane 0 polls, the warp follows
+// lane 0 polls, the warp follows; false (to lane 0): the copy did not arrive in time
 __device__ __forceinline__ bool ka_bar_wait(uint32_t bar, uint32_t parity, int lane) {
   bool ok = true;
   if (lane == 0 && !ka_bar_test(bar, parity)) ok = ka_bar_wait_long(bar, parity);
-  return __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok;
 }
 
 // ---- arithmetic --------------------------------------------------------------------------------------------------------------
@@ -223,25 +226,30 @@ template <typename T, int NG, int NC, int NT> struct KaCfg {
   // resident CTAs: what the accumulators (8 NG NT registers) and q (4 NG NT) leave of 64 K registers
   static constexpr int CTAS = NG * NT <= 4 ? 4 : NG * NT <= 8 ? 3 : 2;
   static constexpr int FIXED = HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + (int)sizeof(KaScan) + 512;
-  static constexpr int FIT = (233472 / CTAS - 1024 - FIXED) / (KA_WARPS * (BLK + 8));
-  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+  // a warp's step, one stage of its ring: two blocks if the ring then has two stages, else one
+  static constexpr int ROOM = (233472 / CTAS - 1024 - FIXED) / KA_WARPS;
+  static constexpr int STEP = ROOM / (2 * BLK + 8) >= 2 ? 2 : 1;
+  static constexpr int TILE = KA_WARPS * STEP * KV4_ROWS;
+  static constexpr int STAGE = STEP * BLK;
+  static constexpr int STAGES = ROOM / (STAGE + 8) >= 4 ? 4 : ROOM / (STAGE + 8);
   static_assert(STAGES >= 2, "the ring needs two stages");
-  static constexpr int SMEM = KA_WARPS * STAGES * (BLK + 8) + FIXED;
+  static constexpr int SMEM = KA_WARPS * STAGES * (STAGE + 8) + FIXED;
+  static constexpr int U = NT == 1 && NF * NG <= 16 ? STEP : 1;  // blocks whose scores and weights are held at a time
 };
 
 template <typename T, int NG, int NC, int NT>
 __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   using C = KaCfg<T, NG, NC, NT>;
-  constexpr int D = C::D, SL = C::SL, GP = C::GP, NF = C::NF, W = C::W, HC = C::HC, S = C::STAGES;
+  constexpr int D = C::D, SL = C::SL, GP = C::GP, NF = C::NF, W = C::W, HC = C::HC, S = C::STAGES, U = C::U, STEP = C::STEP, TILE = C::TILE;
   extern __shared__ __align__(128) uint8_t smem[];
-  // [warps][S][BLK] ring | [warps][S] barriers | merge buffer | reference and sum of every warp and column | scan
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + KA_WARPS * S * C::BLK);
+  // [warps][S][STAGE] ring | [warps][S] barriers | merge buffer | reference and sum of every warp and column | scan
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + KA_WARPS * S * C::STAGE);
   float* s_o = reinterpret_cast<float*>(bars + KA_WARPS * S);
   float* s_ref = s_o + HC * C::OSTR;
   float* s_sum = s_ref + KA_WARPS * W;
   KaScan* scan = reinterpret_cast<KaScan*>(s_sum + KA_WARPS * W);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * S * C::BLK;
+  uint8_t* ring = smem + warp * S * C::STAGE;
   const uint32_t bar0 = ka_smem(bars + warp * S);
   if (lane < S) ka_bar_init(bar0 + lane * 8);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -263,33 +271,45 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
   int64_t left = total - lo < per ? total - lo : per;          // tiles of this run that are still to do
 
   Kv4Seq seq = ka_seq(a, at.b);
-  int end = ka_end(a, seq, at.ct), tiles = (end + KA_TILE - 1) / KA_TILE;
+  int end = ka_end(a, seq, at.ct), tiles = (end + TILE - 1) / TILE;
   int cts = ka_col_tiles(a, seq);
-  uint32_t issued = 0, taken = 0;                              // blocks of this warp's ring so far
+  uint32_t put = 0, take = 0, phase = 0;                       // stage to fill next, stage to read next and its parity
+  int flying = 0;                                              // copies under way
   bool dead = false;
-  // block i of this warp in the current piece is tile first + i; the piece has `mine` of them
-  auto issue = [&](const int32_t* row, int h, int tile) {
-    const uint32_t st = issued % S;
+  const int pb = a.v.page_blocks_log2();
+  const int32_t* row = a.v.tables + (int64_t)seq.slot * a.v.max_pages;
+  // requests this warp's blocks of a tile; `blocks` = blocks of the segment
+  auto issue = [&](const int32_t* row, int h, int tile, int blocks) {
     if (lane == 0) {
-      const uint8_t* src = a.v.block(row, tile * KA_WARPS + warp, h);
-      if (!src) {                                              // no such page: recorded, the result is undefined
-        *(volatile int*)a.status = (int)BQ_ERR_ARG;
-        src = a.v.pages;
-      }
-      ka_bulk_load(ka_smem(ring + st * C::BLK), src, C::BLK, bar0 + st * 8);
+      const uint32_t bar = bar0 + put * 8, dst = ka_smem(ring + put * C::STAGE);
+      const int b0 = (tile * KA_WARPS + warp) * STEP, n = blocks - b0 < STEP ? blocks - b0 : STEP;
+      ka_bar_expect(bar, n * C::BLK);
+      auto load = [&](int blk, int count, uint32_t to) {
+        uint32_t id = (uint32_t)row[blk >> pb];
+        if (id >= (uint64_t)a.v.n_pages) {                     // no such page: recorded, the result is undefined
+          *(volatile int*)a.status = (int)BQ_ERR_ARG;
+          id = 0;
+        }
+        const uint32_t in = ((uint32_t)h << pb) + (blk & ((1 << pb) - 1));
+        ka_bulk_load(to, a.v.pages + (int64_t)id * a.v.page_bytes + (a.v.layer_off + (int64_t)in * C::BLK), count * C::BLK, bar);
+      };
+      if (pb > 0) load(b0, n, dst);                            // a page holds both
+      else
+        for (int j = 0; j < n; ++j) load(b0 + j, 1, dst + j * C::BLK);
     }
-    ++issued;
+    put = put + 1 == S ? 0 : put + 1;
+    ++flying;
   };
   int first = at.tile;
   int last = (int)(tiles - first < left ? tiles : first + left);         // this piece: tiles first .. last - 1
-  const int32_t* row = a.v.tables + (int64_t)seq.slot * a.v.max_pages;
-  auto my_blocks = [&]() {
-    const int full = (end - warp * KV4_ROWS + KA_TILE - 1) / KA_TILE;    // tiles in which this warp has a block
+  int blocks = (end + KV4_ROWS - 1) / KV4_ROWS;
+  auto my_steps = [&]() {                                      // tiles of the piece in which this warp has a block
+    const int full = (blocks - warp * STEP + KA_WARPS * STEP - 1) / (KA_WARPS * STEP);
     const int n = (full < last ? full : last) - first;
     return n > 0 ? n : 0;
   };
-  int mine = my_blocks(), ahead = 0;                           // blocks of this piece: all, and requested
-  for (; ahead < S && ahead < mine; ++ahead) issue(row, at.h, first + ahead);
+  int mine = my_steps(), ahead = 0;                            // steps of this piece: all, and requested
+  for (; ahead < S && ahead < mine; ++ahead) issue(row, at.h, first + ahead, blocks);
 
   while (true) {
     // ---- the columns: q as B fragments ------------------------------------------------------------------------------------
@@ -374,205 +394,225 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
       l[nt][0] = l[nt][1] = 0.0f;
     }
     for (int i = 0; i < mine; ++i) {
-      const uint32_t st = taken % S;
-      const uint8_t* blk = ring + st * C::BLK;
-      if (!ka_bar_wait(bar0 + st * 8, (taken / S) & 1u, lane) && !dead) {
-        dead = true;                                           // a copy did not arrive: record it and go on with what is there
+      const uint8_t* stage = ring + take * C::STAGE;
+      if (!ka_bar_wait(bar0 + take * 8, phase, lane)) {        // a copy did not arrive: record it and go on with what is there
+        dead = true;
         *(volatile int*)a.status = (int)BQ_ERR_TIMEOUT;
       }
-      ++taken;
-      const int p0 = ((first + i) * KA_WARPS + warp) * KV4_ROWS;
-      // scores
-      float s[NT][4];
+      const int step0 = ((first + i) * KA_WARPS + warp) * STEP * KV4_ROWS;
+#pragma unroll 1
+      for (int u0 = 0; u0 < STEP; u0 += U) {
+        if (U == 1 && u0 && step0 + KV4_ROWS >= end) break;    // no second block
+        const uint8_t* blk0 = stage + u0 * C::BLK;
+        const int p0 = step0 + u0 * KV4_ROWS;
+        // scores
+        float s[U][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < U; ++u) {
+          const uint8_t* blk = blk0 + u * C::BLK;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
+          for (int f = 0; f < NF; ++f) {
+            float c[NT][4];
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        float c[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          c[nt][0] = c[nt][2] = start[nt][f][0];
-          c[nt][1] = c[nt][3] = start[nt][f][1];
-        }
-#pragma unroll
-        for (int gi = 0; gi < GP; ++gi) {
-          const int G = f * GP + gi;
-          const uint2 w2 = *reinterpret_cast<const uint2*>(blk + G * 256 + lane * 8);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t w = h ? w2.y : w2.x, u = w >> 8;
-            uint32_t r0, r1, r2, r3;
-            if (C::SUBNORMAL) {
-              r0 = w & 0x000F000Fu; r1 = w & 0x00F000F0u; r2 = u & 0x000F000Fu; r3 = u & 0x00F000F0u;
-            } else {
-              r0 = ka_code(w); r1 = ka_code16(w); r2 = ka_code(u); r3 = ka_code16(u);
+            for (int nt = 0; nt < NT; ++nt) {
+              c[nt][0] = c[nt][2] = start[nt][f][0];
+              c[nt][1] = c[nt][3] = start[nt][f][1];
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) ka_mma(c[nt], r0, r2, r1, r3, bq[nt][2 * G + h][0], bq[nt][2 * G + h][1]);
+            for (int gi = 0; gi < GP; ++gi) {
+              const int G = f * GP + gi;
+              const uint2 w2 = *reinterpret_cast<const uint2*>(blk + G * 256 + lane * 8);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t w = h ? w2.y : w2.x, x = w >> 8;
+                uint32_t r0, r1, r2, r3;
+                if (C::SUBNORMAL) {
+                  r0 = w & 0x000F000Fu; r1 = w & 0x00F000F0u; r2 = x & 0x000F000Fu; r3 = x & 0x00F000F0u;
+                } else {
+                  r0 = ka_code(w); r1 = ka_code16(w); r2 = ka_code(x); r3 = ka_code16(x);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) ka_mma(c[nt], r0, r2, r1, r3, bq[nt][2 * G + h][0], bq[nt][2 * G + h][1]);
+              }
+            }
+            // scales of rows g and g + 8: of the column's group, or (NC == 1) of the two columns' groups
+            const __half* ks = reinterpret_cast<const __half*>(blk + kv4_kscale_off(D));
+            float2 k0, k1;
+            if (NC == 1) {
+              k0 = __half22float2(*reinterpret_cast<const __half2*>(ks + g * NG + f * 8 + 2 * t));
+              k1 = __half22float2(*reinterpret_cast<const __half2*>(ks + (g + 8) * NG + f * 8 + 2 * t));
+            } else {
+              const int G = NC == 8 ? f : NC == 4 ? f * 2 + (t >> 1) : f * 4 + t;
+              k0.x = k0.y = __half2float(ks[g * NG + G]);
+              k1.x = k1.y = __half2float(ks[(g + 8) * NG + G]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              s[u][nt][0] = f ? fmaf(k0.x, c[nt][0], s[u][nt][0]) : k0.x * c[nt][0];
+              s[u][nt][1] = f ? fmaf(k0.y, c[nt][1], s[u][nt][1]) : k0.y * c[nt][1];
+              s[u][nt][2] = f ? fmaf(k1.x, c[nt][2], s[u][nt][2]) : k1.x * c[nt][2];
+              s[u][nt][3] = f ? fmaf(k1.y, c[nt][3], s[u][nt][3]) : k1.y * c[nt][3];
+            }
           }
         }
-        const __half* ks = reinterpret_cast<const __half*>(blk + kv4_kscale_off(D));
-        const int Ga = NC == 8 ? f : NC == 4 ? f * 2 + (t >> 1) : NC == 2 ? f * 4 + t : f * 8 + 2 * t;      // group of column 2t
-        const float k0 = __half2float(ks[g * NG + Ga]), k1 = __half2float(ks[(g + 8) * NG + Ga]);
-        const float k0b = NC == 1 ? __half2float(ks[g * NG + Ga + 1]) : k0, k1b = NC == 1 ? __half2float(ks[(g + 8) * NG + Ga + 1]) : k1;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[nt][0] += k0 * c[nt][0];
-          s[nt][1] += k0b * c[nt][1];
-          s[nt][2] += k1 * c[nt][2];
-          s[nt][3] += k1b * c[nt][3];
-        }
-      }
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (NC == 1) {
-          s[nt][0] += s[nt][1];
-          s[nt][2] += s[nt][3];
+          for (int nt = 0; nt < NT; ++nt) {
+            float* z = s[u][nt];
+            if (NC == 1) {
+              z[0] += z[1];
+              z[2] += z[3];
 #pragma unroll
-          for (int j = 0; j < 4; j += 2) {
-            s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 1);
-            s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 2);
-            s[nt][j + 1] = s[nt][j];
+              for (int j = 0; j < 4; j += 2) {
+                z[j] += __shfl_xor_sync(0xffffffffu, z[j], 1);
+                z[j] += __shfl_xor_sync(0xffffffffu, z[j], 2);
+                z[j + 1] = z[j];
+              }
+            } else if (NC < 8) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (NC == 2) z[j] += __shfl_xor_sync(0xffffffffu, z[j], 1);
+                z[j] += __shfl_xor_sync(0xffffffffu, z[j], 2);
+              }
+            }
+            if (SL == 2) {
+              z[0] = z[1] = z[0] + z[1] * KA_LO;
+              z[2] = z[3] = z[2] + z[3] * KA_LO;
+            }
           }
-        } else if (NC < 8) {
+        const bool masked = p0 + U * KV4_ROWS - 1 > all_see;   // positions past the end, or past a column's own
+        if (masked) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (NC == 2) s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 1);
-            s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 2);
-          }
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (p0 + u * KV4_ROWS + g + (j >> 1) * 8 > vis[nt][j & 1]) s[u][nt][j] = -INFINITY;
         }
-        if (SL == 2) {
-          s[nt][0] = s[nt][1] = s[nt][0] + s[nt][1] * KA_LO;
-          s[nt][2] = s[nt][3] = s[nt][2] + s[nt][3] * KA_LO;
-        }
-      }
-      const bool masked = p0 + KV4_ROWS - 1 > all_see;         // positions past the end, or past a column's own
-      if (masked) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (p0 + g + (j >> 1) * 8 > vis[nt][j & 1]) s[nt][j] = -INFINITY;
-      }
-      // weights; wv = weight * scale of the values, the B fragments of the second product
-      float p[NT][4];
-      uint32_t wv[NT][NF][2];
+        // weights; wv = weight * scale of the values, the B fragments of the second product
+        float p[U][NT][4];
+        uint32_t wv[U][NT][NF][2];
 #pragma unroll 1
-      for (int tries = 0; tries < 8; ++tries) {
-        bool over = false;
+        for (int tries = 0;; ++tries) {
+          float high = -INFINITY;
+          __half2 top = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int u = 0; u < U; ++u) {
+            const uint8_t* vsc = blk0 + u * C::BLK + kv4_vscale_off(D) + (NC < 8 ? g / NC : 0) * 32 + t * 8;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            p[nt][j] = fmaf(s[nt][j], kappa[nt][j & 1], -ref[nt][j & 1]);
-            over |= p[nt][j] > A + 4.0f;
+            for (int nt = 0; nt < NT; ++nt) {
+              float* w = p[u][nt];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                w[j] = fmaf(s[u][nt][j], kappa[nt][j & 1], -ref[nt][j & 1]);
+                high = fmaxf(high, w[j]);
+                w[j] = ka_exp2(w[j]);
+              }
+              uint32_t m0, m1;                                 // rows g, g + 8: columns 2t, 2t + 1
+              if (SL == 1) {
+                m0 = ka_pack(w[0], w[1]);
+                m1 = ka_pack(w[2], w[3]);
+              } else {
+                const float h0 = __half2float(__float2half_rn(w[0])), h1 = __half2float(__float2half_rn(w[2]));
+                m0 = ka_pack(h0, (w[0] - h0) * 2048.0f);
+                m1 = ka_pack(h1, (w[2] - h1) * 2048.0f);
+              }
+              m0 = ka_transpose(m0);                           // column g: positions 2t, 2t + 1
+              m1 = ka_transpose(m1);                           //           positions 2t + 8, 2t + 9
+              if (SL == 1) {
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                  const uint2 vs = *reinterpret_cast<const uint2*>(vsc + f * GP * 32);
+                  wv[u][nt][f][0] = ka_mul2(m0, vs.x);
+                  wv[u][nt][f][1] = ka_mul2(m1, vs.y);
+                }
+                if (masked) {                                  // a scale behind the last position can be anything: no weight, no product
+                  const uint32_t live0 = __hne2_mask(ka_half2(m0), __floats2half2_rn(0.0f, 0.0f));
+                  const uint32_t live1 = __hne2_mask(ka_half2(m1), __floats2half2_rn(0.0f, 0.0f));
+#pragma unroll
+                  for (int f = 0; f < NF; ++f) { wv[u][nt][f][0] &= live0; wv[u][nt][f][1] &= live1; }
+                }
+#pragma unroll
+                for (int f = 0; f < NF; ++f) top = __hmax2(top, __hmax2(ka_half2(wv[u][nt][f][0]), ka_half2(wv[u][nt][f][1])));
+              } else {
+                // the partner lane holds the other half of the same weight: 22 bits times the scale, split again
+                const uint32_t o0 = __shfl_xor_sync(0xffffffffu, m0, 4), o1 = __shfl_xor_sync(0xffffffffu, m1, 4);
+                const bool odd = g & 1;
+                const float2 a0 = __half22float2(ka_half2(odd ? o0 : m0)), b0 = __half22float2(ka_half2(odd ? m0 : o0));
+                const float2 a1 = __half22float2(ka_half2(odd ? o1 : m1)), b1 = __half22float2(ka_half2(odd ? m1 : o1));
+                const float w4[4] = {a0.x + b0.x * KA_LO, a0.y + b0.y * KA_LO, a1.x + b1.x * KA_LO, a1.y + b1.y * KA_LO};
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                  const uint2 vs = *reinterpret_cast<const uint2*>(vsc + f * GP * 32);
+                  const float2 va = __half22float2(ka_half2(vs.x)), vb = __half22float2(ka_half2(vs.y));
+                  const float v4[4] = {va.x, va.y, vb.x, vb.y};
+                  float z[4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    z[j] = w4[j] == 0.0f ? 0.0f : w4[j] * v4[j];
+                    const float h = __half2float(__float2half_rn(z[j]));
+                    if (h > 60000.0f) top = __floats2half2_rn(65504.0f, 65504.0f);
+                    z[j] = odd ? (z[j] - h) * 2048.0f : h;
+                  }
+                  wv[u][nt][f][0] = ka_pack(z[0], z[1]);
+                  wv[u][nt][f][1] = ka_pack(z[2], z[3]);
+                }
+              }
+            }
           }
-        if (__any_sync(0xffffffffu, over)) {                   // the reference moves up to the maximum so far
+          const bool over = high > A + 4.0f || fmaxf(__low2float(top), __high2float(top)) > 60000.0f;
+          if (!__any_sync(0xffffffffu, over) || tries == 8) break;
+          // The reference moves up to the maximum so far; if that was not enough, a weight times its scale leaves fp16 and
+          // all weights become 16 times smaller.
+          const float drop = tries ? 4.0f : 0.0f;
+          A -= drop;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float m = fmaxf(s[nt][j], s[nt][j + 2]) * kappa[nt][j];
+              float m = -INFINITY;
+#pragma unroll
+              for (int u = 0; u < U; ++u) m = fmaxf(m, fmaxf(s[u][nt][j], s[u][nt][j + 2]));
+              m *= kappa[nt][j];
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-              const float r = fmaxf(ref[nt][j], m - A), corr = ka_exp2(ref[nt][j] - r);
+              const float r = fmaxf(ref[nt][j] + drop, m - A), corr = ka_exp2(ref[nt][j] - r);
               ref[nt][j] = r;
               l[nt][j] *= corr;
 #pragma unroll
               for (int x = 0; x < 2 * NG; ++x) { acc[nt][x][j] *= corr; acc[nt][x][j + 2] *= corr; }
-              p[nt][j] = fmaf(s[nt][j], kappa[nt][j], -r);
-              p[nt][j + 2] = fmaf(s[nt][j + 2], kappa[nt][j], -r);
             }
         }
-        __half2 top = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) p[nt][j] = ka_exp2(p[nt][j]);
-          uint32_t m0, m1;                                     // rows g, g + 8: columns 2t, 2t + 1
-          if (SL == 1) {
-            m0 = ka_pack(p[nt][0], p[nt][1]);
-            m1 = ka_pack(p[nt][2], p[nt][3]);
-          } else {
-            const float h0 = __half2float(__float2half_rn(p[nt][0])), h1 = __half2float(__float2half_rn(p[nt][2]));
-            m0 = ka_pack(h0, (p[nt][0] - h0) * 2048.0f);
-            m1 = ka_pack(h1, (p[nt][2] - h1) * 2048.0f);
+          for (int nt = 0; nt < NT; ++nt) {
+            l[nt][0] += p[u][nt][0] + p[u][nt][2];
+            l[nt][1] += p[u][nt][1] + p[u][nt][3];
           }
-          m0 = ka_transpose(m0);                               // column g: positions 2t, 2t + 1
-          m1 = ka_transpose(m1);                               //           positions 2t + 8, 2t + 9
-          if (SL == 1) {
-            const uint32_t live0 = masked ? __hne2_mask(ka_half2(m0), __floats2half2_rn(0.0f, 0.0f)) : 0xFFFFFFFFu;
-            const uint32_t live1 = masked ? __hne2_mask(ka_half2(m1), __floats2half2_rn(0.0f, 0.0f)) : 0xFFFFFFFFu;
+        // values
 #pragma unroll
-            for (int f = 0; f < NF; ++f) {
-              const int G = f * GP + (NC < 8 ? g / NC : 0);
-              const uint2 vs = *reinterpret_cast<const uint2*>(blk + kv4_vscale_off(D) + G * 32 + t * 8);
-              // a scale behind the last position can be anything: no weight, no product
-              wv[nt][f][0] = ka_mul2(m0, vs.x) & live0;
-              wv[nt][f][1] = ka_mul2(m1, vs.y) & live1;
-              top = __hmax2(top, __hmax2(ka_half2(wv[nt][f][0]), ka_half2(wv[nt][f][1])));
-            }
-          } else {
-            // the partner lane holds the other half of the same weight: 22 bits times the scale, split again
-            const uint32_t o0 = __shfl_xor_sync(0xffffffffu, m0, 4), o1 = __shfl_xor_sync(0xffffffffu, m1, 4);
-            const bool odd = g & 1;
-            const float2 a0 = __half22float2(ka_half2(odd ? o0 : m0)), b0 = __half22float2(ka_half2(odd ? m0 : o0));
-            const float2 a1 = __half22float2(ka_half2(odd ? o1 : m1)), b1 = __half22float2(ka_half2(odd ? m1 : o1));
-            const float w4[4] = {a0.x + b0.x * KA_LO, a0.y + b0.y * KA_LO, a1.x + b1.x * KA_LO, a1.y + b1.y * KA_LO};
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int f = 0; f < NF; ++f) {
-              const int G = f * GP + (NC < 8 ? g / NC : 0);
-              const uint2 vs = *reinterpret_cast<const uint2*>(blk + kv4_vscale_off(D) + G * 32 + t * 8);
-              const float2 va = __half22float2(ka_half2(vs.x)), vb = __half22float2(ka_half2(vs.y));
-              const float v4[4] = {va.x, va.y, vb.x, vb.y};
-              float z[4];
+          for (int G = 0; G < NG; ++G) {
+            const uint2 w2 = *reinterpret_cast<const uint2*>(blk0 + u * C::BLK + kv4_v_off(D) + G * 256 + lane * 8);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                z[j] = w4[j] == 0.0f ? 0.0f : w4[j] * v4[j];
-                const float h = __half2float(__float2half_rn(z[j]));
-                if (h > 60000.0f) top = __floats2half2_rn(65504.0f, 65504.0f);
-                z[j] = odd ? (z[j] - h) * 2048.0f : h;
-              }
-              wv[nt][f][0] = ka_pack(z[0], z[1]);
-              wv[nt][f][1] = ka_pack(z[2], z[3]);
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w = h ? w2.y : w2.x, x = w >> 8;
+              const uint32_t r0 = ka_code(w), r1 = ka_code16(w), r2 = ka_code(x), r3 = ka_code16(x);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                ka_mma(acc[nt][2 * G + h], r0, r1, r2, r3, wv[u][nt][G / GP][0], wv[u][nt][G / GP][1]);
             }
           }
-        }
-        if (!__any_sync(0xffffffffu, fmaxf(__low2float(top), __high2float(top)) > 60000.0f)) break;
-        // a weight times its scale leaves fp16: all weights become 16 times smaller
-        A -= 4.0f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            ref[nt][j] += 4.0f;
-            l[nt][j] *= 0.0625f;
-#pragma unroll
-            for (int x = 0; x < 2 * NG; ++x) { acc[nt][x][j] *= 0.0625f; acc[nt][x][j + 2] *= 0.0625f; }
-          }
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        l[nt][0] += p[nt][0] + p[nt][2];
-        l[nt][1] += p[nt][1] + p[nt][3];
-      }
-      // values
-#pragma unroll
-      for (int G = 0; G < NG; ++G) {
-        const uint2 w2 = *reinterpret_cast<const uint2*>(blk + kv4_v_off(D) + G * 256 + lane * 8);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w = h ? w2.y : w2.x, u = w >> 8;
-          const uint32_t r0 = ka_code(w), r1 = ka_code16(w), r2 = ka_code(u), r3 = ka_code16(u);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) ka_mma(acc[nt][2 * G + h], r0, r1, r2, r3, wv[nt][G / GP][0], wv[nt][G / GP][1]);
-        }
-      }
+      --flying;
+      if (++take == S) { take = 0; phase ^= 1u; }
       __syncwarp();                                            // the stage has been read by every lane
-      if (ahead < mine) { issue(row, at.h, first + ahead); ++ahead; }
+      if (ahead < mine) { issue(row, at.h, first + ahead, blocks); ++ahead; }
     }
 
     // ---- where this run goes next: its first copies travel while this piece is merged ------------------------------------------
@@ -597,11 +637,12 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
     }
     if (left > 0) {
       end = ka_end(a, seq, at.ct);
-      tiles = (end + KA_TILE - 1) / KA_TILE;
+      tiles = (end + TILE - 1) / TILE;
       first = 0;
       last = (int)(tiles < left ? tiles : left);
-      mine = my_blocks();
-      for (ahead = 0; ahead < S && ahead < mine; ++ahead) issue(row, at.h, ahead);
+      blocks = (end + KV4_ROWS - 1) / KV4_ROWS;
+      mine = my_steps();
+      for (ahead = 0; ahead < S && ahead < mine; ++ahead) issue(row, at.h, ahead, blocks);
     }
 
     // ---- the four warps' states become one ---------------------------------------------------------------------------------------
@@ -690,8 +731,11 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
     if (left <= 0) break;
     __syncthreads();                                           // the merge buffers are free again
   }
-  if (dead) {                                                  // do not leave with copies in flight
-    for (; taken < issued; ++taken) ka_bar_wait(bar0 + taken % S * 8, (taken / S) & 1u, lane);
+  if (__shfl_sync(0xffffffffu, dead, 0)) {                     // do not leave with copies in flight
+    for (; flying > 0; --flying) {
+      ka_bar_wait(bar0 + take * 8, phase, lane);
+      if (++take == S) { take = 0; phase ^= 1u; }
+    }
   }
 }
 
@@ -742,9 +786,10 @@ int ka_launch(KaArgs a, cudaStream_t s) {
     sized = true;
   }
   a.width = C::W;
+  a.tile = C::TILE;
   a.sl = C::SL;
   // a list cannot be longer than the tables allow
-  const double most = (double)a.B * a.v.Hkv * (double)((((int64_t)a.v.max_pages << a.v.page_log2) + KA_TILE - 1) / KA_TILE) *
+  const double most = (double)a.B * a.v.Hkv * (double)((((int64_t)a.v.max_pages << a.v.page_log2) + C::TILE - 1) / C::TILE) *
                       (double)((a.n_rows * a.rep * C::SL + C::W - 1) / C::W);
   int64_t runs = (int64_t)sm_count() * C::CTAS;
   if ((double)runs * KA_MIN_TILES > most) runs = ((int64_t)most + KA_MIN_TILES - 1) / KA_MIN_TILES;
