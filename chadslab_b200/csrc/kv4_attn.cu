@@ -34,7 +34,9 @@ extern "C" {
 int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype) {
   if (!p || p->head_dim <= 0 || Hq <= 0) return 0;
   const int64_t width = KA_MAX_WIDTH / (dtype == BQ_DT_F32 ? 2 : 1);
-  return (int64_t)sm_count() * KA_MAX_CTAS * 2 * width * (p->head_dim + 2) * (int64_t)sizeof(float);
+  int64_t runs = (int64_t)sm_count() * KA_MAX_CTAS;
+  if (runs > KA_MAX_RUNS) runs = KA_MAX_RUNS;
+  return KA_MAX_RUNS * 8 * (int64_t)sizeof(int) + runs * 2 * width * (p->head_dim + 4) * (int64_t)sizeof(float);
 }
 
 int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq, void* out, int Hq, int dtype, const int32_t* slots,
@@ -54,7 +56,7 @@ int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq
   if (ldq < (int64_t)Hq * p->head_dim || (ldq & 1) || (reinterpret_cast<uintptr_t>(q) & pair) || (reinterpret_cast<uintptr_t>(work) & 15))
     return fail(BQ_ERR_ARG, "bq_kv4_attention: rows of q must be aligned to two elements, an even number of elements apart and not overlap; "
                             "work must be 16-byte aligned");
-  a.q = q; a.out = out; a.part = static_cast<float*>(work);
+  a.q = q; a.out = out; a.cut = static_cast<int*>(work); a.part = reinterpret_cast<float*>(a.cut + KA_MAX_RUNS * 8);
   a.ldq = ldq; a.n_rows = n_rows;
   a.slots = slots; a.pos = pos; a.starts = starts; a.status = status_word();
   a.B = (int)B; a.Hq = Hq; a.rep = rep;

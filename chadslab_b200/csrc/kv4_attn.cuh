@@ -46,7 +46,8 @@ struct KaArgs {
   Kv4View v;
   const void* q;
   void* out;
-  float* part;                                        // [runs][2][HC * (D + 2)]
+  float* part;                                        // [runs][2][HC * (D + 4)]: outputs, then (reference, sum) pairs
+  int* cut;                                           // [runs][8]: the segment that a run begins and does not finish
   int64_t ldq, n_rows;
   const int32_t *slots, *pos, *starts;
   int* status;
@@ -64,11 +65,52 @@ __device__ __forceinline__ int ka_end(const KaArgs& a, const Kv4Seq& s, int ct) 
   return s.pos + (rows < s.n ? rows : s.n);
 }
 __device__ __forceinline__ int ka_tiles(const KaArgs& a, const Kv4Seq& s, int ct) { return (ka_end(a, s, ct) + a.tile - 1) / a.tile; }
-__device__ __forceinline__ int64_t ka_head_tiles(const KaArgs& a, const Kv4Seq& s) {   // of one KV head of a sequence
-  const int cts = ka_col_tiles(a, s);
+// Tiles of one KV head of each lane's sequence.  A sequence with many column tiles is summed by the whole warp.
+__device__ __forceinline__ int64_t ka_head_tiles(const KaArgs& a, const Kv4Seq& s) {
+  const int lane = threadIdx.x & 31, cts = ka_col_tiles(a, s);
   int64_t n = 0;
-  for (int ct = 0; ct < cts; ++ct) n += ka_tiles(a, s, ct);
+  if (cts <= 4)
+    for (int ct = 0; ct < cts; ++ct) n += ka_tiles(a, s, ct);
+  for (unsigned many = __ballot_sync(0xffffffffu, cts > 4); many; many &= many - 1) {
+    const int src = __ffs(many) - 1;
+    Kv4Seq o = {};
+    o.n = __shfl_sync(0xffffffffu, s.n, src);
+    o.pos = __shfl_sync(0xffffffffu, s.pos, src);
+    const int all = __shfl_sync(0xffffffffu, cts, src);
+    int64_t sum = 0;
+    for (int ct = lane; ct < all; ct += 32) sum += ka_tiles(a, o, ct);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == src) n = sum;
+  }
   return n;
+}
+// The column tile that holds tile *rem of one KV head; *rem becomes the tile within it.
+__device__ __forceinline__ int ka_find_col_tile(const KaArgs& a, const Kv4Seq& s, int64_t* rem) {
+  const int lane = threadIdx.x & 31, cts = ka_col_tiles(a, s);
+  int64_t r = *rem;
+  int ct0 = 0;
+  if (cts > 1) {
+    for (;; ct0 += 32) {
+      const int64_t n = ct0 + lane < cts ? ka_tiles(a, s, ct0 + lane) : 0;
+      int64_t upto = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, upto, off);
+        if (lane >= off) upto += o;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, upto > r);
+      if (past || ct0 + 32 >= cts) {
+        const int l = past ? __ffs(past) - 1 : 31;
+        r -= __shfl_sync(0xffffffffu, upto - n, l);
+        ct0 += l;
+        break;
+      }
+      r -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  *rem = r;
+  return ct0;
 }
 __device__ __forceinline__ Kv4Seq ka_seq(const KaArgs& a, int b) { return kv4_seq(a.v, a.slots, a.pos, a.starts, b, a.n_rows, a.status); }
 
@@ -99,13 +141,26 @@ __device__ __forceinline__ int64_t ka_scan(int64_t v, KaScan* sc, int64_t* total
   return v;
 }
 // Length of the list and of a run, and the place of the first tile of run `run` (false: the list ends before it).
+template <typename T>
 static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc, KaPlace* at, int64_t* total, int64_t* per) {
   int64_t sum = 0, mine = 0, upto = 0, chunk;
   for (int b0 = 0; b0 < a.B; b0 += KA_THREADS) {
     const int b = b0 + (int)threadIdx.x;
-    mine = b < a.B ? ka_head_tiles(a, ka_seq(a, b)) * a.v.Hkv : 0;
+    Kv4Seq s = {};
+    if (b < a.B) s = ka_seq(a, b);
+    mine = ka_head_tiles(a, s) * a.v.Hkv;
     upto = ka_scan(mine, sc, &chunk);
     sum += chunk;
+    // rows of refused sequences are zero: the runs share them
+    if (__syncthreads_or(s.pos < 0 && s.n > 0))
+      for (int j = 0; j < KA_THREADS && b0 + j < a.B; ++j) {
+        if ((b0 + j) % runs != run) continue;
+        const Kv4Seq z = ka_seq(a, b0 + j);
+        if (z.pos >= 0) continue;
+        const int64_t n = (int64_t)z.n * a.Hq * a.v.D;
+        T* o = static_cast<T*>(a.out) + (int64_t)z.row0 * a.Hq * a.v.D;
+        for (int64_t e = threadIdx.x; e < n; e += KA_THREADS) o[e] = from_float<T>(0.0f);
+      }
   }
   *total = sum;
   *per = (sum + runs - 1) / runs;
@@ -116,7 +171,9 @@ static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc,
   for (int b0 = 0; b0 < a.B; b0 += KA_THREADS) {
     if (a.B > KA_THREADS) {                           // otherwise the sums of the loop above are still there
       const int b = b0 + (int)threadIdx.x;
-      mine = b < a.B ? ka_head_tiles(a, ka_seq(a, b)) * a.v.Hkv : 0;
+      Kv4Seq s = {};
+      if (b < a.B) s = ka_seq(a, b);
+      mine = ka_head_tiles(a, s) * a.v.Hkv;
       upto = ka_scan(mine, sc, &chunk);
     }
     const int64_t from = before + upto - mine;
@@ -128,12 +185,10 @@ static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc,
   at->b = sc->b;
   int64_t rem = sc->rem;
   const Kv4Seq s = ka_seq(a, at->b);
-  const int64_t head = ka_head_tiles(a, s);
+  const int64_t head = __shfl_sync(0xffffffffu, ka_head_tiles(a, s), 0);
   at->h = (int)(rem / head);
   rem -= at->h * head;
-  int ct = 0;
-  for (int n; rem >= (n = ka_tiles(a, s, ct)); ++ct) rem -= n;
-  at->ct = ct;
+  at->ct = ka_find_col_tile(a, s, &rem);
   at->tile = (int)rem;
   return true;
 }
@@ -257,16 +312,11 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
   pdl_wait();
   __syncthreads();
 
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {          // rows of refused sequences are zero
-    const Kv4Seq s = ka_seq(a, b);
-    if (s.pos >= 0) continue;
-    T* o = static_cast<T*>(a.out) + (int64_t)s.row0 * a.Hq * D;
-    for (int64_t e = threadIdx.x; e < (int64_t)s.n * a.Hq * D; e += KA_THREADS) o[e] = from_float<T>(0.0f);
-  }
-
+  int* cut = a.cut + (int64_t)blockIdx.x * 8;
+  if (threadIdx.x == 0) cut[0] = -1;
   KaPlace at;
   int64_t total, per;
-  if (!ka_locate(a, gridDim.x, blockIdx.x, scan, &at, &total, &per)) return;
+  if (!ka_locate<T>(a, gridDim.x, blockIdx.x, scan, &at, &total, &per)) return;
   const int64_t lo = (int64_t)blockIdx.x * per;
   int64_t left = total - lo < per ? total - lo : per;          // tiles of this run that are still to do
 
@@ -619,6 +669,7 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
     const KaPlace was = at;
     const Kv4Seq was_seq = seq;
     const bool begins = first == 0, ends = last == tiles;
+    const int was_last = last, was_tiles = tiles;
     left -= last - first;
     if (left > 0) {
       if (++at.ct >= cts) {
@@ -709,7 +760,12 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
       }
       __syncthreads();
     }
-    float* part = a.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * (HC * (D + 2));
+    float* part = a.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * (HC * (D + 4));
+    if (begins && !ends && threadIdx.x == 0) {                 // the merge starts from here: it begins at the end of this run
+      const int64_t begin = lo + per - was_last;
+      cut[1] = was_seq.row0; cut[2] = was_seq.n; cut[3] = was.h; cut[4] = was.ct;
+      cut[0] = (int)((begin + was_tiles - 1) / per);           // the last run that holds a piece of it
+    }
     const int heads = was_seq.n * a.rep;                       // (row, head) pairs of the sequence
     for (int e = threadIdx.x; e < HC * D; e += KA_THREADS) {
       const int hc = e / D, d = e % D, c = hc * SL;
@@ -739,38 +795,71 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
   }
 }
 
-// Segments that were cut: one CTA row per run boundary; the first boundary inside a segment merges its pieces in run order.
-// grid: (runs, (row, head) pairs of a tile)
+// Segments that were cut, merged in run order.  grid: (runs, (row, head) pairs of a tile); a run that begins a segment and
+// does not finish it has left its place in `cut`, the others have nothing to do.
+constexpr int KA_MERGE_THREADS = 256, KA_MAX_RUNS = 1024;
 template <typename T>
-__global__ void __launch_bounds__(KA_THREADS) kv4_attention_merge_kernel(const __grid_constant__ KaArgs a, int runs) {
-  __shared__ KaScan scan;
+__global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(const __grid_constant__ KaArgs a) {
+  __shared__ float s_f[KA_MAX_RUNS], s_red[KA_MERGE_THREADS / 32][2];
+  __shared__ float4 s_o[KA_MERGE_THREADS];
   pdl_launch_dependents();
   pdl_wait();
-  const int run = blockIdx.x + 1, HC = a.width / a.sl, hc = blockIdx.y, D = a.v.D;
-  KaPlace at;
-  int64_t total, per;
-  if (!ka_locate(a, runs, run, &scan, &at, &total, &per)) return;
-  if (at.tile == 0 || at.tile > per) return;                   // not inside a segment / an earlier boundary is inside it too
-  const Kv4Seq seq = ka_seq(a, at.b);
-  const int64_t begin = run * per - at.tile, stop = begin + ka_tiles(a, seq, at.ct);
-  const int rh = at.ct * HC + hc;
-  if (rh >= seq.n * a.rep) return;
-  const int last = (int)((stop - 1) / per);                    // the segment lies in runs run - 1 .. last
-  const int64_t slot = (int64_t)HC * (D + 2);
-  const float* p0 = a.part + ((int64_t)(run - 1) * 2 + 1) * slot;
-  float r = p0[HC * D + 2 * hc];
-  for (int k = run; k <= last; ++k) r = fmaxf(r, a.part[(int64_t)k * 2 * slot + HC * D + 2 * hc]);
-  T* out = static_cast<T*>(a.out) + ((int64_t)(seq.row0 + rh / a.rep) * a.Hq + at.h * a.rep + rh % a.rep) * D;
-  for (int d = threadIdx.x; d < D; d += KA_THREADS) {
-    const float f0 = ka_exp2(p0[HC * D + 2 * hc] - r);
-    float z = p0[HC * D + 2 * hc + 1] * f0, o = p0[hc * D + d] * f0;
-    for (int k = run; k <= last; ++k) {
-      const float* p = a.part + (int64_t)k * 2 * slot;
-      const float f = ka_exp2(p[HC * D + 2 * hc] - r);
-      z += p[HC * D + 2 * hc + 1] * f;
-      o += p[hc * D + d] * f;
+  const int run = blockIdx.x, hc = blockIdx.y, HC = a.width / a.sl, D = a.v.D, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int* cut = a.cut + (int64_t)run * 8;
+  const int last = cut[0];
+  if (last < 0) return;
+  const int row0 = cut[1], n = cut[2], h = cut[3], rh = cut[4] * HC + hc;
+  if (rh >= n * a.rep) return;
+  const int64_t slot = (int64_t)HC * (D + 4);
+  const int pieces = last - run + 1;
+  // piece 0 is this run's second state, piece j > 0 the first state of run run + j
+  const float* p0 = a.part + ((int64_t)run * 2 + 1) * slot;
+  const float* p1 = a.part + (int64_t)run * 2 * slot;
+  float r = -INFINITY;
+  for (int j = threadIdx.x; j < pieces; j += KA_MERGE_THREADS) r = fmaxf(r, (j ? p1 + 2 * j * slot : p0)[HC * D + 2 * hc]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, off));
+  if (lane == 0) s_red[warp][0] = r;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < KA_MERGE_THREADS / 32; ++w) r = fmaxf(r, s_red[w][0]);
+  float z = 0.0f;
+  for (int j = threadIdx.x; j < pieces; j += KA_MERGE_THREADS) {
+    const float* st = (j ? p1 + 2 * j * slot : p0) + HC * D + 2 * hc;
+    const float f = ka_exp2(st[0] - r);
+    s_f[j] = f;
+    z += st[1] * f;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
+  if (lane == 0) s_red[warp][1] = z;
+  __syncthreads();
+  z = 0.0f;
+#pragma unroll
+  for (int w = 0; w < KA_MERGE_THREADS / 32; ++w) z += s_red[w][1];
+  // a thread sums four dimensions over every slices-th piece
+  const int quads = D / 4, slices = KA_MERGE_THREADS / quads, q = threadIdx.x % quads, sl = threadIdx.x / quads;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (sl < slices) {
+#pragma unroll 4
+    for (int j = sl; j < pieces; j += slices) {
+      const float4 v = *reinterpret_cast<const float4*>((j ? p1 + 2 * j * slot : p0) + hc * D + q * 4);
+      const float f = s_f[j];
+      o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
     }
-    out[d] = from_float<T>(o / z);
+  }
+  s_o[threadIdx.x] = o;
+  __syncthreads();
+  if (sl == 0) {
+    const int used = slices < pieces ? slices : pieces;
+    for (int k = 1; k < used; ++k) {
+      const float4 v = s_o[k * quads + q];
+      o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+    }
+    T* out = static_cast<T*>(a.out) + ((int64_t)(row0 + rh / a.rep) * a.Hq + h * a.rep + rh % a.rep) * D + q * 4;
+    const float inv[4] = {o.x / z, o.y / z, o.z / z, o.w / z};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = from_float<T>(inv[j]);
   }
 }
 
@@ -792,11 +881,12 @@ int ka_launch(KaArgs a, cudaStream_t s) {
   const double most = (double)a.B * a.v.Hkv * (double)((((int64_t)a.v.max_pages << a.v.page_log2) + C::TILE - 1) / C::TILE) *
                       (double)((a.n_rows * a.rep * C::SL + C::W - 1) / C::W);
   int64_t runs = (int64_t)sm_count() * C::CTAS;
+  if (runs > KA_MAX_RUNS) runs = KA_MAX_RUNS;
   if ((double)runs * KA_MIN_TILES > most) runs = ((int64_t)most + KA_MIN_TILES - 1) / KA_MIN_TILES;
   BQ_CUDA(launch_chain(kv4_attention_kernel<T, NG, NC, NT>, dim3((unsigned)runs), dim3(KA_THREADS), C::SMEM, s, 1, a));
   count_launch();
   if (runs > 1) {
-    BQ_CUDA(launch_chain(kv4_attention_merge_kernel<T>, dim3((unsigned)(runs - 1), (unsigned)C::HC), dim3(KA_THREADS), 0, s, 1, a, (int)runs));
+    BQ_CUDA(launch_chain(kv4_attention_merge_kernel<T>, dim3((unsigned)(runs - 1), (unsigned)C::HC), dim3(KA_MERGE_THREADS), 0, s, 1, a));
     count_launch();
   }
   BQ_CUDA(cudaGetLastError());
