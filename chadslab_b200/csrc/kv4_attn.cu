@@ -53,8 +53,10 @@ int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq
   if (B == 0 || n_rows == 0) return BQ_OK;
   if (!q || !out || !pos || !work) return fail(BQ_ERR_ARG, "bq_kv4_attention: null pointer");
   const uintptr_t pair = dtype == BQ_DT_F32 ? 7 : 3;
-  if (ldq < (int64_t)Hq * p->head_dim || (ldq & 1) || (reinterpret_cast<uintptr_t>(q) & pair) || (reinterpret_cast<uintptr_t>(work) & 15))
-    return fail(BQ_ERR_ARG, "bq_kv4_attention: rows of q must be aligned to two elements, an even number of elements apart and not overlap; "
+  if (ldq < (int64_t)Hq * p->head_dim || (ldq & 1) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & pair) ||
+      (reinterpret_cast<uintptr_t>(work) & 15))
+    return fail(BQ_ERR_ARG, "bq_kv4_attention: rows of q and out must be aligned to two elements, those of q an even number of "
+                            "elements apart and not overlap; "
                             "work must be 16-byte aligned");
   a.q = q; a.out = out; a.cut = static_cast<int*>(work); a.part = reinterpret_cast<float*>(a.cut + KA_MAX_RUNS * 8);
   a.ldq = ldq; a.n_rows = n_rows;

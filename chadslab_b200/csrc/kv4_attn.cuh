@@ -86,17 +86,16 @@ __device__ __forceinline__ int64_t ka_head_tiles(const KaArgs& a, const Kv4Seq& 
   return n;
 }
 // The column tile that holds tile *rem of one KV head; *rem becomes the tile within it.
-__device__ __forceinline__ int ka_find_col_tile(const KaArgs& a, const Kv4Seq& s, int64_t* rem) {
+__device__ __forceinline__ int ka_find_col_tile(const KaArgs& a, const Kv4Seq& s, int* rem) {
   const int lane = threadIdx.x & 31, cts = ka_col_tiles(a, s);
-  int64_t r = *rem;
-  int ct0 = 0;
+  int r = *rem, ct0 = 0;
   if (cts > 1) {
     for (;; ct0 += 32) {
-      const int64_t n = ct0 + lane < cts ? ka_tiles(a, s, ct0 + lane) : 0;
-      int64_t upto = n;
+      const int n = ct0 + lane < cts ? ka_tiles(a, s, ct0 + lane) : 0;
+      int upto = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const int64_t o = __shfl_up_sync(0xffffffffu, upto, off);
+        const int o = __shfl_up_sync(0xffffffffu, upto, off);
         if (lane >= off) upto += o;
       }
       const unsigned past = __ballot_sync(0xffffffffu, upto > r);
@@ -116,9 +115,8 @@ __device__ __forceinline__ Kv4Seq ka_seq(const KaArgs& a, int b) { return kv4_se
 
 struct KaPlace { int b, h, ct, tile; };               // a tile of the list
 struct KaScan {
-  int64_t part[KA_WARPS], total, per;
-  int64_t rem;
-  int b;
+  int64_t part[KA_WARPS];
+  int b, rem;
 };
 // inclusive sum of v over the CTA (all threads), *total = the sum of all
 __device__ __forceinline__ int64_t ka_scan(int64_t v, KaScan* sc, int64_t* total) {
@@ -142,7 +140,7 @@ __device__ __forceinline__ int64_t ka_scan(int64_t v, KaScan* sc, int64_t* total
 }
 // Length of the list and of a run, and the place of the first tile of run `run` (false: the list ends before it).
 template <typename T>
-static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc, KaPlace* at, int64_t* total, int64_t* per) {
+static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc, KaPlace* at, int* total, int* per) {
   int64_t sum = 0, mine = 0, upto = 0, chunk;
   for (int b0 = 0; b0 < a.B; b0 += KA_THREADS) {
     const int b = b0 + (int)threadIdx.x;
@@ -162,8 +160,12 @@ static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc,
         for (int64_t e = threadIdx.x; e < n; e += KA_THREADS) o[e] = from_float<T>(0.0f);
       }
   }
-  *total = sum;
-  *per = (sum + runs - 1) / runs;
+  if (sum > 0x7FFFFFFF) {                              // weeks of work: not taken on
+    *(volatile int*)a.status = (int)BQ_ERR_UNSUPPORTED;
+    return false;
+  }
+  *total = (int)sum;
+  *per = (int)(((unsigned)sum + runs - 1) / (unsigned)runs);
   if (*per < KA_MIN_TILES) *per = KA_MIN_TILES;
   const int64_t lo = (int64_t)run * *per;
   if (lo >= sum) return false;
@@ -177,19 +179,19 @@ static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc,
       upto = ka_scan(mine, sc, &chunk);
     }
     const int64_t from = before + upto - mine;
-    if (lo >= from && lo < from + mine) { sc->b = b0 + (int)threadIdx.x; sc->rem = lo - from; }
+    if (lo >= from && lo < from + mine) { sc->b = b0 + (int)threadIdx.x; sc->rem = (int)(lo - from); }
     before += chunk;
     if (lo < before) break;
   }
   __syncthreads();
   at->b = sc->b;
-  int64_t rem = sc->rem;
+  int rem = sc->rem;
   const Kv4Seq s = ka_seq(a, at->b);
-  const int64_t head = __shfl_sync(0xffffffffu, ka_head_tiles(a, s), 0);
-  at->h = (int)(rem / head);
+  const int head = __shfl_sync(0xffffffffu, (int)ka_head_tiles(a, s), 0);
+  at->h = rem / head;
   rem -= at->h * head;
   at->ct = ka_find_col_tile(a, s, &rem);
-  at->tile = (int)rem;
+  at->tile = rem;
   return true;
 }
 
@@ -262,6 +264,10 @@ __device__ __forceinline__ float2 ka_q2(const __nv_bfloat16* p) {
   const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
+__device__ __forceinline__ void ka_store2(float* p, float x, float y) { *reinterpret_cast<float2*>(p) = make_float2(x, y); }
+__device__ __forceinline__ void ka_store2(__nv_bfloat16* p, float x, float y) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
+}
 constexpr float KA_LO = 1.0f / 2048.0f;               // weight of the second column of an fp32 row
 
 // ---- variants ------------------------------------------------------------------------------------------------------------------
@@ -277,10 +283,11 @@ template <typename T, int NG, int NC, int NT> struct KaCfg {
   static_assert(W % SL == 0, "an fp32 row takes two columns");
   static constexpr bool SUBNORMAL = SL == 1;          // keys as fp16 subnormals
   static constexpr int BLK = kv4_block_bytes(D);
-  static constexpr int OSTR = D + 4;                  // row pitch of the merge buffer: a quad's columns hit different banks
+  static constexpr int QG = NG % 4 == 0 ? NG / 4 : 1;  // groups that are merged over the warps at a time
+  static constexpr int OSTR = QG * 32 + 4;            // row pitch of the merge buffer: a quad's columns hit different banks
   // resident CTAs: what the accumulators (8 NG NT registers) and q (4 NG NT) leave of 64 K registers
   static constexpr int CTAS = NG * NT <= 4 ? 4 : NG * NT <= 8 ? 3 : 2;
-  static constexpr int FIXED = HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + (int)sizeof(KaScan) + 512;
+  static constexpr int FIXED = KA_WARPS * HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + HC * 12 + (int)sizeof(KaScan) + 64;
   // a warp's step, one stage of its ring: two blocks if the ring then has two stages, else one
   static constexpr int ROOM = (233472 / CTAS - 1024 - FIXED) / KA_WARPS;
   static constexpr int STEP = ROOM / (2 * BLK + 8) >= 2 ? 2 : 1;
@@ -299,10 +306,12 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
   extern __shared__ __align__(128) uint8_t smem[];
   // [warps][S][STAGE] ring | [warps][S] barriers | merge buffer | reference and sum of every warp and column | scan
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + KA_WARPS * S * C::STAGE);
-  float* s_o = reinterpret_cast<float*>(bars + KA_WARPS * S);
-  float* s_ref = s_o + HC * C::OSTR;
+  float* s_o = reinterpret_cast<float*>(bars + KA_WARPS * S);  // [warps][HC][OSTR]
+  float* s_ref = s_o + KA_WARPS * HC * C::OSTR;
   float* s_sum = s_ref + KA_WARPS * W;
   KaScan* scan = reinterpret_cast<KaScan*>(s_sum + KA_WARPS * W);
+  int64_t* s_to = reinterpret_cast<int64_t*>(scan + 1);
+  float* s_div = reinterpret_cast<float*>(s_to + HC);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * S * C::STAGE;
   const uint32_t bar0 = ka_smem(bars + warp * S);
@@ -315,51 +324,56 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
   int* cut = a.cut + (int64_t)blockIdx.x * 8;
   if (threadIdx.x == 0) cut[0] = -1;
   KaPlace at;
-  int64_t total, per;
+  int total, per;
   if (!ka_locate<T>(a, gridDim.x, blockIdx.x, scan, &at, &total, &per)) return;
-  const int64_t lo = (int64_t)blockIdx.x * per;
-  int64_t left = total - lo < per ? total - lo : per;          // tiles of this run that are still to do
+  const int lo = (int)blockIdx.x * per;
+  int left = total - lo < per ? total - lo : per;              // tiles of this run that are still to do
 
   Kv4Seq seq = ka_seq(a, at.b);
   int end = ka_end(a, seq, at.ct), tiles = (end + TILE - 1) / TILE;
   int cts = ka_col_tiles(a, seq);
-  uint32_t put = 0, take = 0, phase = 0;                       // stage to fill next, stage to read next and its parity
+  int put = 0, take = 0;
+  uint32_t phase = 0;                                          // stage to fill next, stage to read next and its parity
   int flying = 0;                                              // copies under way
   bool dead = false;
   const int pb = a.v.page_blocks_log2();
   const int32_t* row = a.v.tables + (int64_t)seq.slot * a.v.max_pages;
-  // requests this warp's blocks of a tile; `blocks` = blocks of the segment
-  auto issue = [&](const int32_t* row, int h, int tile, int blocks) {
-    if (lane == 0) {
-      const uint32_t bar = bar0 + put * 8, dst = ka_smem(ring + put * C::STAGE);
-      const int b0 = (tile * KA_WARPS + warp) * STEP, n = blocks - b0 < STEP ? blocks - b0 : STEP;
-      ka_bar_expect(bar, n * C::BLK);
-      auto load = [&](int blk, int count, uint32_t to) {
-        uint32_t id = (uint32_t)row[blk >> pb];
-        if (id >= (uint64_t)a.v.n_pages) {                     // no such page: recorded, the result is undefined
-          *(volatile int*)a.status = (int)BQ_ERR_ARG;
-          id = 0;
-        }
-        const uint32_t in = ((uint32_t)h << pb) + (blk & ((1 << pb) - 1));
-        ka_bulk_load(to, a.v.pages + (int64_t)id * a.v.page_bytes + (a.v.layer_off + (int64_t)in * C::BLK), count * C::BLK, bar);
-      };
-      if (pb > 0) load(b0, n, dst);                            // a page holds both
-      else
-        for (int j = 0; j < n; ++j) load(b0 + j, 1, dst + j * C::BLK);
-    }
-    put = put + 1 == S ? 0 : put + 1;
-    ++flying;
+  // One lane requests this warp's blocks of a tile into stage `st`; `blocks` = blocks of the segment
+  auto request = [&](const int32_t* row, int h, int tile, int blocks, int st) {
+    const uint32_t bar = bar0 + st * 8, dst = ka_smem(ring + st * C::STAGE);
+    const int b0 = (tile * KA_WARPS + warp) * STEP, n = blocks - b0 < STEP ? blocks - b0 : STEP;
+    ka_bar_expect(bar, n * C::BLK);
+    auto load = [&](int blk, int count, uint32_t to) {
+      uint32_t id = (uint32_t)row[blk >> pb];
+      if (id >= (uint64_t)a.v.n_pages) {                       // no such page: recorded, the result is undefined
+        *(volatile int*)a.status = (int)BQ_ERR_ARG;
+        id = 0;
+      }
+      const uint32_t in = ((uint32_t)h << pb) + (blk & ((1 << pb) - 1));
+      ka_bulk_load(to, a.v.pages + (int64_t)id * a.v.page_bytes + (a.v.layer_off + (int64_t)in * C::BLK), count * C::BLK, bar);
+    };
+    if (STEP == 1 || pb > 0) load(b0, n, dst);                 // a page holds them all
+    else
+      for (int j = 0; j < n; ++j) load(b0 + j, 1, dst + j * C::BLK);
+  };
+  // The ring is empty: the first steps of a piece, one lane each
+  auto fill = [&](const int32_t* row, int h, int first, int steps, int blocks) {
+    const int n = steps < S ? steps : S;
+    if (lane < n) request(row, h, first + lane, blocks, put + lane >= S ? put + lane - S : put + lane);
+    put = put + n >= S ? put + n - S : put + n;
+    flying += n;
+    return n;
   };
   int first = at.tile;
-  int last = (int)(tiles - first < left ? tiles : first + left);         // this piece: tiles first .. last - 1
+  int last = tiles - first < left ? tiles : first + left;         // this piece: tiles first .. last - 1
   int blocks = (end + KV4_ROWS - 1) / KV4_ROWS;
   auto my_steps = [&]() {                                      // tiles of the piece in which this warp has a block
     const int full = (blocks - warp * STEP + KA_WARPS * STEP - 1) / (KA_WARPS * STEP);
     const int n = (full < last ? full : last) - first;
     return n > 0 ? n : 0;
   };
-  int mine = my_steps(), ahead = 0;                            // steps of this piece: all, and requested
-  for (; ahead < S && ahead < mine; ++ahead) issue(row, at.h, first + ahead, blocks);
+  int mine = my_steps();                                       // steps of this piece: all, and requested
+  int ahead = fill(row, at.h, first, mine, blocks);
 
   while (true) {
     // ---- the columns: q as B fragments ------------------------------------------------------------------------------------
@@ -373,14 +387,17 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
       const int col = at.ct * W + c, rh = col / SL, i = rh / a.rep;
       const bool ok = col < cols;
       const T* qp = static_cast<const T*>(a.q) + (ok ? (int64_t)(seq.row0 + i) * a.ldq + (int64_t)(at.h * a.rep + rh % a.rep) * D : 0) + 2 * t;
+      // this lane's groups are f * GP + gi; the loads are all under way before the first is used
+      float2 x[NF][4];
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[f][k] = ok ? ka_q2(qp + (f * GP + gi) * 32 + k * 8) : make_float2(0.0f, 0.0f);
       float big = 0.0f;
 #pragma unroll
       for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 x = ok ? ka_q2(qp + (f * GP + gi) * 32 + k * 8) : make_float2(0.0f, 0.0f);
-          big = fmaxf(big, fmaxf(fabsf(x.x), fabsf(x.y)));
-        }
+        for (int k = 0; k < 4; ++k) big = fmaxf(big, fmaxf(fabsf(x[f][k].x), fabsf(x[f][k].y)));
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1)
         if (off < 4 || off >= 4 * NC) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
@@ -390,25 +407,24 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
       const bool second = SL == 2 && (col & 1);
       float sum[NF];
 #pragma unroll
-      for (int f = 0; f < NF; ++f) sum[f] = 0.0f;
-#pragma unroll
-      for (int G = 0; G < NG; ++G) {
-        const int f = G / GP;
-        const bool here = NC == 8 || G % GP == gi;
+      for (int f = 0; f < NF; ++f) {
+        sum[f] = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           // k = 2 * tile + (high k): the high half meets codes that carry 16 times as much
-          float2 x = ok && here ? ka_q2(qp + G * 32 + k * 8) : make_float2(0.0f, 0.0f);
           const float m = (k & 1) ? up * 0.0625f : up;
-          x.x *= m; x.y *= m;
+          float2 z = make_float2(x[f][k].x * m, x[f][k].y * m);
           if (second) {
-            x.x = (x.x - __half2float(__float2half_rn(x.x))) * 2048.0f;
-            x.y = (x.y - __half2float(__float2half_rn(x.y))) * 2048.0f;
+            z.x = (z.x - __half2float(__float2half_rn(z.x))) * 2048.0f;
+            z.y = (z.y - __half2float(__float2half_rn(z.y))) * 2048.0f;
           }
-          const __half2 hx = __floats2half2_rn(x.x, x.y);
-          bq[nt][2 * G + (k >> 1)][k & 1] = ka_bits(hx);
-          const float2 back = __half22float2(hx);
-          sum[f] += (back.x + back.y) * ((k & 1) ? 16.0f : 1.0f);
+          const __half2 hx = __floats2half2_rn(z.x, z.y);
+          if (C::SUBNORMAL) {
+            const float2 back = __half22float2(hx);
+            sum[f] += (back.x + back.y) * ((k & 1) ? 16.0f : 1.0f);
+          }
+#pragma unroll
+          for (int o = 0; o < GP; ++o) bq[nt][2 * (f * GP + o) + (k >> 1)][k & 1] = GP == 1 || o == gi ? ka_bits(hx) : 0u;
         }
       }
       // what the accumulator layout needs of columns 2t and 2t + 1
@@ -662,7 +678,12 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
       --flying;
       if (++take == S) { take = 0; phase ^= 1u; }
       __syncwarp();                                            // the stage has been read by every lane
-      if (ahead < mine) { issue(row, at.h, first + ahead, blocks); ++ahead; }
+      if (ahead < mine) {
+        if (lane == 0) request(row, at.h, first + ahead, blocks, put);
+        put = put + 1 == S ? 0 : put + 1;
+        ++flying;
+        ++ahead;
+      }
     }
 
     // ---- where this run goes next: its first copies travel while this piece is merged ------------------------------------------
@@ -690,10 +711,10 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
       end = ka_end(a, seq, at.ct);
       tiles = (end + TILE - 1) / TILE;
       first = 0;
-      last = (int)(tiles < left ? tiles : left);
+      last = tiles < left ? tiles : left;
       blocks = (end + KV4_ROWS - 1) / KV4_ROWS;
       mine = my_steps();
-      for (ahead = 0; ahead < S && ahead < mine; ++ahead) issue(row, at.h, ahead, blocks);
+      ahead = fill(row, at.h, 0, mine, blocks);
     }
 
     // ---- the four warps' states become one ---------------------------------------------------------------------------------------
@@ -723,69 +744,79 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
         for (int w = 1; w < KA_WARPS; ++w) r = fmaxf(r, s_ref[w * W + c]);
         corr[nt][j] = ka_exp2(ref[nt][j] - r) * (SL == 2 && j ? KA_LO : 1.0f);
       }
-#pragma unroll 1
-    for (int w = 0; w < KA_WARPS; ++w) {                       // one after the other: one order of additions
-      if (warp == w) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int G = 0; G < NG; ++G) {
-            const int n0 = 2 * t;                              // this lane's columns n0, n0 + 1; group G % GP owns NC of them
-            if (NC < 8 && (NC == 1 ? (n0 >> 1) != (G % GP) >> 1 : n0 / NC != G % GP)) continue;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float* x = acc[nt][2 * G + h];
-              const int d = (2 * G + h) * 16 + g;
-              if (SL == 2) {
-                float* o = s_o + (nt * 4 + (NC < 8 ? n0 % NC : n0) / 2) * C::OSTR + d;
-                const float y0 = x[0] * corr[nt][0] + x[1] * corr[nt][1], y1 = (x[2] * corr[nt][0] + x[3] * corr[nt][1]) * 0.0625f;
-                o[0] = w ? o[0] + y0 : y0;
-                o[8] = w ? o[8] + y1 : y1;
-              } else if (NC == 1) {
-                float* o = s_o + d;
-                const float y0 = (G & 1 ? x[1] : x[0]) * corr[nt][0], y1 = (G & 1 ? x[3] : x[2]) * (corr[nt][0] * 0.0625f);
-                o[0] = w ? o[0] + y0 : y0;
-                o[8] = w ? o[8] + y1 : y1;
-              } else {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                  float* o = s_o + (nt * 8 + (NC < 8 ? n0 % NC : n0) + j) * C::OSTR + d;
-                  const float y0 = x[j] * corr[nt][j], y1 = x[j + 2] * (corr[nt][j] * 0.0625f);
-                  o[0] = w ? o[0] + y0 : y0;
-                  o[8] = w ? o[8] + y1 : y1;
-                }
-              }
-            }
-          }
-      }
-      __syncthreads();
-    }
+    // (row, head) hc = column hc * SL of the tile: its reference and sum, and where its output goes
     float* part = a.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * (HC * (D + 4));
-    if (begins && !ends && threadIdx.x == 0) {                 // the merge starts from here: it begins at the end of this run
-      const int64_t begin = lo + per - was_last;
-      cut[1] = was_seq.row0; cut[2] = was_seq.n; cut[3] = was.h; cut[4] = was.ct;
-      cut[0] = (int)((begin + was_tiles - 1) / per);           // the last run that holds a piece of it
-    }
-    const int heads = was_seq.n * a.rep;                       // (row, head) pairs of the sequence
-    for (int e = threadIdx.x; e < HC * D; e += KA_THREADS) {
-      const int hc = e / D, d = e % D, c = hc * SL;
+    const bool whole = begins && ends;
+    if (threadIdx.x < HC) {
+      const int hc = threadIdx.x, c = hc * SL, rh = was.ct * HC + hc;
       float r = s_ref[c], z = 0.0f;
 #pragma unroll
       for (int w = 1; w < KA_WARPS; ++w) r = fmaxf(r, s_ref[w * W + c]);
 #pragma unroll
       for (int w = 0; w < KA_WARPS; ++w) z += s_sum[w * W + c] * ka_exp2(s_ref[w * W + c] - r);
-      const float o = s_o[hc * C::OSTR + d];
-      if (begins && ends) {
-        const int rh = was.ct * HC + hc;
-        if (rh < heads)
-          static_cast<T*>(a.out)[((int64_t)(was_seq.row0 + rh / a.rep) * a.Hq + was.h * a.rep + rh % a.rep) * D + d] = from_float<T>(o / z);
-      } else {
-        part[e] = o;
-        if (d == 0) { part[HC * D + 2 * hc] = r; part[HC * D + 2 * hc + 1] = z; }
+      if (!whole) { part[HC * D + 2 * hc] = r; part[HC * D + 2 * hc + 1] = z; }
+      s_div[hc] = whole ? z : 1.0f;
+      s_to[hc] = whole ? (rh < was_seq.n * a.rep ? ((int64_t)(was_seq.row0 + rh / a.rep) * a.Hq + was.h * a.rep + rh % a.rep) * D : -1)
+                       : (int64_t)hc * D;
+    }
+    if (begins && !ends && threadIdx.x == 0) {                 // the merge starts from here: it begins at the end of this run
+      const int begin = lo + per - was_last;
+      cut[1] = was_seq.row0; cut[2] = was_seq.n; cut[3] = was.h; cut[4] = was.ct;
+      cut[0] = (begin + was_tiles - 1) / per;                  // the last run that holds a piece of it
+    }
+    // QG groups at a time: every warp leaves its sums, all threads add the four in order and store
+#pragma unroll
+    for (int G0 = 0; G0 < NG; G0 += C::QG) {
+      constexpr int QD = C::QG * 32, QSTR = C::OSTR;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int G = G0; G < G0 + C::QG; ++G) {
+          const int n0 = 2 * t;                                // this lane's columns n0, n0 + 1; group G % GP owns NC of them
+          if (NC < 8 && (NC == 1 ? (n0 >> 1) != (G % GP) >> 1 : n0 / NC != G % GP)) continue;
+          const int c0 = nt * 8 + (NC < 8 ? n0 % NC : n0);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* x = acc[nt][2 * G + h];
+            float* o = s_o + (warp * HC + c0 / SL) * QSTR + (G - G0) * 32 + h * 16 + g;
+            if (SL == 2) {
+              o[0] = x[0] * corr[nt][0] + x[1] * corr[nt][1];
+              o[8] = (x[2] * corr[nt][0] + x[3] * corr[nt][1]) * 0.0625f;
+            } else if (NC == 1) {
+              o[0] = (G & 1 ? x[1] : x[0]) * corr[nt][0];
+              o[8] = (G & 1 ? x[3] : x[2]) * (corr[nt][0] * 0.0625f);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                o[j * QSTR] = x[j] * corr[nt][j];
+                o[j * QSTR + 8] = x[j + 2] * (corr[nt][j] * 0.0625f);
+              }
+            }
+          }
+        }
+      __syncthreads();
+#pragma unroll
+      for (int e0 = 0; e0 < HC * QD; e0 += KA_THREADS * 2) {   // two dimensions per thread
+        const int e = e0 + 2 * (int)threadIdx.x;
+        if (e >= HC * QD) break;
+        const int hc = e / QD, d = e % QD;
+        float2 o = *reinterpret_cast<const float2*>(s_o + hc * QSTR + d);
+#pragma unroll
+        for (int w = 1; w < KA_WARPS; ++w) {
+          const float2 v = *reinterpret_cast<const float2*>(s_o + (w * HC + hc) * QSTR + d);
+          o.x += v.x; o.y += v.y;
+        }
+        const int64_t to = s_to[hc];
+        if (whole) {
+          const float z = s_div[hc];
+          if (to >= 0) ka_store2(static_cast<T*>(a.out) + to + G0 * 32 + d, o.x / z, o.y / z);
+        } else {
+          *reinterpret_cast<float2*>(part + to + G0 * 32 + d) = o;
+        }
       }
+      __syncthreads();
     }
     if (left <= 0) break;
-    __syncthreads();                                           // the merge buffers are free again
   }
   if (__shfl_sync(0xffffffffu, dead, 0)) {                     // do not leave with copies in flight
     for (; flying > 0; --flying) {
@@ -872,6 +903,10 @@ int ka_launch(KaArgs a, cudaStream_t s) {
   static bool sized = false;
   if (!sized) {
     BQ_CUDA(cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    // an SM that another kernel has set up for less shared memory takes fewer of these CTAs until it is idle, and a run that
+    // has to wait for a slot doubles the kernel's time (batch 64 x 2048 x 16 heads of 256: 182 us with 21 of 444 runs late)
+    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NC, NT>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_merge_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
     sized = true;
   }
   a.width = C::W;
