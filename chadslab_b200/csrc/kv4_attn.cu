@@ -34,7 +34,7 @@ extern "C" {
 int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype) {
   if (!p || p->head_dim <= 0 || Hq <= 0) return 0;
   const int64_t width = KA_MAX_WIDTH / (dtype == BQ_DT_F32 ? 2 : 1);
-  int64_t runs = (int64_t)sm_count() * KA_MAX_CTAS;
+  int64_t runs = (int64_t)sm_count() * KA_MAX_TEAMS;
   if (runs > KA_MAX_RUNS) runs = KA_MAX_RUNS;
   return KA_MAX_RUNS * 8 * (int64_t)sizeof(int) + runs * 2 * width * (p->head_dim + 4) * (int64_t)sizeof(float);
 }

@@ -28,7 +28,9 @@
 // drops when weight * scale overflows, i.e. for values far above one.
 //
 // Work.  The tiles (128 positions, or 64 where two steps of 32 per warp do not fit into shared memory) of all (sequence, KV head, column tile) segments form one list that is cut into equal runs,
-// one per resident CTA: ragged batches and few long sequences fill the machine alike.  A warp takes 32 (16) positions of every
+// one per team of four warps: ragged batches and few long sequences fill the machine alike.  The teams of an SM (two to
+// four) are one CTA: as CTAs of their own some found no contiguous registers beside the preceding kernel's and started
+// when the others were done, which doubled the kernel's time (8 of 444 late: 169 us for 100 us of work).  A warp takes 32 (16) positions of every
 // tile through its own ring of bulk copies (no barrier between warps inside a segment).  A segment that lies in one
 // run is finished there; one that is cut leaves partial states in the caller's scratch, which a second kernel merges in run
 // order.  Every result has one order of additions: repeated calls give the same bits.
@@ -37,10 +39,21 @@
 
 namespace bq {
 
-constexpr int KA_WARPS = 4;
+constexpr int KA_WARPS = 4;                           // of a team: the warps that work on one run
 constexpr int KA_THREADS = KA_WARPS * 32;
 constexpr int KA_MIN_TILES = 1;                       // a run is at least this long
 constexpr uint64_t KA_WAIT_NS = 2000000000ull;        // bound of the wait for a copy
+
+// x / d for 0 <= x < 2^31
+struct KaDiv {
+  uint32_t mul, shift, d;
+  __device__ __forceinline__ int operator()(int x) const { return (int)((__umulhi(mul, (uint32_t)x) + (uint32_t)x) >> shift); }
+};
+inline KaDiv ka_div(uint32_t d) {
+  uint32_t s = 0;
+  while (((uint64_t)1 << s) < d) ++s;
+  return KaDiv{(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - d)) / d + 1), s, d};
+}
 
 struct KaArgs {
   Kv4View v;
@@ -52,19 +65,22 @@ struct KaArgs {
   const int32_t *slots, *pos, *starts;
   int* status;
   int B, Hq, rep;
-  int width, sl;                                      // columns of a tile; columns per (row, head): 1, or 2 for fp32 rows
-  int tile;                                           // positions of a tile: 16 or 32 per warp
+  KaDiv by_rep, by_row;                               // query heads of a KV head; columns of a row: those times sl
+  int width_log2, sl;                                 // columns of a tile; columns per (row, head): 1, or 2 for fp32 rows
+  int tile_log2;                                      // positions of a tile: 16 or 32 per warp
 };
 
 // ---- the list of tiles ---------------------------------------------------------------------------------------------------
-__device__ __forceinline__ int ka_col_tiles(const KaArgs& a, const Kv4Seq& s) {
-  return s.n > 0 && s.pos >= 0 ? (int)(((int64_t)s.n * a.rep * a.sl + a.width - 1) / a.width) : 0;
+__device__ __forceinline__ int ka_col_tiles(const KaArgs& a, const Kv4Seq& s) {      // rows * columns of a row < 2^31
+  return s.n > 0 && s.pos >= 0 ? (s.n * (int)a.by_row.d + (1 << a.width_log2) - 1) >> a.width_log2 : 0;
 }
 __device__ __forceinline__ int ka_end(const KaArgs& a, const Kv4Seq& s, int ct) {      // positions that column tile ct sees
-  const int rows = (int)((((int64_t)ct + 1) * a.width - 1) / (a.rep * a.sl)) + 1;
+  const int rows = a.by_row(((ct + 1) << a.width_log2) - 1) + 1;
   return s.pos + (rows < s.n ? rows : s.n);
 }
-__device__ __forceinline__ int ka_tiles(const KaArgs& a, const Kv4Seq& s, int ct) { return (ka_end(a, s, ct) + a.tile - 1) / a.tile; }
+__device__ __forceinline__ int ka_tiles(const KaArgs& a, const Kv4Seq& s, int ct) {
+  return (ka_end(a, s, ct) + (1 << a.tile_log2) - 1) >> a.tile_log2;
+}
 // Tiles of one KV head of each lane's sequence.  A sequence with many column tiles is summed by the whole warp.
 __device__ __forceinline__ int64_t ka_head_tiles(const KaArgs& a, const Kv4Seq& s) {
   const int lane = threadIdx.x & 31, cts = ka_col_tiles(a, s);
@@ -113,22 +129,37 @@ __device__ __forceinline__ int ka_find_col_tile(const KaArgs& a, const Kv4Seq& s
 }
 __device__ __forceinline__ Kv4Seq ka_seq(const KaArgs& a, int b) { return kv4_seq(a.v, a.slots, a.pos, a.starts, b, a.n_rows, a.status); }
 
+// barrier of a team (1 + its number; 0 is the CTA's)
+__device__ __forceinline__ void ka_sync(int team) { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(KA_THREADS) : "memory"); }
+__device__ __forceinline__ bool ka_sync_or(int team, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(team + 1), "n"(KA_THREADS), "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+
 struct KaPlace { int b, h, ct, tile; };               // a tile of the list
 struct KaScan {
   int64_t part[KA_WARPS];
   int b, rem;
 };
-// inclusive sum of v over the CTA (all threads), *total = the sum of all
-__device__ __forceinline__ int64_t ka_scan(int64_t v, KaScan* sc, int64_t* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// inclusive sum of v over the team, *total = the sum of all
+__device__ __forceinline__ int64_t ka_scan(int64_t v, KaScan* sc, int team, int64_t* total) {
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % KA_WARPS;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const int64_t o = __shfl_up_sync(0xffffffffu, v, off);
     if (lane >= off) v += o;
   }
-  __syncthreads();
+  ka_sync(team);
   if (lane == 31) sc->part[warp] = v;
-  __syncthreads();
+  ka_sync(team);
   int64_t t = 0;
 #pragma unroll
   for (int w = 0; w < KA_WARPS; ++w) {
@@ -140,24 +171,25 @@ __device__ __forceinline__ int64_t ka_scan(int64_t v, KaScan* sc, int64_t* total
 }
 // Length of the list and of a run, and the place of the first tile of run `run` (false: the list ends before it).
 template <typename T>
-static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc, KaPlace* at, int* total, int* per) {
+static __device__ bool ka_locate(const KaArgs& a, int runs, int run, int team, KaScan* sc, KaPlace* at, int* total, int* per) {
+  const int tid = threadIdx.x % KA_THREADS;
   int64_t sum = 0, mine = 0, upto = 0, chunk;
   for (int b0 = 0; b0 < a.B; b0 += KA_THREADS) {
-    const int b = b0 + (int)threadIdx.x;
+    const int b = b0 + tid;
     Kv4Seq s = {};
     if (b < a.B) s = ka_seq(a, b);
     mine = ka_head_tiles(a, s) * a.v.Hkv;
-    upto = ka_scan(mine, sc, &chunk);
+    upto = ka_scan(mine, sc, team, &chunk);
     sum += chunk;
     // rows of refused sequences are zero: the runs share them
-    if (__syncthreads_or(s.pos < 0 && s.n > 0))
+    if (ka_sync_or(team, s.pos < 0 && s.n > 0))
       for (int j = 0; j < KA_THREADS && b0 + j < a.B; ++j) {
         if ((b0 + j) % runs != run) continue;
         const Kv4Seq z = ka_seq(a, b0 + j);
         if (z.pos >= 0) continue;
         const int64_t n = (int64_t)z.n * a.Hq * a.v.D;
         T* o = static_cast<T*>(a.out) + (int64_t)z.row0 * a.Hq * a.v.D;
-        for (int64_t e = threadIdx.x; e < n; e += KA_THREADS) o[e] = from_float<T>(0.0f);
+        for (int64_t e = tid; e < n; e += KA_THREADS) o[e] = from_float<T>(0.0f);
       }
   }
   if (sum > 0x7FFFFFFF) {                              // weeks of work: not taken on
@@ -172,18 +204,18 @@ static __device__ bool ka_locate(const KaArgs& a, int runs, int run, KaScan* sc,
   int64_t before = 0;
   for (int b0 = 0; b0 < a.B; b0 += KA_THREADS) {
     if (a.B > KA_THREADS) {                           // otherwise the sums of the loop above are still there
-      const int b = b0 + (int)threadIdx.x;
+      const int b = b0 + tid;
       Kv4Seq s = {};
       if (b < a.B) s = ka_seq(a, b);
       mine = ka_head_tiles(a, s) * a.v.Hkv;
-      upto = ka_scan(mine, sc, &chunk);
+      upto = ka_scan(mine, sc, team, &chunk);
     }
     const int64_t from = before + upto - mine;
-    if (lo >= from && lo < from + mine) { sc->b = b0 + (int)threadIdx.x; sc->rem = (int)(lo - from); }
+    if (lo >= from && lo < from + mine) { sc->b = b0 + tid; sc->rem = (int)(lo - from); }
     before += chunk;
     if (lo < before) break;
   }
-  __syncthreads();
+  ka_sync(team);
   at->b = sc->b;
   int rem = sc->rem;
   const Kv4Seq s = ka_seq(a, at->b);
@@ -285,25 +317,28 @@ template <typename T, int NG, int NC, int NT> struct KaCfg {
   static constexpr int BLK = kv4_block_bytes(D);
   static constexpr int QG = NG % 4 == 0 ? NG / 4 : 1;  // groups that are merged over the warps at a time
   static constexpr int OSTR = QG * 32 + 4;            // row pitch of the merge buffer: a quad's columns hit different banks
-  // resident CTAs: what the accumulators (8 NG NT registers) and q (4 NG NT) leave of 64 K registers
-  static constexpr int CTAS = NG * NT <= 4 ? 4 : NG * NT <= 8 ? 3 : 2;
-  static constexpr int FIXED = KA_WARPS * HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + HC * 12 + (int)sizeof(KaScan) + 64;
+  // teams of an SM: what the accumulators (8 NG NT registers) and q (4 NG NT) leave of 64 K registers
+  static constexpr int TEAMS = NG * NT <= 4 ? 4 : NG * NT <= 8 ? 3 : 2;
+  static constexpr int FIXED = KA_WARPS * HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + HC * 12 + (int)sizeof(KaScan) + 128;
   // a warp's step, one stage of its ring: two blocks if the ring then has two stages, else one
-  static constexpr int ROOM = (233472 / CTAS - 1024 - FIXED) / KA_WARPS;
+  static constexpr int ROOM = (232448 / TEAMS - FIXED) / KA_WARPS;
   static constexpr int STEP = ROOM / (2 * BLK + 8) >= 2 ? 2 : 1;
   static constexpr int TILE = KA_WARPS * STEP * KV4_ROWS;
   static constexpr int STAGE = STEP * BLK;
   static constexpr int STAGES = ROOM / (STAGE + 8) >= 4 ? 4 : ROOM / (STAGE + 8);
   static_assert(STAGES >= 2, "the ring needs two stages");
-  static constexpr int SMEM = KA_WARPS * STAGES * (STAGE + 8) + FIXED;
+  static constexpr int SMEM = (KA_WARPS * STAGES * (STAGE + 8) + FIXED) / 128 * 128;      // of a team
   static constexpr int U = NT == 1 && NF * NG <= 16 ? STEP : 1;  // blocks whose scores and weights are held at a time
 };
 
 template <typename T, int NG, int NC, int NT>
-__global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_attention_kernel(const __grid_constant__ KaArgs a) {
+__global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1) kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   using C = KaCfg<T, NG, NC, NT>;
   constexpr int D = C::D, SL = C::SL, GP = C::GP, NF = C::NF, W = C::W, HC = C::HC, S = C::STAGES, U = C::U, STEP = C::STEP, TILE = C::TILE;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem_all[];
+  const int team = threadIdx.x / KA_THREADS, tid = threadIdx.x % KA_THREADS;
+  const int run = team * gridDim.x + blockIdx.x, runs = gridDim.x * C::TEAMS;      // few runs: one per SM first
+  uint8_t* smem = smem_all + team * C::SMEM;
   // [warps][S][STAGE] ring | [warps][S] barriers | merge buffer | reference and sum of every warp and column | scan
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + KA_WARPS * S * C::STAGE);
   float* s_o = reinterpret_cast<float*>(bars + KA_WARPS * S);  // [warps][HC][OSTR]
@@ -312,21 +347,21 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
   KaScan* scan = reinterpret_cast<KaScan*>(s_sum + KA_WARPS * W);
   int64_t* s_to = reinterpret_cast<int64_t*>(scan + 1);
   float* s_div = reinterpret_cast<float*>(s_to + HC);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % KA_WARPS, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * S * C::STAGE;
   const uint32_t bar0 = ka_smem(bars + warp * S);
   if (lane < S) ka_bar_init(bar0 + lane * 8);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_launch_dependents();
   pdl_wait();
-  __syncthreads();
+  ka_sync(team);
 
-  int* cut = a.cut + (int64_t)blockIdx.x * 8;
-  if (threadIdx.x == 0) cut[0] = -1;
+  int* cut = a.cut + (int64_t)run * 8;
+  if (tid == 0) cut[0] = -1;
   KaPlace at;
   int total, per;
-  if (!ka_locate<T>(a, gridDim.x, blockIdx.x, scan, &at, &total, &per)) return;
-  const int lo = (int)blockIdx.x * per;
+  if (!ka_locate<T>(a, runs, run, team, scan, &at, &total, &per)) return;
+  const int lo = run * per;
   int left = total - lo < per ? total - lo : per;              // tiles of this run that are still to do
 
   Kv4Seq seq = ka_seq(a, at.b);
@@ -384,9 +419,9 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int c = NC < 8 ? g % NC : nt * 8 + g, gi = NC < 8 ? g / NC : 0;
-      const int col = at.ct * W + c, rh = col / SL, i = rh / a.rep;
+      const int col = at.ct * W + c, rh = col / SL, i = a.by_rep(rh);
       const bool ok = col < cols;
-      const T* qp = static_cast<const T*>(a.q) + (ok ? (int64_t)(seq.row0 + i) * a.ldq + (int64_t)(at.h * a.rep + rh % a.rep) * D : 0) + 2 * t;
+      const T* qp = static_cast<const T*>(a.q) + (ok ? (int64_t)(seq.row0 + i) * a.ldq + (int64_t)(at.h * a.rep + rh - i * a.rep) * D : 0) + 2 * t;
       // this lane's groups are f * GP + gi; the loads are all under way before the first is used
       float2 x[NF][4];
 #pragma unroll
@@ -445,7 +480,7 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
         for (int j = 0; j < 2; ++j) start[nt][f][j] = __shfl_sync(0xffffffffu, z, (2 * t + j) * 4);
       }
     }
-    const int all_see = seq.pos + (int)((int64_t)at.ct * W / (a.rep * SL));        // every column sees positions up to here
+    const int all_see = seq.pos + a.by_row(at.ct * W);        // every column sees positions up to here
 
     // ---- the positions ----------------------------------------------------------------------------------------------------
     float acc[NT][2 * NG][4], ref[NT][2], l[NT][2];
@@ -456,8 +491,12 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
       for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[nt][i][j] = 0.0f;
-      ref[nt][0] = ref[nt][1] = -3.0e38f;
-      l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // a column without a row has no weight anywhere: it must not take part in the search for a reference
+        ref[nt][j] = vis[nt][j] == 0x7FFFFFFF ? 3.0e38f : -3.0e38f;
+        l[nt][j] = 0.0f;
+      }
     }
     for (int i = 0; i < mine; ++i) {
       const uint8_t* stage = ring + take * C::STAGE;
@@ -732,7 +771,7 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
           s_sum[warp * W + nt * 8 + n] = z;
         }
       }
-    __syncthreads();
+    ka_sync(team);
     float corr[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -745,10 +784,10 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
         corr[nt][j] = ka_exp2(ref[nt][j] - r) * (SL == 2 && j ? KA_LO : 1.0f);
       }
     // (row, head) hc = column hc * SL of the tile: its reference and sum, and where its output goes
-    float* part = a.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * (HC * (D + 4));
+    float* part = a.part + ((int64_t)run * 2 + (begins ? 1 : 0)) * (HC * (D + 4));
     const bool whole = begins && ends;
-    if (threadIdx.x < HC) {
-      const int hc = threadIdx.x, c = hc * SL, rh = was.ct * HC + hc;
+    if (tid < HC) {
+      const int hc = tid, c = hc * SL, rh = was.ct * HC + hc;
       float r = s_ref[c], z = 0.0f;
 #pragma unroll
       for (int w = 1; w < KA_WARPS; ++w) r = fmaxf(r, s_ref[w * W + c]);
@@ -756,10 +795,10 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
       for (int w = 0; w < KA_WARPS; ++w) z += s_sum[w * W + c] * ka_exp2(s_ref[w * W + c] - r);
       if (!whole) { part[HC * D + 2 * hc] = r; part[HC * D + 2 * hc + 1] = z; }
       s_div[hc] = whole ? z : 1.0f;
-      s_to[hc] = whole ? (rh < was_seq.n * a.rep ? ((int64_t)(was_seq.row0 + rh / a.rep) * a.Hq + was.h * a.rep + rh % a.rep) * D : -1)
-                       : (int64_t)hc * D;
+      const int i = a.by_rep(rh);
+      s_to[hc] = !whole ? (int64_t)hc * D : i < was_seq.n ? ((int64_t)(was_seq.row0 + i) * a.Hq + was.h * a.rep + rh - i * a.rep) * D : -1;
     }
-    if (begins && !ends && threadIdx.x == 0) {                 // the merge starts from here: it begins at the end of this run
+    if (begins && !ends && tid == 0) {                 // the merge starts from here: it begins at the end of this run
       const int begin = lo + per - was_last;
       cut[1] = was_seq.row0; cut[2] = was_seq.n; cut[3] = was.h; cut[4] = was.ct;
       cut[0] = (begin + was_tiles - 1) / per;                  // the last run that holds a piece of it
@@ -794,10 +833,10 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
             }
           }
         }
-      __syncthreads();
+      ka_sync(team);
 #pragma unroll
       for (int e0 = 0; e0 < HC * QD; e0 += KA_THREADS * 2) {   // two dimensions per thread
-        const int e = e0 + 2 * (int)threadIdx.x;
+        const int e = e0 + 2 * tid;
         if (e >= HC * QD) break;
         const int hc = e / QD, d = e % QD;
         float2 o = *reinterpret_cast<const float2*>(s_o + hc * QSTR + d);
@@ -814,7 +853,7 @@ __global__ void __launch_bounds__(KA_THREADS, (KaCfg<T, NG, NC, NT>::CTAS)) kv4_
           *reinterpret_cast<float2*>(part + to + G0 * 32 + d) = o;
         }
       }
-      __syncthreads();
+      ka_sync(team);
     }
     if (left <= 0) break;
   }
@@ -835,7 +874,7 @@ __global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(c
   __shared__ float4 s_o[KA_MERGE_THREADS];
   pdl_launch_dependents();
   pdl_wait();
-  const int run = blockIdx.x, hc = blockIdx.y, HC = a.width / a.sl, D = a.v.D, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int run = blockIdx.x, hc = blockIdx.y, HC = (1 << a.width_log2) / a.sl, D = a.v.D, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int* cut = a.cut + (int64_t)run * 8;
   const int last = cut[0];
   if (last < 0) return;
@@ -894,36 +933,31 @@ __global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(c
   }
 }
 
-// most runs of any variant, and most floats of a run's two partial states
-constexpr int KA_MAX_CTAS = 4, KA_MAX_WIDTH = 16;
+constexpr int KA_MAX_TEAMS = 4, KA_MAX_WIDTH = 16;    // of any variant
 
 template <typename T, int NG, int NC, int NT>
 int ka_launch(KaArgs a, cudaStream_t s) {
   using C = KaCfg<T, NG, NC, NT>;
+  static_assert(C::TEAMS <= KA_MAX_TEAMS && C::W <= KA_MAX_WIDTH, "the caller's scratch is sized for these");
   static bool sized = false;
   if (!sized) {
-    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    // an SM that another kernel has set up for less shared memory takes fewer of these CTAs until it is idle, and a run that
-    // has to wait for a slot doubles the kernel's time (batch 64 x 2048 x 16 heads of 256: 182 us with 21 of 444 runs late)
-    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NC, NT>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
-    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_merge_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TEAMS * C::SMEM));
     sized = true;
   }
-  a.width = C::W;
-  a.tile = C::TILE;
+  a.by_rep = ka_div(a.rep);
+  a.by_row = ka_div(a.rep * C::SL);
   a.sl = C::SL;
+  for (a.width_log2 = 0; 1 << a.width_log2 < C::W;) ++a.width_log2;
+  for (a.tile_log2 = 0; 1 << a.tile_log2 < C::TILE;) ++a.tile_log2;
   // a list cannot be longer than the tables allow
   const double most = (double)a.B * a.v.Hkv * (double)((((int64_t)a.v.max_pages << a.v.page_log2) + C::TILE - 1) / C::TILE) *
                       (double)((a.n_rows * a.rep * C::SL + C::W - 1) / C::W);
-  int64_t runs = (int64_t)sm_count() * C::CTAS;
-  if (runs > KA_MAX_RUNS) runs = KA_MAX_RUNS;
-  if ((double)runs * KA_MIN_TILES > most) runs = ((int64_t)most + KA_MIN_TILES - 1) / KA_MIN_TILES;
-  BQ_CUDA(launch_chain(kv4_attention_kernel<T, NG, NC, NT>, dim3((unsigned)runs), dim3(KA_THREADS), C::SMEM, s, 1, a));
-  count_launch();
-  if (runs > 1) {
-    BQ_CUDA(launch_chain(kv4_attention_merge_kernel<T>, dim3((unsigned)(runs - 1), (unsigned)C::HC), dim3(KA_MERGE_THREADS), 0, s, 1, a));
-    count_launch();
-  }
+  int64_t grid = sm_count();
+  if (grid > KA_MAX_RUNS / C::TEAMS) grid = KA_MAX_RUNS / C::TEAMS;
+  if ((double)grid * KA_MIN_TILES > most) grid = ((int64_t)most + KA_MIN_TILES - 1) / KA_MIN_TILES;
+  BQ_CUDA(launch_chain(kv4_attention_kernel<T, NG, NC, NT>, dim3((unsigned)grid), dim3(C::TEAMS * KA_THREADS), C::TEAMS * C::SMEM, s, 1, a));
+  BQ_CUDA(launch_chain(kv4_attention_merge_kernel<T>, dim3((unsigned)(grid * C::TEAMS - 1), (unsigned)C::HC), dim3(KA_MERGE_THREADS), 0, s, 1, a));
+  count_launch(2);
   BQ_CUDA(cudaGetLastError());
   return BQ_OK;
 }

@@ -328,6 +328,25 @@ def test_attention_ranges(cuda_lib, q_scale, vscale, dtype):
     check(kv, 0, data, lens, [1, 1], 4, dtype, rng, q_scale)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,rep", [(64, 1), (64, 5), (128, 3), (256, 1), (256, 17), (96, 2)])
+def test_bytes_behind_a_sequence_do_not_matter(cuda_lib, D, rep, dtype):
+    """The rest of a last block can hold anything (scales of infinity, NaN, 65504, negative ones): the same bits."""
+    lens, new = [3, 17, 64, 41, 1], [1, 1, 1, 9, 1]
+    got = []
+    for fill_with in (0, 0x7C00, 0x7E00, 0x7BFF, -0x8000 + 0x7C00, -1):
+        rng = np.random.default_rng(21)
+        kv = make(1, 1, D, page=32)
+        kv.pages.view(torch.int16).fill_(fill_with)
+        fill(kv, 0, lens, rng, dtype)
+        q = rows(rng, sum(new), rep, D, dtype)
+        pos = [n - m for n, m in zip(lens, new)]
+        got.append([kv.attention(0, q, None, ints(pos), starts_of(new)), kv.attention(0, q[:5], None, ints([n - 1 for n in lens]))])
+    for g in got[1:]:
+        assert torch.equal(g[0], got[0][0]) and torch.equal(g[1], got[0][1])
+    assert torch.isfinite(got[0][0]).all() and status() == 0
+
+
 def test_attention_rows_of_nobody(cuda_lib):
     """Rows behind the last sequence stay as they were, rows of a refused sequence are zero."""
     rng = np.random.default_rng(2)
