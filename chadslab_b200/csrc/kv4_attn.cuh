@@ -19,8 +19,8 @@
 // q is scaled per column by a power of two so that fp16 holds it exactly (bf16 has 8 bits); fp32 rows take two columns, the
 // value and its remainder times 2^11 (22 bits), and so do their weights.
 //
-// Few columns (one query head per KV head: one).  m16n8k16 has 8 columns, so NC < 8 columns leave room for 8 / NC groups side
-// by side: column n = group * NC + c of the B operand is zero outside its group's dimensions, one accumulator tile then holds
+// Few columns (one query head per KV head: one).  m16n8k16 has 8 columns, so NC < 8 columns leave room for up to 8 / NC groups
+// side by side: column n = group * NC + c of the B operand is zero outside its group's dimensions, one accumulator tile then holds
 // 8 / NC groups' sums, each still apart for its scale; weights times scales of 8 / NC groups share one B fragment likewise.
 //
 // Softmax runs in the exp2 domain with a reference R per column that lags behind the maximum: weights are 2^(s - R), R = max -
@@ -307,12 +307,13 @@ template <typename T, int NG, int NC, int NT> struct KaCfg {
   static_assert(NC == 8 || NT == 1, "several column tiles need full ones");
   static constexpr int SL = sizeof(T) == 4 ? 2 : 1;
   static constexpr int D = NG * GROUP;
-  static constexpr int GP = 8 / NC;                   // groups side by side in a fragment
+  static constexpr int GP = 8 / NC < NG ? 8 / NC : NG; // groups side by side in a fragment
   static_assert(NG % GP == 0, "whole fragments");
   static constexpr int NF = NG / GP;
   static constexpr int W = NC * NT;                   // columns of a tile
   static constexpr int HC = W / SL;
   static_assert(W % SL == 0, "an fp32 row takes two columns");
+  static constexpr int J = NC == 1 || SL == 2 ? 1 : 2;  // different (row, head) pairs among a lane's two columns
   static constexpr bool SUBNORMAL = SL == 1;          // keys as fp16 subnormals
   static constexpr int BLK = kv4_block_bytes(D);
   static constexpr int QG = NG % 4 == 0 ? NG / 4 : 1;  // groups that are merged over the warps at a time
@@ -334,7 +335,7 @@ template <typename T, int NG, int NC, int NT> struct KaCfg {
 template <typename T, int NG, int NC, int NT>
 __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1) kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   using C = KaCfg<T, NG, NC, NT>;
-  constexpr int D = C::D, SL = C::SL, GP = C::GP, NF = C::NF, W = C::W, HC = C::HC, S = C::STAGES, U = C::U, STEP = C::STEP, TILE = C::TILE;
+  constexpr int D = C::D, SL = C::SL, GP = C::GP, NF = C::NF, W = C::W, HC = C::HC, S = C::STAGES, U = C::U, STEP = C::STEP, TILE = C::TILE, J = C::J;
   extern __shared__ __align__(128) uint8_t smem_all[];
   const int team = threadIdx.x / KA_THREADS, tid = threadIdx.x % KA_THREADS;
   const int run = team * gridDim.x + blockIdx.x, runs = gridDim.x * C::TEAMS;      // few runs: one per SM first
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
 #pragma unroll
       for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[f][k] = ok ? ka_q2(qp + (f * GP + gi) * 32 + k * 8) : make_float2(0.0f, 0.0f);
+        for (int k = 0; k < 4; ++k) x[f][k] = ok && gi < GP ? ka_q2(qp + (f * GP + gi) * 32 + k * 8) : make_float2(0.0f, 0.0f);
       float big = 0.0f;
 #pragma unroll
       for (int f = 0; f < NF; ++f)
@@ -515,6 +516,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const uint8_t* blk = blk0 + u * C::BLK;
+          uint2 kq0, kq1;
 #pragma unroll
           for (int f = 0; f < NF; ++f) {
             float c[NT][4];
@@ -544,10 +546,19 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
             const __half* ks = reinterpret_cast<const __half*>(blk + kv4_kscale_off(D));
             float2 k0, k1;
             if (NC == 1) {
-              k0 = __half22float2(*reinterpret_cast<const __half2*>(ks + g * NG + f * 8 + 2 * t));
-              k1 = __half22float2(*reinterpret_cast<const __half2*>(ks + (g + 8) * NG + f * 8 + 2 * t));
+              const int G = f * GP + (2 * t < GP ? 2 * t : 0);         // columns past the groups hold zeros
+              k0 = __half22float2(*reinterpret_cast<const __half2*>(ks + g * NG + G));
+              k1 = __half22float2(*reinterpret_cast<const __half2*>(ks + (g + 8) * NG + G));
+            } else if (NC == 8 && NG % 4 == 0) {               // four groups by one load per row
+              if (f % 4 == 0) {
+                kq0 = *reinterpret_cast<const uint2*>(ks + g * NG + f);
+                kq1 = *reinterpret_cast<const uint2*>(ks + (g + 8) * NG + f);
+              }
+              const float2 x0 = __half22float2(ka_half2(f % 4 < 2 ? kq0.x : kq0.y)), x1 = __half22float2(ka_half2(f % 4 < 2 ? kq1.x : kq1.y));
+              k0.x = k0.y = f % 2 ? x0.y : x0.x;
+              k1.x = k1.y = f % 2 ? x1.y : x1.x;
             } else {
-              const int G = NC == 8 ? f : NC == 4 ? f * 2 + (t >> 1) : f * 4 + t;
+              const int at_col = 2 * t / NC, G = f * GP + (at_col < GP ? at_col : 0);
               k0.x = k0.y = __half2float(ks[g * NG + G]);
               k1.x = k1.y = __half2float(ks[(g + 8) * NG + G]);
             }
@@ -594,7 +605,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                if (p0 + u * KV4_ROWS + g + (j >> 1) * 8 > vis[nt][j & 1]) s[u][nt][j] = -INFINITY;
+                if ((J == 2 || !(j & 1)) && p0 + u * KV4_ROWS + g + (j >> 1) * 8 > vis[nt][j & 1]) s[u][nt][j] = -INFINITY;
         }
         // weights; wv = weight * scale of the values, the B fragments of the second product
         float p[U][NT][4];
@@ -605,12 +616,13 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
           __half2 top = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const uint8_t* vsc = blk0 + u * C::BLK + kv4_vscale_off(D) + (NC < 8 ? g / NC : 0) * 32 + t * 8;
+            const uint8_t* vsc = blk0 + u * C::BLK + kv4_vscale_off(D) + (g / NC < GP ? g / NC : 0) * 32 + t * 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               float* w = p[u][nt];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
+                if (J == 1 && (j & 1)) { w[j] = w[j - 1]; continue; }
                 w[j] = fmaf(s[u][nt][j], kappa[nt][j & 1], -ref[nt][j & 1]);
                 high = fmaxf(high, w[j]);
                 w[j] = ka_exp2(w[j]);
@@ -677,6 +689,10 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
+              if (J == 1 && j) {
+                ref[nt][1] = ref[nt][0];
+                continue;
+              }
               float m = -INFINITY;
 #pragma unroll
               for (int u = 0; u < U; ++u) m = fmaxf(m, fmaxf(s[u][nt][j], s[u][nt][j + 2]));
@@ -688,7 +704,10 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
               ref[nt][j] = r;
               l[nt][j] *= corr;
 #pragma unroll
-              for (int x = 0; x < 2 * NG; ++x) { acc[nt][x][j] *= corr; acc[nt][x][j + 2] *= corr; }
+              for (int x = 0; x < 2 * NG; ++x) {
+                acc[nt][x][j] *= corr; acc[nt][x][j + 2] *= corr;
+                if (J == 1) { acc[nt][x][1] *= corr; acc[nt][x][3] *= corr; }
+              }
             }
         }
 #pragma unroll
@@ -696,7 +715,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             l[nt][0] += p[u][nt][0] + p[u][nt][2];
-            l[nt][1] += p[u][nt][1] + p[u][nt][3];
+            if (J == 2) l[nt][1] += p[u][nt][1] + p[u][nt][3];
           }
         // values
 #pragma unroll

@@ -4,6 +4,8 @@
 namespace bq {
 
 template <typename T> static int pick(const KaArgs& a, int64_t cols, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (cols <= 1) return ka_launch<T, 4, 1, 1>(a, s);
   if (cols <= 2) return ka_launch<T, 4, 2, 1>(a, s);
   if (cols <= 4) return ka_launch<T, 4, 4, 1>(a, s);
   if (cols <= 8) return ka_launch<T, 4, 8, 1>(a, s);

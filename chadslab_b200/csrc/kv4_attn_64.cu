@@ -4,6 +4,9 @@
 namespace bq {
 
 template <typename T> static int pick(const KaArgs& a, int64_t cols, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (cols <= 1) return ka_launch<T, 2, 1, 1>(a, s);
+  if (cols <= 2) return ka_launch<T, 2, 2, 1>(a, s);
   if (cols <= 4) return ka_launch<T, 2, 4, 1>(a, s);
   if (cols <= 8) return ka_launch<T, 2, 8, 1>(a, s);
   return ka_launch<T, 2, 8, 2>(a, s);
