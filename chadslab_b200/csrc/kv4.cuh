@@ -93,10 +93,6 @@ __device__ __forceinline__ __half kv4_scale(float amax) {
   const float s = __fmul_rn(amax, 1.0f / 7.0f);
   return __float2half_rn(s > 65504.0f ? 65504.0f : s);
 }
-__device__ __forceinline__ uint32_t kv4_nibble(float x, float s) {
-  const float q = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(x, s)), -7.0f), 7.0f) : 0.0f;
-  return (uint32_t)((int)q + 8);
-}
 #endif
 
 }  // namespace bq

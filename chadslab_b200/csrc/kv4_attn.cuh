@@ -319,7 +319,7 @@ template <typename T, int NG, int NC, int NT> struct KaCfg {
   static constexpr int QG = NG % 4 == 0 ? NG / 4 : 1;  // groups that are merged over the warps at a time
   static constexpr int OSTR = QG * 32 + 4;            // row pitch of the merge buffer: a quad's columns hit different banks
   // teams of an SM: what the accumulators (8 NG NT registers) and q (4 NG NT) leave of 64 K registers
-  static constexpr int TEAMS = NG * NT <= 4 ? 4 : NG * NT <= 8 ? 3 : 2;
+  static constexpr int TEAMS = NG * NT <= (NC == 8 ? 3 : 4) ? 4 : NG * NT <= (NC == 8 ? 5 : 8) ? 3 : 2;
   static constexpr int FIXED = KA_WARPS * HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + HC * 12 + (int)sizeof(KaScan) + 128;
   // a warp's step, one stage of its ring: two blocks if the ring then has two stages, else one
   static constexpr int ROOM = (232448 / TEAMS - FIXED) / KA_WARPS;

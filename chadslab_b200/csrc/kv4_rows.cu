@@ -1,16 +1,20 @@
 // Rows in and out of the 4-bit KV cache: append (quantise rows into their blocks), the same with the rotary embedding of a
 // fused q|k|v projection in front, and gather (back to rows).
 //
-// One warp handles K or V of one (16-position block, head).  It works in the fragment order of the block (kv4.cuh): for K a
-// lane holds eight dimensions of two positions per group and the absmax of a group is a maximum over the four lanes of a
-// quad; for V it holds four dimensions of four positions and the maximum runs over the eight quads.  A block that the call
-// fills completely is stored as whole words, otherwise each position's bytes are stored by themselves.
+// Two warps handle K or V of one (16-position block, head), half the rows each, row by row: a lane owns eight neighbouring dimensions (one or two
+// 16-byte loads), four lanes a group, so the absmax takes two exchanges for the whole row, whatever head_dim.  The eight
+// codes of a lane and of its neighbour share eight bytes (elements e and e + 8 of a 16-wide tile): one exchange pairs them.
+// A block that the call fills completely is put together in shared memory and leaves as 16-byte stores; otherwise the bytes
+// of its rows are stored one by one (a decode step has one row per block, and other rows' bytes must stay).
+// Bound: launch latency for a decode step; for prompts the instructions of the quantiser.
 #include "kv4.cuh"
 
 namespace bq {
 
 constexpr int KR_WARPS = 8;
 constexpr int KR_THREADS = KR_WARPS * 32;
+constexpr int KR_TASKS = KR_WARPS / 2;                 // two warps share a task: (block, head, K or V)
+__device__ __forceinline__ void kr_pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory"); }
 
 // The place of a work item: rows r_lo .. r_hi - 1 of block `blk` of one sequence; row r is row first + r of the call's rows
 struct KrItem {
@@ -34,139 +38,118 @@ __device__ __forceinline__ KrItem kr_item(const Kv4View& v, const int32_t* slots
   return it;
 }
 
-// two neighbouring elements of a row
-__device__ __forceinline__ float2 kr_load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
-__device__ __forceinline__ float2 kr_load2(const __nv_bfloat16* p) {
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-// Where a warp's rows come from: element d of row r of the block.
+// Eight neighbouring elements of a row, from a row of the call ...
 template <typename T> struct KrPlain {
   const T* base;                                       // row 0 of the block, this head
   int64_t ld;
-  __device__ __forceinline__ float one(int r, int d) const { return to_float<T>(base[r * ld + d]); }
-  __device__ __forceinline__ float2 two(int r, int d) const { return kr_load2(base + r * ld + d); }
+  bool vec;                                            // rows are 16-byte aligned
+  __device__ __forceinline__ void eight(int r, int d, float* x) const {
+    const T* p = base + r * ld + d;
+    if (vec) {
+      load8<T>(p, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = to_float<T>(p[j]);
+    }
+  }
 };
-// ... of the fp32 projection output, rotated by the angles of row r (the roundings of rope_kv_append_kernel)
+// ... or of the fp32 projection output, rotated by the angles of row r (the roundings of rope_kv_append_kernel)
 template <typename T> struct KrRope {
   const float* base;
   int64_t ld;
   const float *cs, *sn;                                // [16][D / 2]
   int D;
   bool rotate;
-  __device__ __forceinline__ float one(int r, int d) const {
-    return rope_elem<T>(base + r * ld, d, D, cs + r * (D / 2), sn + r * (D / 2), rotate);
+  __device__ __forceinline__ void eight(int r, int d, float* x) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = rope_elem<T>(base + r * ld, d + j, D, cs + r * (D / 2), sn + r * (D / 2), rotate);
   }
-  __device__ __forceinline__ float2 two(int r, int d) const { return make_float2(one(r, d), one(r, d + 1)); }
 };
 
+// code + 8 of x: rint(x / scale).  The product with the reciprocal is off by less than 2^-20 of a step, so only next to a
+// border between two codes is the quotient itself needed.
+__device__ __forceinline__ uint32_t kr_nibble(float x, float s, float inv) {
+  const float y = x * inv;
+  float f = rintf(y);
+  if (fabsf(fabsf(y - f) - 0.5f) < 1e-5f) f = rintf(__fdiv_rn(x, s));
+  return (uint32_t)((int)fminf(fmaxf(f, -7.0f), 7.0f) + 8);
+}
+// Byte of the codes that holds elements e and e + 8 (e < 8) of tile `tile` of group G at position r
+__device__ __forceinline__ int kr_byte(bool values, int r, int G, int tile, int e) {
+  return G * 256 + 4 * tile + (r >> 3) + (values ? (e * 4 + ((r & 7) >> 1)) * 8 + 2 * (r & 1) : ((r & 7) * 4 + (e >> 1)) * 8 + 2 * (e & 1));
+}
+__device__ __forceinline__ int kr_scale(bool values, int r, int G, int NG) {
+  return values ? G * 16 + ((r & 7) >> 1) * 4 + (r >> 3) * 2 + (r & 1) : r * NG + G;
+}
+// Quantises rows r_lo .. r_hi - 1 of a block into `to`: its codes and scales in global memory, or a copy in shared memory.
+// 256 / D rows at a time; the next ones are on their way while these are quantised.
 template <typename SRC>
-__device__ __forceinline__ void kr_append_k(const SRC& src, uint8_t* blk, int NG, int r_lo, int r_hi) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const bool in0 = g >= r_lo && g < r_hi, in1 = g + 8 >= r_lo && g + 8 < r_hi, whole = r_lo == 0 && r_hi == KV4_ROWS;
-  __half* scales = reinterpret_cast<__half*>(blk + 256 * NG);
-  for (int G = 0; G < NG; ++G) {
-    float x[2][8];                                     // [row g / g + 8][tile][2t, 2t + 1, 2t + 8, 2t + 9]
-    float amax[2] = {0.0f, 0.0f};
+__device__ __forceinline__ void kr_quantise(const SRC& src, uint8_t* to, bool values, int D, int r_lo, int r_hi) {
+  const int lane = threadIdx.x & 31, NG = D / GROUP, per = D / 8, rows = 32 / per, sub = lane / per, l = lane - sub * per;
+  const int G = l >> 2, tile = (l >> 1) & 1;
+  __half* scales = reinterpret_cast<__half*>(to + 256 * NG);
+  auto load = [&](int r, float* x) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+    if (sub < rows && r < r_hi) src.eight(r, l * 8, x);
+  };
+  float next[8];
+  load(r_lo + sub, next);
+  for (int r0 = r_lo; r0 < r_hi; r0 += rows) {
+    const int r = r0 + sub;
+    float x[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float2 p = make_float2(0.0f, 0.0f);
-        if (u ? in1 : in0) p = src.two(g + 8 * u, G * 32 + j * 8 + 2 * t);
-        x[u][2 * j] = p.x; x[u][2 * j + 1] = p.y;
-        amax[u] = kv4_absmax(amax[u], kv4_absmax(p.x, p.y));
-      }
-      amax[u] = kv4_absmax(amax[u], __shfl_xor_sync(0xffffffffu, amax[u], 1));
-      amax[u] = kv4_absmax(amax[u], __shfl_xor_sync(0xffffffffu, amax[u], 2));
+    for (int j = 0; j < 8; ++j) x[j] = next[j];
+    load(r + rows, next);
+    float amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = kv4_absmax(amax, x[j]);
+    amax = kv4_absmax(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = kv4_absmax(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const __half sh = kv4_scale(amax);
+    const float s = __half2float(sh), inv = s > 0.0f ? 1.0f / s : 0.0f;
+    uint32_t mine = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mine |= kr_nibble(x[j], s, inv) << (4 * j);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+    if (sub >= rows || r >= r_hi) continue;
+    // the even lane (elements 0-7 of the tile) has the low nibbles; each lane stores four of the eight bytes
+    const uint32_t low = l & 1 ? other : mine, high = l & 1 ? mine : other;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = ((j + G) & 3) * 2 + (l & 1);                         // (groups start at different banks)
+      to[kr_byte(values, r, G, tile, e)] = (uint8_t)(((low >> (4 * e)) & 15u) | (((high >> (4 * e)) & 15u) << 4));
     }
-    uint32_t w[2] = {0u, 0u};                          // the lane's words of the two tiles
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const __half sh = kv4_scale(amax[u]);
-      const float s = __half2float(sh);
-      if (t == 0 && (u ? in1 : in0)) scales[(g + 8 * u) * NG + G] = sh;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)                    // e = 2 * (high k) + odd
-          w[i] |= kv4_nibble(x[u][i * 4 + e], s) << (8 * u + 16 * (e & 1) + 4 * (e >> 1));
-    }
-    uint8_t* at = blk + G * 256 + lane * 8;
-    if (whole) {
-      *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (u ? in1 : in0) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            at[i * 4 + u] = (uint8_t)(w[i] >> (8 * u));
-            at[i * 4 + 2 + u] = (uint8_t)(w[i] >> (16 + 8 * u));
-          }
-        }
-    }
+    if ((l & 3) == 0) scales[kr_scale(values, r, G, NG)] = sh;
   }
 }
-
+// the same by a pair of warps: through `stage` (288 * NG bytes of shared memory of the pair's own) if the whole block is written
 template <typename SRC>
-__device__ __forceinline__ void kr_append_v(const SRC& src, uint8_t* blk, int NG, int r_lo, int r_hi) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const bool whole = r_lo == 0 && r_hi == KV4_ROWS;
-  __half* scales = reinterpret_cast<__half*>(blk + 256 * NG);
-  for (int G = 0; G < NG; ++G) {
-    uint32_t w[2] = {0u, 0u};
-    __half sh[4];
-    bool in[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {                      // byte j of a word: position 2t + 8 (j & 1) + (j >> 1)
-      const int r = 2 * t + 8 * (j & 1) + (j >> 1);
-      in[j] = r >= r_lo && r < r_hi;
-      float x[4], amax = 0.0f;                         // dimensions g, g + 8 of the two tiles
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = in[j] ? src.one(r, G * 32 + e * 8 + g) : 0.0f;
-        amax = kv4_absmax(amax, x[e]);
-      }
-      amax = kv4_absmax(amax, __shfl_xor_sync(0xffffffffu, amax, 4));
-      amax = kv4_absmax(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
-      amax = kv4_absmax(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
-      sh[j] = kv4_scale(amax);
-      const float s = __half2float(sh[j]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e >> 1] |= kv4_nibble(x[e], s) << (8 * j + 4 * (e & 1));
-    }
-    uint8_t* at = blk + G * 256 + lane * 8;
-    if (whole) {
-      *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (in[j]) {
-          at[j] = (uint8_t)(w[0] >> (8 * j));
-          at[4 + j] = (uint8_t)(w[1] >> (8 * j));
-        }
-    }
-    if (g == 0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {                    // scale order: low even, low odd, high even, high odd position
-        const int o = 2 * (j & 1) + (j >> 1);
-        if (in[j]) scales[G * 16 + t * 4 + o] = sh[j];
-      }
-    }
+__device__ __forceinline__ void kr_append(const SRC& src, uint8_t* blk, uint8_t* stage, bool values, int D, int r_lo, int r_hi) {
+  const int pair = threadIdx.x >> 6, half = (threadIdx.x >> 5) & 1;
+  if (r_hi - r_lo < KV4_ROWS) {
+    const int mid = (r_lo + r_hi + 1) >> 1;
+    kr_quantise(src, blk, values, D, half ? mid : r_lo, half ? r_hi : mid);
+    return;
   }
+  kr_quantise(src, stage, values, D, half * 8, half * 8 + 8);
+  kr_pair_sync(pair);
+  for (int e = (threadIdx.x & 63) * 16; e < 288 * (D / GROUP); e += 1024)
+    *reinterpret_cast<uint4*>(blk + e) = *reinterpret_cast<const uint4*>(stage + e);
 }
+constexpr int KR_STAGE = 288 * 8;                      // of the largest head_dim
 
-// grid: (items, heads by warps); a warp takes (head, K or V)
+// grid: (items, tasks by pairs of warps); a task is (head, K or V)
 template <typename T>
 __global__ void __launch_bounds__(KR_THREADS) kv4_append_kernel(Kv4View v, const T* __restrict__ k, const T* __restrict__ val, int64_t ldk,
                                                                 int64_t ldv, const int32_t* __restrict__ slots,
                                                                 const int32_t* __restrict__ pos, const int32_t* __restrict__ starts, int B,
-                                                                int64_t n_rows, int* __restrict__ status) {
+                                                                int64_t n_rows, int* __restrict__ status, bool vec) {
+  __shared__ __align__(16) uint8_t stage[KR_TASKS][KR_STAGE];
   pdl_launch_dependents();
   pdl_wait();
   const KrItem it = kr_item(v, slots, pos, starts, B, n_rows, blockIdx.x, status);
-  const int task = blockIdx.y * KR_WARPS + (threadIdx.x >> 5);
+  const int pair = threadIdx.x >> 6, task = blockIdx.y * KR_TASKS + pair;
   if (!it.live || task >= 2 * v.Hkv) return;
   const int h = task >> 1;
   uint8_t* blk = v.block(v.tables + (int64_t)it.slot * v.max_pages, it.blk, h);
@@ -174,9 +157,10 @@ __global__ void __launch_bounds__(KR_THREADS) kv4_append_kernel(Kv4View v, const
     *(volatile int*)status = (int)BQ_ERR_ARG;
     return;
   }
-  const int NG = v.D / GROUP;
-  if (!(task & 1)) kr_append_k(KrPlain<T>{k + (int64_t)it.first * ldk + (int64_t)h * v.D, ldk}, blk, NG, it.r_lo, it.r_hi);
-  else kr_append_v(KrPlain<T>{val + (int64_t)it.first * ldv + (int64_t)h * v.D, ldv}, blk + kv4_v_off(v.D), NG, it.r_lo, it.r_hi);
+  const bool values = task & 1;
+  const int64_t ld = values ? ldv : ldk;
+  kr_append(KrPlain<T>{(values ? val : k) + (int64_t)it.first * ld + (int64_t)h * v.D, ld, vec}, blk + (values ? kv4_v_off(v.D) : 0), stage[pair],
+            values, v.D, it.r_lo, it.r_hi);
 }
 
 // The same behind a fused projection: qkv fp32 [n_rows][(Hq + 2 Hkv) * D].  Tasks 0 .. 2 Hkv - 1 are the heads' K and V,
@@ -187,6 +171,7 @@ __global__ void __launch_bounds__(KR_THREADS) kv4_rope_append_kernel(Kv4View v, 
                                                                      const int32_t* __restrict__ pos, const int32_t* __restrict__ starts, int B,
                                                                      int64_t n_rows, int* __restrict__ status) {
   extern __shared__ float s_ang[];                     // cos [16][D / 2], sin [16][D / 2]
+  __shared__ __align__(16) uint8_t stage[KR_TASKS][KR_STAGE];
   pdl_launch_dependents();
   pdl_wait();
   const KrItem it = kr_item(v, slots, pos, starts, B, n_rows, blockIdx.x, status);
@@ -199,13 +184,13 @@ __global__ void __launch_bounds__(KR_THREADS) kv4_rope_append_kernel(Kv4View v, 
     sincosf((float)(it.pos0 + r) * inv, &sn[r * half + j], &cs[r * half + j]);
   }
   __syncthreads();
-  const int task = blockIdx.y * KR_WARPS + (threadIdx.x >> 5);
+  const int task = blockIdx.y * KR_TASKS + (threadIdx.x >> 6);
   if (task >= 2 * v.Hkv + Hq) return;
   const int64_t ld = (int64_t)(Hq + 2 * v.Hkv) * D;
   const float* rows = qkv + (int64_t)it.first * ld;
   if (task >= 2 * v.Hkv) {
     const int h = task - 2 * v.Hkv;
-    for (int e = threadIdx.x & 31; e < (it.r_hi - it.r_lo) * D; e += 32) {
+    for (int e = threadIdx.x & 63; e < (it.r_hi - it.r_lo) * D; e += 64) {
       const int r = it.r_lo + e / D, d = e % D;
       q_out[((int64_t)(it.first + r) * Hq + h) * D + d] =
           from_float<T>(rope_elem<T>(rows + r * ld + (int64_t)h * D, d, D, cs + r * half, sn + r * half, true));
@@ -218,61 +203,50 @@ __global__ void __launch_bounds__(KR_THREADS) kv4_rope_append_kernel(Kv4View v, 
     *(volatile int*)status = (int)BQ_ERR_ARG;
     return;
   }
-  const int NG = D / GROUP;
-  if (!(task & 1)) kr_append_k(KrRope<T>{rows + (int64_t)(Hq + h) * D, ld, cs, sn, D, true}, blk, NG, it.r_lo, it.r_hi);
-  else kr_append_v(KrRope<T>{rows + (int64_t)(Hq + v.Hkv + h) * D, ld, cs, sn, D, false}, blk + kv4_v_off(D), NG, it.r_lo, it.r_hi);
+  const bool values = task & 1;
+  kr_append(KrRope<T>{rows + (int64_t)(Hq + (values ? v.Hkv : 0) + h) * D, ld, cs, sn, D, !values}, blk + (values ? kv4_v_off(D) : 0),
+            stage[threadIdx.x >> 6], values, D, it.r_lo, it.r_hi);
 }
-
-// code * scale of one nibble of a word
-__device__ __forceinline__ float kr_value(uint32_t w, int shift, float s) { return (float)((int)((w >> shift) & 15u) - 8) * s; }
 
 template <typename T>
 __global__ void __launch_bounds__(KR_THREADS) kv4_gather_kernel(Kv4View v, T* __restrict__ k, T* __restrict__ val, const int32_t* __restrict__ slots,
                                                                 const int32_t* __restrict__ pos, const int32_t* __restrict__ starts, int B,
-                                                                int64_t n_rows, int* __restrict__ status) {
+                                                                int64_t n_rows, int* __restrict__ status, bool vec) {
+  __shared__ __align__(16) uint8_t all[KR_TASKS][KR_STAGE];
   pdl_launch_dependents();
   pdl_wait();
   const KrItem it = kr_item(v, slots, pos, starts, B, n_rows, blockIdx.x, status);
-  const int task = blockIdx.y * KR_WARPS + (threadIdx.x >> 5);
+  const int pair = threadIdx.x >> 6, task = blockIdx.y * KR_TASKS + pair;
   if (!it.live || task >= 2 * v.Hkv) return;
-  const int h = task >> 1, D = v.D, NG = D / GROUP;
+  const int h = task >> 1, D = v.D, NG = D / GROUP, lane = threadIdx.x & 31;
+  const bool values = task & 1;
   const uint8_t* blk = v.block(v.tables + (int64_t)it.slot * v.max_pages, it.blk, h);
   if (!blk) {
     *(volatile int*)status = (int)BQ_ERR_ARG;
     return;
   }
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (values) blk += kv4_v_off(D);
+  uint8_t* stage = all[pair];
+#pragma unroll
+  for (int e = (threadIdx.x & 63) * 16; e < KR_STAGE; e += 1024)
+    if (e < 288 * NG) *reinterpret_cast<uint4*>(stage + e) = *reinterpret_cast<const uint4*>(blk + e);
+  kr_pair_sync(pair);
+  const int per = D / 8, rows = 32 / per, sub = lane / per, l = lane - sub * per;       // 256 / D rows at a time
+  if (sub >= rows) return;
+  const int G = l >> 2, tile = (l >> 1) & 1, shift = 4 * (l & 1);
+  const __half* scales = reinterpret_cast<const __half*>(stage + 256 * NG);
   const int64_t ld = (int64_t)v.Hkv * D;
-  T* out = ((task & 1) ? val : k) + (int64_t)it.first * ld + (int64_t)h * D;
-  if (task & 1) blk += kv4_v_off(D);
-  const __half* scales = reinterpret_cast<const __half*>(blk + 256 * NG);
-  for (int G = 0; G < NG; ++G) {
-    const uint2 w2 = *reinterpret_cast<const uint2*>(blk + G * 256 + lane * 8);
-    const uint32_t w[2] = {w2.x, w2.y};
-    if (!(task & 1)) {
+  T* out = (values ? val : k) + (int64_t)it.first * ld + (int64_t)h * D + l * 8;
+  for (int r = it.r_lo + ((threadIdx.x >> 5) & 1) * rows + sub; r < it.r_hi; r += 2 * rows) {
+    const float s = __half2float(scales[kr_scale(values, r, G, NG)]);
+    float x[8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int r = g + 8 * u;
-        if (r < it.r_lo || r >= it.r_hi) continue;
-        const float s = __half2float(scales[r * NG + G]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int hi = 0; hi < 2; ++hi) {
-            T* o = out + r * ld + G * 32 + i * 16 + hi * 8 + 2 * t;
-            o[0] = from_float<T>(kr_value(w[i], 8 * u + 4 * hi, s));
-            o[1] = from_float<T>(kr_value(w[i], 16 + 8 * u + 4 * hi, s));
-          }
-      }
+    for (int e = 0; e < 8; ++e) x[e] = (float)((int)((stage[kr_byte(values, r, G, tile, e)] >> shift) & 15) - 8) * s;
+    if (vec) {
+      store8<T>(out + r * ld, x);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = 2 * t + 8 * (j & 1) + (j >> 1);
-        if (r < it.r_lo || r >= it.r_hi) continue;
-        const float s = __half2float(scales[G * 16 + t * 4 + 2 * (j & 1) + (j >> 1)]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[r * ld + G * 32 + e * 8 + g] = from_float<T>(kr_value(w[e >> 1], 8 * j + 4 * (e & 1), s));
-      }
+      for (int e = 0; e < 8; ++e) out[r * ld + e] = from_float<T>(x[e]);
     }
   }
 }
@@ -303,17 +277,18 @@ int bq_kv4_append(const bq_kv4_pool* p, int layer, const void* k, const void* v,
   if (B == 0 || n_rows == 0) return BQ_OK;
   if (!k || !v) return fail(BQ_ERR_ARG, "bq_kv4_append: null pointer");
   const int64_t row = (int64_t)p->kv_heads * p->head_dim;
-  const uintptr_t pair = dtype == BQ_DT_F32 ? 7 : 3;
-  if (ldk < row || ldv < row || (ldk & 1) || (ldv & 1) || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & pair))
-    return fail(BQ_ERR_ARG, "bq_kv4_append: rows must be aligned to two elements, an even number of elements apart and not overlap");
-  const dim3 grid((unsigned)kr_items(B, n_rows, starts != nullptr), (unsigned)((2 * p->kv_heads + KR_WARPS - 1) / KR_WARPS));
+  const uintptr_t size = dtype == BQ_DT_F32 ? 4 : 2;
+  const uintptr_t align = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
+  if (ldk < row || ldv < row || (align & (size - 1))) return fail(BQ_ERR_ARG, "bq_kv4_append: rows overlap or are not aligned to their elements");
+  const bool vec = ((align | (uintptr_t)ldk * size | (uintptr_t)ldv * size) & 15) == 0;
+  const dim3 grid((unsigned)kr_items(B, n_rows, starts != nullptr), (unsigned)((2 * p->kv_heads + KR_TASKS - 1) / KR_TASKS));
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == BQ_DT_F32)
     BQ_CUDA(launch_chain(kv4_append_kernel<float>, grid, dim3(KR_THREADS), 0, s, 1, view, (const float*)k, (const float*)v, ldk, ldv, slots, pos,
-                         starts, (int)B, n_rows, status_word()));
+                         starts, (int)B, n_rows, status_word(), vec));
   else
     BQ_CUDA(launch_chain(kv4_append_kernel<__nv_bfloat16>, grid, dim3(KR_THREADS), 0, s, 1, view, (const __nv_bfloat16*)k,
-                         (const __nv_bfloat16*)v, ldk, ldv, slots, pos, starts, (int)B, n_rows, status_word()));
+                         (const __nv_bfloat16*)v, ldk, ldv, slots, pos, starts, (int)B, n_rows, status_word(), vec));
   count_launch();
   BQ_CUDA(cudaGetLastError());
   return BQ_OK;
@@ -327,7 +302,7 @@ int bq_kv4_rope_append(const bq_kv4_pool* p, int layer, const float* qkv, void* 
   if (Hq <= 0 || Hq % p->kv_heads) return fail(BQ_ERR_ARG, "bq_kv4_rope_append: query heads must be a multiple of the KV heads");
   if (B == 0 || n_rows == 0) return BQ_OK;
   if (!qkv || !q_out) return fail(BQ_ERR_ARG, "bq_kv4_rope_append: null pointer");
-  const dim3 grid((unsigned)kr_items(B, n_rows, starts != nullptr), (unsigned)((2 * p->kv_heads + Hq + KR_WARPS - 1) / KR_WARPS));
+  const dim3 grid((unsigned)kr_items(B, n_rows, starts != nullptr), (unsigned)((2 * p->kv_heads + Hq + KR_TASKS - 1) / KR_TASKS));
   const size_t smem = (size_t)KV4_ROWS * p->head_dim * sizeof(float);
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == BQ_DT_F32)
@@ -348,14 +323,15 @@ int bq_kv4_gather(const bq_kv4_pool* p, int layer, void* k, void* v, int dtype, 
   if (rc || (rc = kr_check(p, B, n_rows, starts, pos, dtype, "bq_kv4_gather"))) return rc;
   if (B == 0 || n_rows == 0) return BQ_OK;
   if (!k || !v) return fail(BQ_ERR_ARG, "bq_kv4_gather: null pointer");
-  const dim3 grid((unsigned)kr_items(B, n_rows, starts != nullptr), (unsigned)((2 * p->kv_heads + KR_WARPS - 1) / KR_WARPS));
+  const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
+  const dim3 grid((unsigned)kr_items(B, n_rows, starts != nullptr), (unsigned)((2 * p->kv_heads + KR_TASKS - 1) / KR_TASKS));
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == BQ_DT_F32)
     BQ_CUDA(launch_chain(kv4_gather_kernel<float>, grid, dim3(KR_THREADS), 0, s, 1, view, (float*)k, (float*)v, slots, pos, starts, (int)B,
-                         n_rows, status_word()));
+                         n_rows, status_word(), vec));
   else
     BQ_CUDA(launch_chain(kv4_gather_kernel<__nv_bfloat16>, grid, dim3(KR_THREADS), 0, s, 1, view, (__nv_bfloat16*)k, (__nv_bfloat16*)v, slots,
-                         pos, starts, (int)B, n_rows, status_word()));
+                         pos, starts, (int)B, n_rows, status_word(), vec));
   count_launch();
   BQ_CUDA(cudaGetLastError());
   return BQ_OK;

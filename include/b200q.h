@@ -375,8 +375,8 @@ int bq_kv4_free(const bq_kv4_pool* p, const int32_t* slots, int64_t n, void* str
  * with the tables, lengths and counts that go with them; `p` is unchanged, and so are the bytes of free pages of `to`.  If
  * `to` has too few pages BQ_ERR_STATE is recorded and `to` is unchanged.                                                 */
 int bq_kv4_compact(const bq_kv4_pool* p, const bq_kv4_pool* to, void* stream);
-/* Quantises rows k, v (n_rows rows of kv_heads * head_dim elements, ldk / ldv elements apart, both even, aligned to two
- * elements) into the pages of `layer`: scale = fp16(min(absmax * fp32(1/7), 65504)), code = clip(rint(x / scale), +-7)
+/* Quantises rows k, v (n_rows rows of kv_heads * head_dim elements, ldk / ldv elements apart; fastest when every row is
+ * 16-byte aligned) into the pages of `layer`: scale = fp16(min(absmax * fp32(1/7), 65504)), code = clip(rint(x / scale), +-7)
  * (bq_quantize divides by 7, which differs in the last bit now and then); a NaN makes its group NaN.  Pages are written whether or not other sequences hold them: call
  * bq_kv4_extend first, once for all layers.                                                                              */
 int bq_kv4_append(const bq_kv4_pool* p, int layer, const void* k, const void* v, int64_t ldk, int64_t ldv, int dtype,
@@ -390,7 +390,8 @@ int bq_kv4_rope_append(const bq_kv4_pool* p, int layer, const float* qkv, void* 
 int bq_kv4_gather(const bq_kv4_pool* p, int layer, void* k, void* v, int dtype, const int32_t* slots, const int32_t* pos,
                   const int32_t* starts, int64_t B, int64_t n_rows, void* stream);
 /* out[n_rows, Hq, head_dim] = softmax(q . K^T / sqrt(head_dim)) . V over positions 0 .. own position of every row
- * (causal), grouped-query heads.  Rows of q are ldq elements apart.  Rows of a sequence with pos < 0 are set to zero.
+ * (causal), grouped-query heads.  Rows of q are ldq elements apart (even; q and out
+ * aligned to two elements).  Rows of a sequence with pos < 0 are set to zero.
  * work: bq_kv4_attention_work_bytes() of device scratch, 16-byte aligned, contents do not matter; calls that may
  * overlap on the device need scratch of their own.                                                                       */
 int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype);
