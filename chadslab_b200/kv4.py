@@ -23,6 +23,8 @@ from . import _lib
 from ._lib import BqError, DT_BF16, DT_F32
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 class PagedKV4:
@@ -62,7 +64,8 @@ class PagedKV4:
             raise ValueError("layers, kv_heads, n_pages, max_seqs and max_pages must be positive")
         if self.max_seqs > 8192 or self.max_pages * self.page > 1 << 30 or self.n_pages >= 1 << 30:
             raise ValueError("a pool holds at most 8192 sequences of 2^30 positions, in fewer than 2^30 pages")
-        self._lib = lib = _lib.init(device.index or 0)
+        self._index = device.index or 0
+        self._lib = lib = _lib.init(self._index)
         self._pool = _lib.Kv4Pool(None, None, None, None, None, self.n_pages, self.max_seqs, self.max_pages, self.layers, self.kv_heads,
                                   self.head_dim, self.page)
         self._p = C.byref(self._pool)
@@ -85,28 +88,31 @@ class PagedKV4:
         """-> int32 CUDA tensor on the pool's device (a sequence of ints is copied there)."""
         if not isinstance(t, torch.Tensor):
             return torch.tensor(t, dtype=torch.int32).to(self.device)
-        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 1:
+        if t.dtype is not torch.int32 or t.device != self.device or t.dim() != 1:
             raise BqError(_lib.ERR_ARG, f"{what} must be a 1-D int32 tensor on {self.device}")
         return t if t.is_contiguous() else t.contiguous()
 
     def _stream(self) -> int:
-        stream = torch.cuda.current_stream()
-        if stream.device != self.device:
-            raise BqError(_lib.ERR_STATE, f"the pool is on {self.device}, the current device is {stream.device}")
-        return stream.cuda_stream
+        if torch.cuda.current_device() != self._index:
+            raise BqError(_lib.ERR_STATE, f"the pool is on {self.device}, the current device is {torch.cuda.current_device()}")
+        return _raw_stream(self._index)
 
     def _batch(self, slots, pos, starts):
+        """-> (slots, pos, starts) on the device, their addresses, B; the tensors are to be kept until the call is made."""
         pos = self._ints(pos, "pos")
         B = pos.numel()
+        at_slots = at_starts = None
         if slots is not None:
             slots = self._ints(slots, "slots")
             if slots.numel() != B:
                 raise ValueError(f"{slots.numel()} slots for {B} positions")
+            at_slots = slots.data_ptr()
         if starts is not None:
             starts = self._ints(starts, "starts")
             if starts.numel() != B + 1:
                 raise ValueError(f"starts must have one entry more than pos ({B}), got {starts.numel()}")
-        return slots, pos, starts, B
+            at_starts = starts.data_ptr()
+        return (slots, pos, starts), at_slots, pos.data_ptr(), at_starts, B
 
     @staticmethod
     def _ptr(t):
@@ -114,17 +120,21 @@ class PagedKV4:
 
     def _rows(self, x, heads: int, what: str):
         """[n_rows, heads, head_dim] whose rows are dense (a slice of a fused projection is; anything else is copied)."""
-        if not x.is_cuda or x.device != self.device:
+        if x.device != self.device:
             raise BqError(_lib.ERR_ARG, f"{what} must be a CUDA tensor on {self.device}")
         if x.dtype not in _DT:
             raise TypeError(f"{what} must be float32 or bfloat16, got {x.dtype}")
-        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != self.head_dim:
-            raise ValueError(f"{what} must be [n_rows, {heads}, {self.head_dim}], got {tuple(x.shape)}")
-        s0, s1, s2 = x.stride()
         D = self.head_dim
-        if x.shape[0] > 1 and (s0 < heads * D or s0 & 7) or s2 != 1 or (heads > 1 and s1 != D) or x.data_ptr() & 15:
-            x = x.clone(memory_format=torch.contiguous_format)
-        return x, (x.stride(0) if x.shape[0] > 1 else heads * D)
+        shape = x.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != D:
+            raise ValueError(f"{what} must be [n_rows, {heads}, {D}], got {tuple(shape)}")
+        dense = heads * D
+        s0, s1, s2 = x.stride()
+        if shape[0] <= 1:
+            s0 = dense
+        if s0 < dense or s0 & 7 or s2 != 1 or (s1 != D and heads > 1) or x.data_ptr() & 15:
+            x, s0 = x.clone(memory_format=torch.contiguous_format), dense
+        return x, s0
 
     # ---- pages --------------------------------------------------------------------------------------------------------
     def extend(self, slots=None, starts=None, batch: int = 0):
@@ -137,7 +147,7 @@ class PagedKV4:
         B = slots.numel() if slots is not None else starts.numel() - 1 if starts is not None else int(batch)
         if starts is not None and starts.numel() != B + 1:
             raise ValueError(f"starts must have one entry more than slots ({B}), got {starts.numel()}")
-        pos = torch.empty(B, dtype=torch.int32, device=self.device)
+        pos = self.lens.new_empty(B)
         _lib.check(self._lib.bq_kv4_extend(self._p, self._ptr(slots), self._ptr(starts), B, pos.data_ptr(), self._stream()))
         return pos
 
@@ -163,18 +173,18 @@ class PagedKV4:
     # ---- rows ---------------------------------------------------------------------------------------------------------
     def append(self, layer: int, k, v, slots, pos, starts=None) -> None:
         """Quantise rows k, v [n_rows, kv_heads, head_dim] (fp32 or bf16) into their positions."""
-        slots, pos, starts, B = self._batch(slots, pos, starts)
+        keep, at_slots, at_pos, at_starts, B = self._batch(slots, pos, starts)
         k, ldk = self._rows(k, self.kv_heads, "k")
         v, ldv = self._rows(v, self.kv_heads, "v")
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
             raise ValueError("k and v must have the same type and number of rows")
-        _lib.check(self._lib.bq_kv4_append(self._p, int(layer), k.data_ptr(), v.data_ptr(), ldk, ldv, _DT[k.dtype], self._ptr(slots),
-                                           pos.data_ptr(), self._ptr(starts), B, k.shape[0], self._stream()))
+        _lib.check(self._lib.bq_kv4_append(self._p, int(layer), k.data_ptr(), v.data_ptr(), ldk, ldv, _DT[k.dtype], at_slots, at_pos,
+                                           at_starts, B, k.shape[0], self._stream()))
 
     def rope_append(self, layer: int, qkv, heads: int, rope_base: float, slots, pos, starts=None, q_out=None, dtype=torch.bfloat16):
         """qkv fp32 [n_rows, (heads + 2 kv_heads) head_dim] of a fused projection: rotates q and k by each row's position,
         quantises k and v into the pages -> q [n_rows, heads, head_dim] in `dtype` (or q_out)."""
-        slots, pos, starts, B = self._batch(slots, pos, starts)
+        keep, at_slots, at_pos, at_starts, B = self._batch(slots, pos, starts)
         if not qkv.is_cuda or qkv.device != self.device or qkv.dtype != torch.float32 or not qkv.is_contiguous():
             raise BqError(_lib.ERR_ARG, f"qkv must be a contiguous fp32 tensor on {self.device}")
         width = (heads + 2 * self.kv_heads) * self.head_dim
@@ -186,40 +196,40 @@ class PagedKV4:
               or q_out.numel() != qkv.shape[0] * heads * self.head_dim):
             raise ValueError("q_out must be a contiguous fp32 or bf16 tensor of n_rows * heads * head_dim elements on the pool's device")
         _lib.check(self._lib.bq_kv4_rope_append(self._p, int(layer), qkv.data_ptr(), q_out.data_ptr(), int(heads), float(rope_base),
-                                                _DT[q_out.dtype], self._ptr(slots), pos.data_ptr(), self._ptr(starts), B, qkv.shape[0],
-                                                self._stream()))
+                                                _DT[q_out.dtype], at_slots, at_pos, at_starts, B, qkv.shape[0], self._stream()))
         return q_out
 
     def gather(self, layer: int, slots, pos, starts=None, rows: int = 0, dtype=torch.float32):
         """What the pages hold (code * scale) of the positions that the rows stand for -> k, v [n_rows, kv_heads, head_dim];
         `rows` gives n_rows where `starts` is given.  Rows of refused sequences, or of none, are left as allocated."""
-        slots, pos, starts, B = self._batch(slots, pos, starts)
+        keep, at_slots, at_pos, at_starts, B = self._batch(slots, pos, starts)
         if dtype not in _DT:
             raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
         n_rows = int(rows) if starts is not None else B
-        k, v = (torch.empty((n_rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
-        _lib.check(self._lib.bq_kv4_gather(self._p, int(layer), k.data_ptr(), v.data_ptr(), _DT[dtype], self._ptr(slots), pos.data_ptr(),
-                                           self._ptr(starts), B, n_rows, self._stream()))
+        shape = (n_rows, self.kv_heads, self.head_dim)
+        k, v = self.lens.new_empty(shape, dtype=dtype), self.lens.new_empty(shape, dtype=dtype)
+        _lib.check(self._lib.bq_kv4_gather(self._p, int(layer), k.data_ptr(), v.data_ptr(), _DT[dtype], at_slots, at_pos, at_starts, B, n_rows,
+                                           self._stream()))
         return k, v
 
     def attention(self, layer: int, q, slots, pos, starts=None, out=None):
         """softmax(q . K^T / sqrt(head_dim)) . V for rows q [n_rows, heads, head_dim] (fp32 or bf16) of the sequences, each
         row over the positions up to its own -> [n_rows, heads, head_dim].  Rows of refused sequences are zero; rows behind
         the last sequence are left as they were."""
-        slots, pos, starts, B = self._batch(slots, pos, starts)
+        keep, at_slots, at_pos, at_starts, B = self._batch(slots, pos, starts)
         if q.dim() != 3 or q.shape[1] % self.kv_heads:
             raise ValueError(f"q must be [n_rows, heads, head_dim] with a multiple of {self.kv_heads} heads, got {tuple(q.shape)}")
         heads = q.shape[1]
         q, ldq = self._rows(q, heads, "q")
         if out is None:
-            out = torch.empty((q.shape[0], heads, self.head_dim), dtype=q.dtype, device=self.device)
+            out = q.new_empty(q.shape)
         elif out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() or out.shape != q.shape:
             raise ValueError("out must be a contiguous tensor like q")
         dt = _DT[q.dtype]
         need = self._attn_bytes.get((heads, dt))
         if need is None:
-            need = self._attn_bytes[(heads, dt)] = int(self._lib.bq_kv4_attention_work_bytes(self._p, heads, dt))
-        work = torch.empty(need, dtype=torch.uint8, device=self.device)
-        _lib.check(self._lib.bq_kv4_attention(self._p, int(layer), q.data_ptr(), ldq, out.data_ptr(), heads, dt, self._ptr(slots),
-                                              pos.data_ptr(), self._ptr(starts), B, q.shape[0], work.data_ptr(), self._stream()))
+            need = self._attn_bytes[(heads, dt)] = int(self._lib.bq_kv4_attention_work_bytes(self._p, heads, dt)) // 4
+        work = self.refs.new_empty(need)                       # of this call alone: calls may overlap
+        _lib.check(self._lib.bq_kv4_attention(self._p, int(layer), q.data_ptr(), ldq, out.data_ptr(), heads, dt, at_slots, at_pos, at_starts, B,
+                                              q.shape[0], work.data_ptr(), self._stream()))
         return out
