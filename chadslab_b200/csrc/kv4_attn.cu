@@ -10,7 +10,7 @@ template <> int ka_pick<float, 4>(const KaArgs& a, int64_t cols, cudaStream_t s)
 template <> int ka_pick<__nv_bfloat16, 4>(const KaArgs& a, int64_t cols, cudaStream_t s);
 template <> int ka_pick<float, 8>(const KaArgs& a, int64_t cols, cudaStream_t s);
 template <> int ka_pick<__nv_bfloat16, 8>(const KaArgs& a, int64_t cols, cudaStream_t s);
-template <typename T, int NG> int ka_pick(const KaArgs& a, int64_t cols, cudaStream_t s) { (void)cols; return ka_launch<T, NG, 8, 1>(a, s); }
+template <typename T, int NG> int ka_pick(const KaArgs& a, int64_t cols, cudaStream_t s) { (void)cols; return ka_launch<T, NG, 8>(a, s); }
 
 template <typename T> static int ka_run(const KaArgs& a, int64_t cols, cudaStream_t s) {
   switch (a.v.D / GROUP) {

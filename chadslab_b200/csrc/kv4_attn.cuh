@@ -303,14 +303,13 @@ __device__ __forceinline__ void ka_store2(__nv_bfloat16* p, float x, float y) {
 constexpr float KA_LO = 1.0f / 2048.0f;               // weight of the second column of an fp32 row
 
 // ---- variants ------------------------------------------------------------------------------------------------------------------
-template <typename T, int NG, int NC, int NT> struct KaCfg {
-  static_assert(NC == 8 || NT == 1, "several column tiles need full ones");
+template <typename T, int NG, int NC> struct KaCfg {
   static constexpr int SL = sizeof(T) == 4 ? 2 : 1;
   static constexpr int D = NG * GROUP;
   static constexpr int GP = 8 / NC < NG ? 8 / NC : NG; // groups side by side in a fragment
   static_assert(NG % GP == 0, "whole fragments");
   static constexpr int NF = NG / GP;
-  static constexpr int W = NC * NT;                   // columns of a tile
+  static constexpr int W = NC;                   // columns of a tile
   static constexpr int HC = W / SL;
   static_assert(W % SL == 0, "an fp32 row takes two columns");
   static constexpr int J = NC == 1 || SL == 2 ? 1 : 2;  // different (row, head) pairs among a lane's two columns
@@ -318,8 +317,10 @@ template <typename T, int NG, int NC, int NT> struct KaCfg {
   static constexpr int BLK = kv4_block_bytes(D);
   static constexpr int QG = NG % 4 == 0 ? NG / 4 : 1;  // groups that are merged over the warps at a time
   static constexpr int OSTR = QG * 32 + 4;            // row pitch of the merge buffer: a quad's columns hit different banks
-  // teams of an SM: what the accumulators (8 NG NT registers) and q (4 NG NT) leave of 64 K registers
-  static constexpr int TEAMS = NG * NT <= (NC == 8 ? 3 : 4) ? 4 : NG * NT <= (NC == 8 ? 5 : 8) ? 3 : 2;
+  // teams of an SM, by the registers that a thread needs: 8 NG accumulators, 4 NG of q, and with eight columns 4 NG more for
+  // starts and weights.  One team more at the price of spills is slower: 32 / 4 heads of 128 take 79 us with four teams of
+  // 128 registers (200 bytes spilled) and 70 with three of 168 (ragged batch of 96)
+  static constexpr int TEAMS = NG <= (NC == 8 ? 3 : 4) ? 4 : NG <= (NC == 8 ? 5 : 8) ? 3 : 2;
   static constexpr int FIXED = KA_WARPS * HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + HC * 12 + (int)sizeof(KaScan) + 128;
   // a warp's step, one stage of its ring: two blocks if the ring then has two stages, else one
   static constexpr int ROOM = (232448 / TEAMS - FIXED) / KA_WARPS;
@@ -329,12 +330,12 @@ template <typename T, int NG, int NC, int NT> struct KaCfg {
   static constexpr int STAGES = ROOM / (STAGE + 8) >= 4 ? 4 : ROOM / (STAGE + 8);
   static_assert(STAGES >= 2, "the ring needs two stages");
   static constexpr int SMEM = (KA_WARPS * STAGES * (STAGE + 8) + FIXED) / 128 * 128;      // of a team
-  static constexpr int U = NT == 1 && NF * NG <= 16 ? STEP : 1;  // blocks whose scores and weights are held at a time
+  static constexpr int U = NF * NG <= 16 ? STEP : 1;  // blocks whose scores and weights are held at a time
 };
 
-template <typename T, int NG, int NC, int NT>
-__global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1) kv4_attention_kernel(const __grid_constant__ KaArgs a) {
-  using C = KaCfg<T, NG, NC, NT>;
+template <typename T, int NG, int NC>
+__global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4_attention_kernel(const __grid_constant__ KaArgs a) {
+  using C = KaCfg<T, NG, NC>;
   constexpr int D = C::D, SL = C::SL, GP = C::GP, NF = C::NF, W = C::W, HC = C::HC, S = C::STAGES, U = C::U, STEP = C::STEP, TILE = C::TILE, J = C::J;
   extern __shared__ __align__(128) uint8_t smem_all[];
   const int team = threadIdx.x / KA_THREADS, tid = threadIdx.x % KA_THREADS;
@@ -413,13 +414,12 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
 
   while (true) {
     // ---- the columns: q as B fragments ------------------------------------------------------------------------------------
-    uint32_t bq[NT][2 * NG][2];
-    float start[NT][NF][2], kappa[NT][2];
-    int vis[NT][2];
+    uint32_t bq[2 * NG][2];
+    float start[NF][2], kappa[2];
+    int vis[2];
     const int cols = seq.n * a.rep * SL;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int c = NC < 8 ? g % NC : nt * 8 + g, gi = NC < 8 ? g / NC : 0;
+    {
+      const int c = NC < 8 ? g % NC : g, gi = NC < 8 ? g / NC : 0;
       const int col = at.ct * W + c, rh = col / SL, i = a.by_rep(rh);
       const bool ok = col < cols;
       const T* qp = static_cast<const T*>(a.q) + (ok ? (int64_t)(seq.row0 + i) * a.ldq + (int64_t)(at.h * a.rep + rh - i * a.rep) * D : 0) + 2 * t;
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
             sum[f] += (back.x + back.y) * ((k & 1) ? 16.0f : 1.0f);
           }
 #pragma unroll
-          for (int o = 0; o < GP; ++o) bq[nt][2 * (f * GP + o) + (k >> 1)][k & 1] = GP == 1 || o == gi ? ka_bits(hx) : 0u;
+          for (int o = 0; o < GP; ++o) bq[2 * (f * GP + o) + (k >> 1)][k & 1] = GP == 1 || o == gi ? ka_bits(hx) : 0u;
         }
       }
       // what the accumulator layout needs of columns 2t and 2t + 1
@@ -468,8 +468,8 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
       const int see = ok ? seq.pos + i : 0x7FFFFFFF;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        kappa[nt][j] = __shfl_sync(0xffffffffu, kap, (2 * t + j) * 4);
-        vis[nt][j] = __shfl_sync(0xffffffffu, see, (2 * t + j) * 4);
+        kappa[j] = __shfl_sync(0xffffffffu, kap, (2 * t + j) * 4);
+        vis[j] = __shfl_sync(0xffffffffu, see, (2 * t + j) * 4);
       }
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
@@ -478,25 +478,24 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
         z += __shfl_xor_sync(0xffffffffu, z, 2);
         z *= C::SUBNORMAL ? -8.0f / 16777216.0f : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) start[nt][f][j] = __shfl_sync(0xffffffffu, z, (2 * t + j) * 4);
+        for (int j = 0; j < 2; ++j) start[f][j] = __shfl_sync(0xffffffffu, z, (2 * t + j) * 4);
       }
     }
     const int all_see = seq.pos + a.by_row(at.ct * W);        // every column sees positions up to here
 
     // ---- the positions ----------------------------------------------------------------------------------------------------
-    float acc[NT][2 * NG][4], ref[NT][2], l[NT][2];
+    float acc[2 * NG][4], ref[2], l[2];
     float A = 11.0f;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    {
 #pragma unroll
       for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[nt][i][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         // a column without a row has no weight anywhere: it must not take part in the search for a reference
-        ref[nt][j] = vis[nt][j] == 0x7FFFFFFF ? 3.0e38f : -3.0e38f;
-        l[nt][j] = 0.0f;
+        ref[j] = vis[j] == 0x7FFFFFFF ? 3.0e38f : -3.0e38f;
+        l[j] = 0.0f;
       }
     }
     for (int i = 0; i < mine; ++i) {
@@ -512,18 +511,17 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
         const uint8_t* blk0 = stage + u0 * C::BLK;
         const int p0 = step0 + u0 * KV4_ROWS;
         // scores
-        float s[U][NT][4];
+        float s[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const uint8_t* blk = blk0 + u * C::BLK;
           uint2 kq0, kq1;
 #pragma unroll
           for (int f = 0; f < NF; ++f) {
-            float c[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              c[nt][0] = c[nt][2] = start[nt][f][0];
-              c[nt][1] = c[nt][3] = start[nt][f][1];
+            float c[4];
+            {
+              c[0] = c[2] = start[f][0];
+              c[1] = c[3] = start[f][1];
             }
 #pragma unroll
             for (int gi = 0; gi < GP; ++gi) {
@@ -538,8 +536,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
                 } else {
                   r0 = ka_code(w); r1 = ka_code16(w); r2 = ka_code(x); r3 = ka_code16(x);
                 }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) ka_mma(c[nt], r0, r2, r1, r3, bq[nt][2 * G + h][0], bq[nt][2 * G + h][1]);
+                ka_mma(c, r0, r2, r1, r3, bq[2 * G + h][0], bq[2 * G + h][1]);
               }
             }
             // scales of rows g and g + 8: of the column's group, or (NC == 1) of the two columns' groups
@@ -562,20 +559,18 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
               k0.x = k0.y = __half2float(ks[g * NG + G]);
               k1.x = k1.y = __half2float(ks[(g + 8) * NG + G]);
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              s[u][nt][0] = f ? fmaf(k0.x, c[nt][0], s[u][nt][0]) : k0.x * c[nt][0];
-              s[u][nt][1] = f ? fmaf(k0.y, c[nt][1], s[u][nt][1]) : k0.y * c[nt][1];
-              s[u][nt][2] = f ? fmaf(k1.x, c[nt][2], s[u][nt][2]) : k1.x * c[nt][2];
-              s[u][nt][3] = f ? fmaf(k1.y, c[nt][3], s[u][nt][3]) : k1.y * c[nt][3];
+            {
+              s[u][0] = f ? fmaf(k0.x, c[0], s[u][0]) : k0.x * c[0];
+              s[u][1] = f ? fmaf(k0.y, c[1], s[u][1]) : k0.y * c[1];
+              s[u][2] = f ? fmaf(k1.x, c[2], s[u][2]) : k1.x * c[2];
+              s[u][3] = f ? fmaf(k1.y, c[3], s[u][3]) : k1.y * c[3];
             }
           }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float* z = s[u][nt];
+          {
+            float* z = s[u];
             if (NC == 1) {
               z[0] += z[1];
               z[2] += z[3];
@@ -602,14 +597,12 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
 #pragma unroll
           for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
               for (int j = 0; j < 4; ++j)
-                if ((J == 2 || !(j & 1)) && p0 + u * KV4_ROWS + g + (j >> 1) * 8 > vis[nt][j & 1]) s[u][nt][j] = -INFINITY;
+                if ((J == 2 || !(j & 1)) && p0 + u * KV4_ROWS + g + (j >> 1) * 8 > vis[j & 1]) s[u][j] = -INFINITY;
         }
         // weights; wv = weight * scale of the values, the B fragments of the second product
-        float p[U][NT][4];
-        uint32_t wv[U][NT][NF][2];
+        float p[U][4];
+        uint32_t wv[U][NF][2];
 #pragma unroll 1
         for (int tries = 0;; ++tries) {
           float high = -INFINITY;
@@ -617,13 +610,12 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const uint8_t* vsc = blk0 + u * C::BLK + kv4_vscale_off(D) + (g / NC < GP ? g / NC : 0) * 32 + t * 8;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float* w = p[u][nt];
+            {
+              float* w = p[u];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 if (J == 1 && (j & 1)) { w[j] = w[j - 1]; continue; }
-                w[j] = fmaf(s[u][nt][j], kappa[nt][j & 1], -ref[nt][j & 1]);
+                w[j] = fmaf(s[u][j], kappa[j & 1], -ref[j & 1]);
                 high = fmaxf(high, w[j]);
                 w[j] = ka_exp2(w[j]);
               }
@@ -642,17 +634,17 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
                   const uint2 vs = *reinterpret_cast<const uint2*>(vsc + f * GP * 32);
-                  wv[u][nt][f][0] = ka_mul2(m0, vs.x);
-                  wv[u][nt][f][1] = ka_mul2(m1, vs.y);
+                  wv[u][f][0] = ka_mul2(m0, vs.x);
+                  wv[u][f][1] = ka_mul2(m1, vs.y);
                 }
                 if (masked) {                                  // a scale behind the last position can be anything: no weight, no product
                   const uint32_t live0 = __hne2_mask(ka_half2(m0), __floats2half2_rn(0.0f, 0.0f));
                   const uint32_t live1 = __hne2_mask(ka_half2(m1), __floats2half2_rn(0.0f, 0.0f));
 #pragma unroll
-                  for (int f = 0; f < NF; ++f) { wv[u][nt][f][0] &= live0; wv[u][nt][f][1] &= live1; }
+                  for (int f = 0; f < NF; ++f) { wv[u][f][0] &= live0; wv[u][f][1] &= live1; }
                 }
 #pragma unroll
-                for (int f = 0; f < NF; ++f) top = __hmax2(top, __hmax2(ka_half2(wv[u][nt][f][0]), ka_half2(wv[u][nt][f][1])));
+                for (int f = 0; f < NF; ++f) top = __hmax2(top, __hmax2(ka_half2(wv[u][f][0]), ka_half2(wv[u][f][1])));
               } else {
                 // the partner lane holds the other half of the same weight: 22 bits times the scale, split again
                 const uint32_t o0 = __shfl_xor_sync(0xffffffffu, m0, 4), o1 = __shfl_xor_sync(0xffffffffu, m1, 4);
@@ -673,8 +665,8 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
                     if (h > 60000.0f) top = __floats2half2_rn(65504.0f, 65504.0f);
                     z[j] = odd ? (z[j] - h) * 2048.0f : h;
                   }
-                  wv[u][nt][f][0] = ka_pack(z[0], z[1]);
-                  wv[u][nt][f][1] = ka_pack(z[2], z[3]);
+                  wv[u][f][0] = ka_pack(z[0], z[1]);
+                  wv[u][f][1] = ka_pack(z[2], z[3]);
                 }
               }
             }
@@ -686,36 +678,33 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
           const float drop = tries ? 4.0f : 0.0f;
           A -= drop;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
             for (int j = 0; j < 2; ++j) {
               if (J == 1 && j) {
-                ref[nt][1] = ref[nt][0];
+                ref[1] = ref[0];
                 continue;
               }
               float m = -INFINITY;
 #pragma unroll
-              for (int u = 0; u < U; ++u) m = fmaxf(m, fmaxf(s[u][nt][j], s[u][nt][j + 2]));
-              m *= kappa[nt][j];
+              for (int u = 0; u < U; ++u) m = fmaxf(m, fmaxf(s[u][j], s[u][j + 2]));
+              m *= kappa[j];
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-              const float r = fmaxf(ref[nt][j] + drop, m - A), corr = ka_exp2(ref[nt][j] - r);
-              ref[nt][j] = r;
-              l[nt][j] *= corr;
+              const float r = fmaxf(ref[j] + drop, m - A), corr = ka_exp2(ref[j] - r);
+              ref[j] = r;
+              l[j] *= corr;
 #pragma unroll
               for (int x = 0; x < 2 * NG; ++x) {
-                acc[nt][x][j] *= corr; acc[nt][x][j + 2] *= corr;
-                if (J == 1) { acc[nt][x][1] *= corr; acc[nt][x][3] *= corr; }
+                acc[x][j] *= corr; acc[x][j + 2] *= corr;
+                if (J == 1) { acc[x][1] *= corr; acc[x][3] *= corr; }
               }
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            l[nt][0] += p[u][nt][0] + p[u][nt][2];
-            if (J == 2) l[nt][1] += p[u][nt][1] + p[u][nt][3];
+          {
+            l[0] += p[u][0] + p[u][2];
+            if (J == 2) l[1] += p[u][1] + p[u][3];
           }
         // values
 #pragma unroll
@@ -727,9 +716,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
             for (int h = 0; h < 2; ++h) {
               const uint32_t w = h ? w2.y : w2.x, x = w >> 8;
               const uint32_t r0 = ka_code(w), r1 = ka_code16(w), r2 = ka_code(x), r3 = ka_code16(x);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                ka_mma(acc[nt][2 * G + h], r0, r1, r2, r3, wv[u][nt][G / GP][0], wv[u][nt][G / GP][1]);
+                ka_mma(acc[2 * G + h], r0, r1, r2, r3, wv[u][G / GP][0], wv[u][G / GP][1]);
             }
           }
       }
@@ -777,30 +764,26 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
 
     // ---- the four warps' states become one ---------------------------------------------------------------------------------------
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float z = l[nt][j];
+        float z = l[j];
         z += __shfl_xor_sync(0xffffffffu, z, 4);
         z += __shfl_xor_sync(0xffffffffu, z, 8);
         z += __shfl_xor_sync(0xffffffffu, z, 16);
         const int n = 2 * t + j;
         if (g == 0 && n < NC) {
-          s_ref[warp * W + nt * 8 + n] = ref[nt][j];
-          s_sum[warp * W + nt * 8 + n] = z;
+          s_ref[warp * W + n] = ref[j];
+          s_sum[warp * W + n] = z;
         }
       }
     ka_sync(team);
-    float corr[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    float corr[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int c = nt * 8 + (NC < 8 ? (2 * t + j) % NC : 2 * t + j);
+        const int c = (NC < 8 ? (2 * t + j) % NC : 2 * t + j);
         float r = s_ref[c];
 #pragma unroll
         for (int w = 1; w < KA_WARPS; ++w) r = fmaxf(r, s_ref[w * W + c]);
-        corr[nt][j] = ka_exp2(ref[nt][j] - r) * (SL == 2 && j ? KA_LO : 1.0f);
+        corr[j] = ka_exp2(ref[j] - r) * (SL == 2 && j ? KA_LO : 1.0f);
       }
     // (row, head) hc = column hc * SL of the tile: its reference and sum, and where its output goes
     float* part = a.part + ((int64_t)run * 2 + (begins ? 1 : 0)) * (HC * (D + 4));
@@ -827,27 +810,25 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC, NT>::TEAMS * KA_THREADS), 1)
     for (int G0 = 0; G0 < NG; G0 += C::QG) {
       constexpr int QD = C::QG * 32, QSTR = C::OSTR;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
         for (int G = G0; G < G0 + C::QG; ++G) {
           const int n0 = 2 * t;                                // this lane's columns n0, n0 + 1; group G % GP owns NC of them
           if (NC < 8 && (NC == 1 ? (n0 >> 1) != (G % GP) >> 1 : n0 / NC != G % GP)) continue;
-          const int c0 = nt * 8 + (NC < 8 ? n0 % NC : n0);
+          const int c0 = (NC < 8 ? n0 % NC : n0);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float* x = acc[nt][2 * G + h];
+            const float* x = acc[2 * G + h];
             float* o = s_o + (warp * HC + c0 / SL) * QSTR + (G - G0) * 32 + h * 16 + g;
             if (SL == 2) {
-              o[0] = x[0] * corr[nt][0] + x[1] * corr[nt][1];
-              o[8] = (x[2] * corr[nt][0] + x[3] * corr[nt][1]) * 0.0625f;
+              o[0] = x[0] * corr[0] + x[1] * corr[1];
+              o[8] = (x[2] * corr[0] + x[3] * corr[1]) * 0.0625f;
             } else if (NC == 1) {
-              o[0] = (G & 1 ? x[1] : x[0]) * corr[nt][0];
-              o[8] = (G & 1 ? x[3] : x[2]) * (corr[nt][0] * 0.0625f);
+              o[0] = (G & 1 ? x[1] : x[0]) * corr[0];
+              o[8] = (G & 1 ? x[3] : x[2]) * (corr[0] * 0.0625f);
             } else {
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                o[j * QSTR] = x[j] * corr[nt][j];
-                o[j * QSTR + 8] = x[j + 2] * (corr[nt][j] * 0.0625f);
+                o[j * QSTR] = x[j] * corr[j];
+                o[j * QSTR + 8] = x[j + 2] * (corr[j] * 0.0625f);
               }
             }
           }
@@ -952,15 +933,15 @@ __global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(c
   }
 }
 
-constexpr int KA_MAX_TEAMS = 4, KA_MAX_WIDTH = 16;    // of any variant
+constexpr int KA_MAX_TEAMS = 4, KA_MAX_WIDTH = 8;      // of any variant
 
-template <typename T, int NG, int NC, int NT>
+template <typename T, int NG, int NC>
 int ka_launch(KaArgs a, cudaStream_t s) {
-  using C = KaCfg<T, NG, NC, NT>;
+  using C = KaCfg<T, NG, NC>;
   static_assert(C::TEAMS <= KA_MAX_TEAMS && C::W <= KA_MAX_WIDTH, "the caller's scratch is sized for these");
   static bool sized = false;
   if (!sized) {
-    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TEAMS * C::SMEM));
+    BQ_CUDA(cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TEAMS * C::SMEM));
     sized = true;
   }
   a.by_rep = ka_div(a.rep);
@@ -974,7 +955,7 @@ int ka_launch(KaArgs a, cudaStream_t s) {
   int64_t grid = sm_count();
   if (grid > KA_MAX_RUNS / C::TEAMS) grid = KA_MAX_RUNS / C::TEAMS;
   if ((double)grid * KA_MIN_TILES > most) grid = ((int64_t)most + KA_MIN_TILES - 1) / KA_MIN_TILES;
-  BQ_CUDA(launch_chain(kv4_attention_kernel<T, NG, NC, NT>, dim3((unsigned)grid), dim3(C::TEAMS * KA_THREADS), C::TEAMS * C::SMEM, s, 1, a));
+  BQ_CUDA(launch_chain(kv4_attention_kernel<T, NG, NC>, dim3((unsigned)grid), dim3(C::TEAMS * KA_THREADS), C::TEAMS * C::SMEM, s, 1, a));
   BQ_CUDA(launch_chain(kv4_attention_merge_kernel<T>, dim3((unsigned)(grid * C::TEAMS - 1), (unsigned)C::HC), dim3(KA_MERGE_THREADS), 0, s, 1, a));
   count_launch(2);
   BQ_CUDA(cudaGetLastError());
