@@ -134,9 +134,9 @@ def _headline(torch, dist, rank, world, dec, cfg, B, ctx, step, tokens, steps, m
 
 
 def run(torch, dist, rank: int, world: int, shape: str = "gemma7b", batches=(1, 16, 64), ctx: int = 2048, steps: int = 16,
-        eager: bool = False, warmup: int = 3, headline_batch=None):
+        eager: bool = False, warmup: int = 3, headline_batch=None, kv_bits: int = 0):
     """Runs on every rank; returns the report (complete on rank 0).  `headline_batch`: also measure that batch end to
-    end from host buffers and time its largest quantized-matmul launch alone (`headline` in the report)."""
+    end from host buffers and time its largest quantized-matmul launch alone (`headline` in the report).  `kv_bits` 4: the cache is held in 4-bit pages."""
     import chadslab_b200 as cb
     from chadslab_b200 import _lib
     from chadslab_b200.decoder import GEMMA_2B_SHAPE, GEMMA_7B_SHAPE, QuantDecoder
@@ -155,16 +155,29 @@ def run(torch, dist, rank: int, world: int, shape: str = "gemma7b", batches=(1, 
             _lib.check(_lib.lib().bq_comm_set_timeout_ms(comm.handle, 1000))   # a benchmark should fail fast
         spare = warmup + 2 * steps + 16            # cache rows behind the context: every step of a batch size writes one
         dec = QuantDecoder.random(cfg, seed=0, act_dtype=torch.bfloat16, rank=rank, world=world, max_seq=ctx + spare,
-                                  max_batch=max_b, comm=comm)
-        for kc, vc in zip(dec.k_cache, dec.v_cache):
-            kc.normal_()
-            vc.normal_()
+                                  max_batch=max_b, comm=comm, kv_bits=kv_bits)
+        if kv_bits == 4:
+            k, v = (torch.randn((max_b * ctx, dec.kv_local, cfg.head_dim), device="cuda").to(torch.bfloat16) for _ in range(2))
+            starts = torch.arange(0, (max_b + 1) * ctx, ctx, dtype=torch.int32, device="cuda")
+            pos = dec.kv.extend(None, starts)
+            for l in range(cfg.layers):
+                dec.kv.append(l, k, v, None, pos, starts)
+            del k, v
+            out["kv_bits"] = 4
+            kv_bytes = cfg.layers * ctx * dec.kv_local * cfg.head_dim * 9 / 8        # K + V codes and scales, per sequence
+        else:
+            for kc, vc in zip(dec.k_cache, dec.v_cache):
+                kc.normal_()
+                vc.normal_()
+            kv_bytes = sum(k[:1, :ctx].numel() * k.element_size() for k in dec.k_cache) * 2      # K + V, per sequence
         bpt = dec.linear_bytes_per_token()
-        kv_bytes = sum(k[:1, :ctx].numel() * k.element_size() for k in dec.k_cache) * 2      # K + V, per sequence
         for B in batches:
             g = torch.Generator(device="cuda").manual_seed(B)
             first = torch.randint(0, cfg.vocab, (B,), device="cuda", generator=g)
             dec.pos = ctx
+            if dec.kv is not None:
+                dec.kv.free(range(max_b))                # forget the rows of the batch size before: the same pages are given out
+                dec.kv.extend(None, starts)              # again, in the same order
             if eager:
                 tokens = first.clone()
                 pos_t = torch.tensor([ctx], device="cuda", dtype=torch.int64)
@@ -273,6 +286,7 @@ def main():
     ap.add_argument("--eager", type=int, default=0)
     ap.add_argument("--prefill", default="", help="BxT: time a prefill pass instead (e.g. 8x4096)")
     ap.add_argument("--fmt", default="", choices=["", "int8", "q4"], help="prefill: weight format (default: the shape's)")
+    ap.add_argument("--kv-bits", type=int, default=0, choices=[0, 4], help="4: the KV cache in pages of 4-bit codes")
     args = ap.parse_args()
     world, rank = int(os.environ.get("WORLD_SIZE", "1")), int(os.environ.get("RANK", "0"))
     local = int(os.environ.get("LOCAL_RANK", "0"))
@@ -286,7 +300,7 @@ def main():
         rep = run_prefill(torch, dist, rank, world, args.shape, fmt, B, T)
     else:
         rep = run(torch, dist, rank, world, args.shape, tuple(int(b) for b in args.batch.split(",")), args.ctx, args.steps,
-                  bool(args.eager))
+                  bool(args.eager), kv_bits=args.kv_bits)
     if rank == 0:
         print(json.dumps(rep))
     if world > 1:

@@ -9,6 +9,8 @@ Prefill runs the glue between the matmuls in PyTorch; the decode step (`_step_st
 kernels and is captured in a CUDA graph.
 Architecture choices the specification leaves open: norm weights multiply the normalised value directly, eps 1e-6,
 no embedding scaling, no logit soft-capping, rotate-half RoPE with base 10000, untied embedding table.
+`kv_bits=4` keeps the KV cache in pages of 4-bit codes (`kv4.PagedKV4`) instead of dense rows of the activation type: a
+prompt attends to its own exact keys and values, everything after it to what the pages hold.
 """
 from __future__ import annotations
 
@@ -21,6 +23,7 @@ import torch
 import torch.nn.functional as F
 
 from . import parallel
+from .kv4 import PagedKV4
 from .ops import LMHead, PackedWeight, QuantLinear, interleave_gate_up, shard, split_gate_up
 from .synth import make_device_weight
 
@@ -65,7 +68,7 @@ def _rope(x, pos, base):
 
 class QuantDecoder:
     def __init__(self, cfg: DecoderConfig, lin: dict, embed, norms: dict, act_dtype=torch.bfloat16, rank: int = 0,
-                 world: int = 1, max_seq: int = 4096, max_batch: int = 1, comm=None):
+                 world: int = 1, max_seq: int = 4096, max_batch: int = 1, comm=None, kv_bits: int = 0, kv_page: int = 64):
         self.cfg, self.lin, self.embed, self.norms = cfg, lin, embed, norms
         # ops.PeerComm (optional, world > 1): the static decode step then sums the row-parallel partial products
         # through peer memory (GEMV deposits -> fused sum + residual add + RMSNorm) instead of NCCL all-reduces
@@ -75,11 +78,23 @@ class QuantDecoder:
         self.h_local = cfg.n_heads // world
         self.kv_local = cfg.n_kv_heads // world if self.kv_sharded else cfg.n_kv_heads
         self.ffn_local = cfg.ffn // world
-        dev = embed.device
-        self.k_cache = [torch.zeros((max_batch, max_seq, self.kv_local, cfg.head_dim), dtype=act_dtype, device=dev)
-                        for _ in range(cfg.layers)]
-        self.v_cache = [torch.zeros_like(self.k_cache[0]) for _ in range(cfg.layers)]
-        self.pos = 0
+        self._make_cache(max_batch, max_seq, kv_bits, kv_page)
+
+    def _make_cache(self, max_batch: int, max_seq: int, kv_bits: int, kv_page: int):
+        """kv_bits 0: dense rows in the activation type; 4: a PagedKV4 with room for every sequence (self.kv)."""
+        if kv_bits not in (0, 4):
+            raise ValueError(f"kv_bits={kv_bits}: the cache is held in the activation type (0) or in 4 bits (4)")
+        c, dev = self.cfg, self.embed.device
+        self.max_batch, self.max_seq, self.pos, self.kv = max_batch, max_seq, 0, None
+        if kv_bits == 4:
+            per_seq = -(-max_seq // kv_page)
+            # one page more per sequence: a shared last page is copied by all that share it before it is given up
+            self.kv = PagedKV4(c.layers, self.kv_local, c.head_dim, n_pages=max_batch * (per_seq + 1), max_seqs=max_batch, max_pages=per_seq,
+                               page=kv_page, device=dev)
+            return
+        self.k_cache = [torch.zeros((max_batch, max_seq, self.kv_local, c.head_dim), dtype=self.act_dtype, device=dev)
+                        for _ in range(c.layers)]
+        self.v_cache = [torch.zeros_like(self.k_cache[0]) for _ in range(c.layers)]
 
     # ---- construction -------------------------------------------------------------------------------
     @staticmethod
@@ -153,13 +168,56 @@ class QuantDecoder:
     # ---- forward ---------------------------------------------------------------------------------------
     def reset(self):
         self.pos = 0
+        if self.kv is not None:
+            self.kv.free(range(self.max_batch))
+
+    def share_prefix(self, batch: int):
+        """After a prompt run alone (batch 1): sequences 0 .. batch-1 all continue it.  They share its pages until they write."""
+        if self.kv is None:
+            raise ValueError("share_prefix() needs the paged cache (kv_bits=4)")
+        if not 1 <= batch <= self.max_batch:
+            raise ValueError(f"the cache holds {self.max_batch} sequences, asked for {batch}")
+        if batch > 1:
+            self.kv.fork([0] * (batch - 1), range(1, batch))
+
+    def _cached_attention(self, l, q, k, v, rows, b0: int = 0):
+        """Appends k, v [B, T, heads, d] at self.pos of sequences b0 .. b0+B-1 of layer l and attends q to them and everything
+        before -> [B, T, heads, d].  `rows`: the paged cache's (slots, pos, starts) of this pass."""
+        B, T = q.shape[:2]
+        S = self.pos + T
+        if self.kv is not None:
+            self.kv.append(l, k.flatten(0, 1), v.flatten(0, 1), *rows)
+            if self.pos or T == 1:
+                return self.kv.attention(l, q.flatten(0, 1), *rows).unflatten(0, (B, T))
+            kk, vv = k, v
+        else:
+            self.k_cache[l][b0:b0 + B, self.pos:S] = k
+            self.v_cache[l][b0:b0 + B, self.pos:S] = v
+            kk, vv = self.k_cache[l][b0:b0 + B, :S], self.v_cache[l][b0:b0 + B, :S]
+        rep = q.shape[2] // kk.shape[2]
+        if rep > 1:
+            kk, vv = kk.repeat_interleave(rep, dim=2), vv.repeat_interleave(rep, dim=2)
+        if self.pos == 0 and T > 1:      # no earlier context: plain causal attention (lets PyTorch pick a fused kernel)
+            o = F.scaled_dot_product_attention(q.transpose(1, 2), kk.transpose(1, 2), vv.transpose(1, 2), is_causal=True)
+        else:
+            mask = torch.arange(S, device=q.device)[None, :] <= torch.arange(self.pos, S, device=q.device)[:, None]      # [T, S]
+            o = F.scaled_dot_product_attention(q.transpose(1, 2), kk.transpose(1, 2), vv.transpose(1, 2), attn_mask=mask)
+        return o.transpose(1, 2)
+
+    def _new_rows(self, B: int, T: int, b0: int = 0):
+        """Room for T more rows of sequences b0 .. b0+B-1 of the paged cache -> (slots, pos, starts)."""
+        if self.kv is None:
+            return None
+        slots = torch.arange(b0, b0 + B, dtype=torch.int32, device=self.embed.device)
+        starts = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device=self.embed.device)
+        return slots, self.kv.extend(slots, starts), starts
 
     def hidden_states(self, tokens):
         """tokens int64 [B, T] -> final normalised hidden states [B, T, hidden]; appends to the KV cache."""
         c = self.cfg
         B, T = tokens.shape
-        if self.pos + T > self.k_cache[0].shape[1] or B > self.k_cache[0].shape[0]:
-            raise ValueError(f"KV cache holds {self.k_cache[0].shape[1]} positions x {self.k_cache[0].shape[0]} sequences; "
+        if self.pos + T > self.max_seq or B > self.max_batch:
+            raise ValueError(f"KV cache holds {self.max_seq} positions x {self.max_batch} sequences; "
                              f"asked for positions {self.pos}..{self.pos + T - 1} of {B} sequences")
         M = B * T
         x = self.embed[tokens].to(self.act_dtype).reshape(M, c.hidden).contiguous()      # residual stream
@@ -167,7 +225,7 @@ class QuantDecoder:
         pos = torch.arange(self.pos, self.pos + T, device=x.device)
         S = self.pos + T
         nq, nkv = self.h_local * c.head_dim, self.kv_local * c.head_dim
-        rep = self.h_local // self.kv_local
+        rows = self._new_rows(B, T)
         delta = None
         for l in range(c.layers):
             self._add_norm(x, delta, self.norms[f"l{l}.norm1"], h)                        # x += delta; h = rmsnorm(x) * w
@@ -176,17 +234,8 @@ class QuantDecoder:
             k = qkv[:, nq:nq + nkv].reshape(B, T, self.kv_local, c.head_dim)
             v = qkv[:, nq + nkv:].reshape(B, T, self.kv_local, c.head_dim)
             q, k = _rope(q, pos, c.rope_base), _rope(k, pos, c.rope_base)
-            self.k_cache[l][:B, self.pos:S] = k
-            self.v_cache[l][:B, self.pos:S] = v
-            kk, vv = self.k_cache[l][:B, :S], self.v_cache[l][:B, :S]
-            if rep > 1:
-                kk, vv = kk.repeat_interleave(rep, dim=2), vv.repeat_interleave(rep, dim=2)
-            if self.pos == 0 and T > 1:      # no earlier context: plain causal attention (lets PyTorch pick a fused kernel)
-                o = F.scaled_dot_product_attention(q.transpose(1, 2), kk.transpose(1, 2), vv.transpose(1, 2), is_causal=True)
-            else:
-                mask = (torch.arange(S, device=x.device)[None, :] <= pos[:, None])      # [T, S]
-                o = F.scaled_dot_product_attention(q.transpose(1, 2), kk.transpose(1, 2), vv.transpose(1, 2), attn_mask=mask)
-            o = o.transpose(1, 2).reshape(M, self.h_local * c.head_dim)
+            o = self._cached_attention(l, q, k, v, rows)
+            o = o.reshape(M, self.h_local * c.head_dim)
             delta = self.lin[f"l{l}.o"](o.contiguous())                                   # fp32 (summed over the ranks when sharded)
             self._add_norm(x, delta, self.norms[f"l{l}.norm2"], h)
             a = self.lin[f"l{l}.gate_up"].gated(h, 0)                                     # GeGLU applied inside the matmul kernel
@@ -239,11 +288,12 @@ class QuantDecoder:
         from .ops import _dt_of_torch, _stream_ptr
         c, lib, st = self.cfg, _lib.lib(), _stream_ptr()
         B = tokens.shape[0]
-        dt = _dt_of_torch(self.k_cache[0])
         dev = tokens.device
         x = self.embed[tokens].to(self.act_dtype).contiguous()                    # residual stream [B, hidden]
+        dt = _dt_of_torch(x)
         h = torch.empty_like(x)
-        S = self.k_cache[0].shape[1]
+        S = self.max_seq
+        at = None if self.kv is None else self.kv.extend(batch=B)
         att = torch.empty((B, self.h_local, c.head_dim), dtype=self.act_dtype, device=dev)
         act = torch.empty((B, self.ffn_local), dtype=self.act_dtype, device=dev)
         comm = self.comm if self.world > 1 else None
@@ -266,10 +316,13 @@ class QuantDecoder:
         for l in range(c.layers):
             add_norm(delta, self.norms[f"l{l}.norm1"])
             qkv = self.lin[f"l{l}.qkv"](h)                                        # fp32 [B, (Hq + 2 Hkv) D]
-            # RoPE, KV append and single-query attention in one launch
-            _lib.check(lib.bq_decode_attention_rope(qkv.data_ptr(), self.k_cache[l].data_ptr(), self.v_cache[l].data_ptr(),
-                                                    pos_t.data_ptr(), att.data_ptr(), B, self.h_local, self.kv_local,
-                                                    c.head_dim, S, c.rope_base, dt, st))
+            if self.kv is not None:
+                q = self.kv.rope_append(l, qkv, self.h_local, c.rope_base, None, at, dtype=self.act_dtype)
+                self.kv.attention(l, q, None, at, out=att)
+            else:                          # RoPE, KV append and single-query attention in one launch
+                _lib.check(lib.bq_decode_attention_rope(qkv.data_ptr(), self.k_cache[l].data_ptr(), self.v_cache[l].data_ptr(),
+                                                        pos_t.data_ptr(), att.data_ptr(), B, self.h_local, self.kv_local,
+                                                        c.head_dim, S, c.rope_base, dt, st))
             delta = row_parallel(f"l{l}.o", att.reshape(B, -1))
             add_norm(delta, self.norms[f"l{l}.norm2"])
             self.lin[f"l{l}.gate_up"].gated(h, 0, out=act)                         # GeGLU in the GEMV's epilogue
@@ -284,7 +337,7 @@ class QuantDecoder:
         pos_t.add_(1)
 
     def _check_graph_room(self, batch: int, start_pos: int):
-        S, Bmax = self.k_cache[0].shape[1], self.k_cache[0].shape[0]
+        S, Bmax = self.max_seq, self.max_batch
         if batch > Bmax or start_pos + 2 > S:
             raise ValueError(f"KV cache holds {S} positions x {Bmax} sequences: no room to capture a step at position "
                              f"{start_pos} for {batch} sequences")
@@ -297,11 +350,15 @@ class QuantDecoder:
         issued next to the launch on the same stream costs ~0.4 ms of start-up per step, measured)."""
         dev = self.embed.device
         self._check_graph_room(batch, start_pos)
+        if self.kv is not None and not bool((self.kv.lens[:batch] == start_pos).all()):
+            raise ValueError(f"not all of sequences 0..{batch - 1} are at position {start_pos}")
         tokens = first_tokens.to(dev).long().clone()
         pos_t = torch.tensor([start_pos], device=dev, dtype=torch.int64)
-        # the two trial steps below (warm-up, capture) write cache positions start_pos and start_pos + 1 only
+        # the trial step below (warm-up) writes cache positions start_pos and start_pos + 1 only; the paged cache takes pages
+        # for them and writes no page that is in use elsewhere, so its bookkeeping is all there is to put back
         sl = (slice(0, batch), slice(start_pos, start_pos + 2))
-        keep = (tokens.clone(), pos_t.clone(), [k[sl].clone() for k in self.k_cache], [v[sl].clone() for v in self.v_cache])
+        caches = [self.kv.tables, self.kv.lens, self.kv.refs] if self.kv is not None else [t[sl] for t in self.k_cache + self.v_cache]
+        keep = (tokens.clone(), pos_t.clone(), [t.clone() for t in caches])
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         if (host_in is not None and not host_in.is_pinned()) or (host_out is not None and not host_out.is_pinned()):
@@ -321,13 +378,11 @@ class QuantDecoder:
             body()
         # restore the state the two trial steps consumed
         tokens.copy_(keep[0]); pos_t.copy_(keep[1])
-        for dst, src in zip(self.k_cache, keep[2]):
-            dst[sl].copy_(src)
-        for dst, src in zip(self.v_cache, keep[3]):
-            dst[sl].copy_(src)
+        for dst, src in zip(caches, keep[2]):
+            dst.copy_(src)
         self.pos = start_pos
 
-        S = self.k_cache[0].shape[1]
+        S = self.max_seq
 
         def step():
             if self.pos >= S:
@@ -353,16 +408,12 @@ class MoEDecoder(QuantDecoder):
     and back through `ops.PeerEP` (device-side stores into peer memory, no host step per layer)."""
 
     def __init__(self, cfg: DecoderConfig, lin: dict, moe: list, embed, norms: dict, act_dtype=torch.bfloat16, rank: int = 0,
-                 world: int = 1, max_seq: int = 4096, max_batch: int = 1, ep=None, keep=None):
+                 world: int = 1, max_seq: int = 4096, max_batch: int = 1, ep=None, keep=None, kv_bits: int = 0, kv_page: int = 64):
         self.cfg, self.lin, self.moe, self.embed, self.norms = cfg, lin, moe, embed, norms
         self.comm, self.ep, self._keep = None, ep, keep
         self.act_dtype, self.rank, self.world = act_dtype, rank, world
         self.h_local, self.kv_local, self.kv_sharded = cfg.n_heads, cfg.n_kv_heads, False
-        dev = embed.device
-        self.k_cache = [torch.zeros((max_batch, max_seq, cfg.n_kv_heads, cfg.head_dim), dtype=act_dtype, device=dev)
-                        for _ in range(cfg.layers)]
-        self.v_cache = [torch.zeros_like(self.k_cache[0]) for _ in range(cfg.layers)]
-        self.pos = 0
+        self._make_cache(max_batch, max_seq, kv_bits, kv_page)
         if world > 1:
             if ep is None:
                 raise ValueError("expert parallel needs an ops.PeerEP exchange object")
@@ -447,15 +498,15 @@ class MoEDecoder(QuantDecoder):
         c = self.cfg
         B, T = tokens.shape
         S = self.pos + T
-        if S > self.k_cache[0].shape[1] or b0 + B > self.k_cache[0].shape[0]:
-            raise ValueError(f"KV cache holds {self.k_cache[0].shape[1]} positions x {self.k_cache[0].shape[0]} sequences; "
+        if S > self.max_seq or b0 + B > self.max_batch:
+            raise ValueError(f"KV cache holds {self.max_seq} positions x {self.max_batch} sequences; "
                              f"asked for positions up to {S - 1} of sequences {b0}..{b0 + B - 1}")
         M = B * T
         x = self.embed[tokens].to(self.act_dtype).reshape(M, c.hidden).contiguous()
         h = torch.empty_like(x)
         pos = torch.arange(self.pos, S, device=x.device)
         nq, nkv = c.n_heads * c.head_dim, c.n_kv_heads * c.head_dim
-        rep = c.n_heads // c.n_kv_heads
+        rows = self._new_rows(B, T, b0)
         delta = None
         for l in range(c.layers):
             self._add_norm(x, delta, self.norms[f"l{l}.norm1"], h)
@@ -464,17 +515,8 @@ class MoEDecoder(QuantDecoder):
             k = qkv[:, nq:nq + nkv].reshape(B, T, c.n_kv_heads, c.head_dim)
             v = qkv[:, nq + nkv:].reshape(B, T, c.n_kv_heads, c.head_dim)
             q, k = _rope(q, pos, c.rope_base), _rope(k, pos, c.rope_base)
-            self.k_cache[l][b0:b0 + B, self.pos:S] = k
-            self.v_cache[l][b0:b0 + B, self.pos:S] = v
-            kk, vv = self.k_cache[l][b0:b0 + B, :S], self.v_cache[l][b0:b0 + B, :S]
-            if rep > 1:
-                kk, vv = kk.repeat_interleave(rep, dim=2), vv.repeat_interleave(rep, dim=2)
-            if self.pos == 0 and T > 1:
-                o = F.scaled_dot_product_attention(q.transpose(1, 2), kk.transpose(1, 2), vv.transpose(1, 2), is_causal=True)
-            else:
-                mask = (torch.arange(S, device=x.device)[None, :] <= pos[:, None])
-                o = F.scaled_dot_product_attention(q.transpose(1, 2), kk.transpose(1, 2), vv.transpose(1, 2), attn_mask=mask)
-            o = o.transpose(1, 2).reshape(M, nq)
+            o = self._cached_attention(l, q, k, v, rows, b0)
+            o = o.reshape(M, nq)
             delta = self.lin[f"l{l}.o"](o.contiguous())
             self._add_norm(x, delta, self.norms[f"l{l}.norm2"], h)
             delta = self.ffn[l](h)                                                        # fp32 [M, hidden]
@@ -511,11 +553,12 @@ class MoEDecoder(QuantDecoder):
         from .ops import _dt_of_torch, _stream_ptr
         c, lib, st = self.cfg, _lib.lib(), _stream_ptr()
         B = tokens.shape[0]
-        dt = _dt_of_torch(self.k_cache[0])
         dev = tokens.device
         x = self.embed[tokens].to(self.act_dtype).contiguous()
+        dt = _dt_of_torch(x)
         h = torch.empty_like(x)
-        S = self.k_cache[0].shape[1]
+        S = self.max_seq
+        at = None if self.kv is None else self.kv.extend(batch=B)
         att = torch.empty((B, c.n_heads, c.head_dim), dtype=self.act_dtype, device=dev)
 
         def add_norm(delta, gamma):
@@ -525,9 +568,13 @@ class MoEDecoder(QuantDecoder):
         for l in range(c.layers):
             add_norm(delta, self.norms[f"l{l}.norm1"])
             qkv = self.lin[f"l{l}.qkv"](h)
-            _lib.check(lib.bq_decode_attention_rope(qkv.data_ptr(), self.k_cache[l].data_ptr(), self.v_cache[l].data_ptr(),
-                                                    pos_t.data_ptr(), att.data_ptr(), B, c.n_heads, c.n_kv_heads,
-                                                    c.head_dim, S, c.rope_base, dt, st))
+            if self.kv is not None:
+                q = self.kv.rope_append(l, qkv, c.n_heads, c.rope_base, None, at, dtype=self.act_dtype)
+                self.kv.attention(l, q, None, at, out=att)
+            else:
+                _lib.check(lib.bq_decode_attention_rope(qkv.data_ptr(), self.k_cache[l].data_ptr(), self.v_cache[l].data_ptr(),
+                                                        pos_t.data_ptr(), att.data_ptr(), B, c.n_heads, c.n_kv_heads,
+                                                        c.head_dim, S, c.rope_base, dt, st))
             delta = self.lin[f"l{l}.o"](att.reshape(B, -1))
             add_norm(delta, self.norms[f"l{l}.norm2"])
             delta = self.ffn[l](h)

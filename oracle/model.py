@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import numpy as np
 
-from . import spec
+from . import kv4, spec
 
 
 def rmsnorm(x, w, eps=1e-6):
@@ -30,8 +30,9 @@ def rope(x, pos, base=10000.0):
 
 
 class OracleDecoder:
-    def __init__(self, cfg: dict, weights: dict):
-        self.c, self.w = cfg, weights
+    def __init__(self, cfg: dict, weights: dict, kv_bits: int = 0):
+        """kv_bits 4: the cache keeps what the 4-bit pages hold; a prompt attends to its own exact keys and values."""
+        self.c, self.w, self.kv_bits = cfg, weights, kv_bits
         self.kc = [np.zeros((0, cfg["n_kv_heads"], cfg["head_dim"]), np.float32) for _ in range(cfg["layers"])]
         self.vc = [np.zeros((0, cfg["n_kv_heads"], cfg["head_dim"]), np.float32) for _ in range(cfg["layers"])]
         self.pos = 0
@@ -51,12 +52,16 @@ class OracleDecoder:
             q = rope(self._lin(f"l{l}.q", h).reshape(T, H, D), pos)
             k = rope(self._lin(f"l{l}.k", h).reshape(T, KV, D), pos)
             v = self._lin(f"l{l}.v", h).reshape(T, KV, D)
+            exact = (k, v)
+            if self.kv_bits == 4:
+                k, v = kv4.held(k).astype(np.float32), kv4.held(v).astype(np.float32)
             self.kc[l] = np.concatenate([self.kc[l], k], 0)
             self.vc[l] = np.concatenate([self.vc[l], v], 0)
             S = self.kc[l].shape[0]
             rep = H // KV
-            kk = np.repeat(self.kc[l], rep, axis=1)          # [S, H, D]
-            vv = np.repeat(self.vc[l], rep, axis=1)
+            k_seen, v_seen = exact if self.pos == 0 and T > 1 else (self.kc[l], self.vc[l])
+            kk = np.repeat(k_seen, rep, axis=1)              # [S, H, D]
+            vv = np.repeat(v_seen, rep, axis=1)
             att = np.einsum("thd,shd->hts", q, kk) / np.sqrt(np.float32(D))
             mask = np.arange(S)[None, :] > pos[:, None]
             att = np.where(mask[None], -np.inf, att)
