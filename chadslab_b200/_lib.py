@@ -105,7 +105,7 @@ PROTOTYPES = {
     "bq_kv4_append": (_i32, [_pool, _i32, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp]),
     "bq_kv4_rope_append": (_i32, [_pool, _i32, _vp, _vp, _i32, C.c_float, _i32, _vp, _vp, _vp, _i64, _i64, _vp]),
     "bq_kv4_gather": (_i32, [_pool, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _vp]),
-    "bq_kv4_attention_work_bytes": (_i64, [_pool, _i32, _i32]),
+    "bq_kv4_attention_work_bytes": (_i64, [_pool, _i32, _i32, _i64, _i64]),
     "bq_kv4_attention": (_i32, [_pool, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
     "bq_qlinear_push": (_i32, [_h, _vp, _i32, _i64, _h, _vp]),
     "bq_allreduce": (_i32, [_h, _vp, _vp, _i64, _vp]),

@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_obj")
 LIB = os.path.join(HERE, "libb200q.so")
 SOURCES = ["api.cu", "simt.cu", "gemv_mma.cu", "gemv_push.cu", "gemv_gated.cu", "gemv_batch.cu", "moe.cu", "tc.cu", "glue.cu", "attn_mma.cu", "comm.cu", "ep.cu", "quant.cu", "kv4_pages.cu",
-           "kv4_rows.cu", "kv4_attn.cu", "kv4_attn_64.cu", "kv4_attn_128.cu", "kv4_attn_256.cu"]
+           "kv4_rows.cu", "kv4_attn.cu", "kv4_attn_64.cu", "kv4_attn_128.cu", "kv4_attn_256.cu", "kv4_chunk.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

@@ -25,18 +25,25 @@ template <typename T> static int ka_run(const KaArgs& a, int64_t cols, cudaStrea
   }
 }
 
+// columns of an average sequence and KV head: any variant is right for any number, this decides which is fast
+static int64_t ka_columns(int64_t B, int64_t n_rows, int rep, int dtype) { return (n_rows + B - 1) / B * rep * (dtype == BQ_DT_F32 ? 2 : 1); }
+
 }  // namespace bq
 
 using namespace bq;
 
 extern "C" {
 
-int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype) {
-  if (!p || p->head_dim <= 0 || Hq <= 0) return 0;
-  const int64_t width = KA_MAX_WIDTH / (dtype == BQ_DT_F32 ? 2 : 1);
-  int64_t runs = (int64_t)sm_count() * KA_MAX_TEAMS;
-  if (runs > KA_MAX_RUNS) runs = KA_MAX_RUNS;
-  return KA_MAX_RUNS * 8 * (int64_t)sizeof(int) + runs * 2 * width * (p->head_dim + 4) * (int64_t)sizeof(float);
+int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype, int64_t B, int64_t n_rows) {
+  if (!p || p->head_dim <= 0 || p->kv_heads <= 0 || Hq <= 0 || B <= 0 || n_rows < 0) return 0;
+  int64_t part = kv4_chunk_part_bytes(p->head_dim);
+  if (!kv4_chunk_supported(p->head_dim, dtype, ka_columns(B, n_rows, Hq / p->kv_heads, dtype))) {
+    const int64_t width = KA_MAX_WIDTH / (dtype == BQ_DT_F32 ? 2 : 1);
+    int64_t runs = (int64_t)sm_count() * KA_MAX_TEAMS;
+    if (runs > KA_MAX_RUNS) runs = KA_MAX_RUNS;
+    part = runs * 2 * width * (p->head_dim + 4) * (int64_t)sizeof(float);
+  }
+  return KA_MAX_RUNS * 8 * (int64_t)sizeof(int) + part;
 }
 
 int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq, void* out, int Hq, int dtype, const int32_t* slots,
@@ -62,8 +69,8 @@ int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq
   a.ldq = ldq; a.n_rows = n_rows;
   a.slots = slots; a.pos = pos; a.starts = starts; a.status = status_word();
   a.B = (int)B; a.Hq = Hq; a.rep = rep;
-  // columns of an average sequence: any variant is right for any number, this one decides what is fast
-  const int64_t cols = (n_rows + B - 1) / B * rep * (dtype == BQ_DT_F32 ? 2 : 1);
+  const int64_t cols = ka_columns(B, n_rows, rep, dtype);
+  if (kv4_chunk_supported(p->head_dim, dtype, cols)) return kv4_chunk(a, (cudaStream_t)stream);
   return dtype == BQ_DT_F32 ? ka_run<float>(a, cols, (cudaStream_t)stream) : ka_run<__nv_bfloat16>(a, cols, (cudaStream_t)stream);
 }
 

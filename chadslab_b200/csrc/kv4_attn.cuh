@@ -866,7 +866,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
 }
 
 // Segments that were cut, merged in run order.  grid: (runs, (row, head) pairs of a tile); a run that begins a segment and
-// does not finish it has left its place in `cut`, the others have nothing to do.
+// does not finish it has left its place in `cut`, the others have nothing to do.  A CTA takes every gridDim.y-th pair.
 constexpr int KA_MERGE_THREADS = 256, KA_MAX_RUNS = 1024;
 template <typename T>
 __global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(const __grid_constant__ KaArgs a) {
@@ -874,62 +874,66 @@ __global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(c
   __shared__ float4 s_o[KA_MERGE_THREADS];
   pdl_launch_dependents();
   pdl_wait();
-  const int run = blockIdx.x, hc = blockIdx.y, HC = (1 << a.width_log2) / a.sl, D = a.v.D, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int run = blockIdx.x, HC = (1 << a.width_log2) / a.sl, D = a.v.D, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int* cut = a.cut + (int64_t)run * 8;
   const int last = cut[0];
   if (last < 0) return;
-  const int row0 = cut[1], n = cut[2], h = cut[3], rh = cut[4] * HC + hc;
-  if (rh >= n * a.rep) return;
+  const int row0 = cut[1], n = cut[2], h = cut[3];
   const int64_t slot = (int64_t)HC * (D + 4);
   const int pieces = last - run + 1;
   // piece 0 is this run's second state, piece j > 0 the first state of run run + j
   const float* p0 = a.part + ((int64_t)run * 2 + 1) * slot;
   const float* p1 = a.part + (int64_t)run * 2 * slot;
-  float r = -INFINITY;
-  for (int j = threadIdx.x; j < pieces; j += KA_MERGE_THREADS) r = fmaxf(r, (j ? p1 + 2 * j * slot : p0)[HC * D + 2 * hc]);
+  for (int hc = blockIdx.y; hc < HC; hc += gridDim.y) {
+    const int rh = cut[4] * HC + hc;
+    if (rh >= n * a.rep) break;
+    if (hc != (int)blockIdx.y) __syncthreads();                 // the buffers are free again
+    float r = -INFINITY;
+    for (int j = threadIdx.x; j < pieces; j += KA_MERGE_THREADS) r = fmaxf(r, (j ? p1 + 2 * j * slot : p0)[HC * D + 2 * hc]);
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, off));
-  if (lane == 0) s_red[warp][0] = r;
-  __syncthreads();
+    for (int off = 16; off > 0; off >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, off));
+    if (lane == 0) s_red[warp][0] = r;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < KA_MERGE_THREADS / 32; ++w) r = fmaxf(r, s_red[w][0]);
-  float z = 0.0f;
-  for (int j = threadIdx.x; j < pieces; j += KA_MERGE_THREADS) {
-    const float* st = (j ? p1 + 2 * j * slot : p0) + HC * D + 2 * hc;
-    const float f = ka_exp2(st[0] - r);
-    s_f[j] = f;
-    z += st[1] * f;
-  }
+    for (int w = 0; w < KA_MERGE_THREADS / 32; ++w) r = fmaxf(r, s_red[w][0]);
+    float z = 0.0f;
+    for (int j = threadIdx.x; j < pieces; j += KA_MERGE_THREADS) {
+      const float* st = (j ? p1 + 2 * j * slot : p0) + HC * D + 2 * hc;
+      const float f = ka_exp2(st[0] - r);
+      s_f[j] = f;
+      z += st[1] * f;
+    }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
-  if (lane == 0) s_red[warp][1] = z;
-  __syncthreads();
-  z = 0.0f;
+    for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
+    if (lane == 0) s_red[warp][1] = z;
+    __syncthreads();
+    z = 0.0f;
 #pragma unroll
-  for (int w = 0; w < KA_MERGE_THREADS / 32; ++w) z += s_red[w][1];
-  // a thread sums four dimensions over every slices-th piece
-  const int quads = D / 4, slices = KA_MERGE_THREADS / quads, q = threadIdx.x % quads, sl = threadIdx.x / quads;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (sl < slices) {
+    for (int w = 0; w < KA_MERGE_THREADS / 32; ++w) z += s_red[w][1];
+    // a thread sums four dimensions over every slices-th piece
+    const int quads = D / 4, slices = KA_MERGE_THREADS / quads, q = threadIdx.x % quads, sl = threadIdx.x / quads;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (sl < slices) {
 #pragma unroll 4
-    for (int j = sl; j < pieces; j += slices) {
-      const float4 v = *reinterpret_cast<const float4*>((j ? p1 + 2 * j * slot : p0) + hc * D + q * 4);
-      const float f = s_f[j];
-      o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+      for (int j = sl; j < pieces; j += slices) {
+        const float4 v = *reinterpret_cast<const float4*>((j ? p1 + 2 * j * slot : p0) + hc * D + q * 4);
+        const float f = s_f[j];
+        o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+      }
     }
-  }
-  s_o[threadIdx.x] = o;
-  __syncthreads();
-  if (sl == 0) {
-    const int used = slices < pieces ? slices : pieces;
-    for (int k = 1; k < used; ++k) {
-      const float4 v = s_o[k * quads + q];
-      o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-    }
-    T* out = static_cast<T*>(a.out) + ((int64_t)(row0 + rh / a.rep) * a.Hq + h * a.rep + rh % a.rep) * D + q * 4;
-    const float inv[4] = {o.x / z, o.y / z, o.z / z, o.w / z};
+    s_o[threadIdx.x] = o;
+    __syncthreads();
+    if (sl == 0) {
+      const int used = slices < pieces ? slices : pieces;
+      for (int k = 1; k < used; ++k) {
+        const float4 v = s_o[k * quads + q];
+        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+      }
+      T* out = static_cast<T*>(a.out) + ((int64_t)(row0 + rh / a.rep) * a.Hq + h * a.rep + rh % a.rep) * D + q * 4;
+      const float inv[4] = {o.x / z, o.y / z, o.z / z, o.w / z};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = from_float<T>(inv[j]);
+      for (int j = 0; j < 4; ++j) out[j] = from_float<T>(inv[j]);
+    }
   }
 }
 
@@ -961,6 +965,12 @@ int ka_launch(KaArgs a, cudaStream_t s) {
   BQ_CUDA(cudaGetLastError());
   return BQ_OK;
 }
+
+// kv4_chunk.cu: many rows per sequence.  From KK_MIN_COLS (row, head) pairs per sequence and KV head on it is faster
+constexpr int KK_MIN_COLS = 48;
+bool kv4_chunk_supported(int D, int dtype, int64_t cols);
+int64_t kv4_chunk_part_bytes(int D);
+int kv4_chunk(const KaArgs& a, cudaStream_t s);
 
 // one per head_dim (kv4_attn_*.cu): picks the variant for `cols` columns per sequence
 template <typename T, int NG> int ka_pick(const KaArgs& a, int64_t cols, cudaStream_t s);

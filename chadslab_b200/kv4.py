@@ -81,7 +81,7 @@ class PagedKV4:
         self._work = torch.empty(int(lib.bq_kv4_work_bytes(self._p)) // 4, dtype=torch.int32, device=device)
         p = self._pool
         p.pages, p.tables, p.lens, p.refs, p.work = (t.data_ptr() for t in (pages, tables, lens, refs, self._work))
-        self._attn_bytes = {}
+        self._attn_ints = {}                 # scratch of an attention call by (heads, dtype, sequences, rows)
 
     # ---- arguments --------------------------------------------------------------------------------------------------
     def _ints(self, t, what: str):
@@ -226,9 +226,10 @@ class PagedKV4:
         elif out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() or out.shape != q.shape:
             raise ValueError("out must be a contiguous tensor like q")
         dt = _DT[q.dtype]
-        need = self._attn_bytes.get((heads, dt))
+        sizes = (heads, dt, B, q.shape[0])
+        need = self._attn_ints.get(sizes)
         if need is None:
-            need = self._attn_bytes[(heads, dt)] = int(self._lib.bq_kv4_attention_work_bytes(self._p, heads, dt)) // 4
+            need = self._attn_ints[sizes] = int(self._lib.bq_kv4_attention_work_bytes(self._p, *sizes)) // 4
         work = self.refs.new_empty(need)                       # of this call alone: calls may overlap
         _lib.check(self._lib.bq_kv4_attention(self._p, int(layer), q.data_ptr(), ldq, out.data_ptr(), heads, dt, at_slots, at_pos, at_starts, B,
                                               q.shape[0], work.data_ptr(), self._stream()))

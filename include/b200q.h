@@ -392,9 +392,9 @@ int bq_kv4_gather(const bq_kv4_pool* p, int layer, void* k, void* v, int dtype, 
 /* out[n_rows, Hq, head_dim] = softmax(q . K^T / sqrt(head_dim)) . V over positions 0 .. own position of every row
  * (causal), grouped-query heads.  Rows of q are ldq elements apart (even; q and out
  * aligned to two elements).  Rows of a sequence with pos < 0 are set to zero.
- * work: bq_kv4_attention_work_bytes() of device scratch, 16-byte aligned, contents do not matter; calls that may
- * overlap on the device need scratch of their own.                                                                       */
-int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype);
+ * work: bq_kv4_attention_work_bytes() of device scratch for a call of these sizes, 16-byte aligned, contents do not
+ * matter; calls that may overlap on the device need scratch of their own.                                                */
+int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype, int64_t B, int64_t n_rows);
 int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq, void* out, int Hq, int dtype,
                      const int32_t* slots, const int32_t* pos, const int32_t* starts, int64_t B, int64_t n_rows, void* work,
                      void* stream);
