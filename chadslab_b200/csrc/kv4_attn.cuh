@@ -866,8 +866,9 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
 }
 
 // Segments that were cut, merged in run order.  grid: (runs, (row, head) pairs of a tile); a run that begins a segment and
-// does not finish it has left its place in `cut`, the others have nothing to do.  A CTA takes every gridDim.y-th pair.
-constexpr int KA_MERGE_THREADS = 256, KA_MAX_RUNS = 1024;
+// does not finish it has left its place in `cut`, the others have nothing to do.  Few pieces: a warp per pair; many: a CTA per
+// pair, whose threads share the pieces (two contexts of 131072 positions have 73; one warp would read them one by one).
+constexpr int KA_MERGE_THREADS = 256, KA_MAX_RUNS = 1024, KA_FEW = 4;
 template <typename T>
 __global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(const __grid_constant__ KaArgs a) {
   __shared__ float s_f[KA_MAX_RUNS], s_red[KA_MERGE_THREADS / 32][2];
@@ -884,6 +885,41 @@ __global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(c
   // piece 0 is this run's second state, piece j > 0 the first state of run run + j
   const float* p0 = a.part + ((int64_t)run * 2 + 1) * slot;
   const float* p1 = a.part + (int64_t)run * 2 * slot;
+  if (pieces <= KA_FEW) {
+    for (int hc = blockIdx.y * (KA_MERGE_THREADS / 32) + warp; hc < HC; hc += gridDim.y * (KA_MERGE_THREADS / 32)) {
+      const int rh = cut[4] * HC + hc;
+      if (rh >= n * a.rep) break;
+      // lane j looks after piece j
+      const float* st = (lane ? p1 + 2 * lane * slot : p0) + HC * D + 2 * hc;
+      float r = lane < pieces ? st[0] : -INFINITY, z = lane < pieces ? st[1] : 0.0f;
+      float top = r;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      const float f = lane < pieces ? ka_exp2(r - top) : 0.0f;
+      z *= f;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
+      const float inv = 1.0f / z;
+      const int i = rh / a.rep;
+      T* out = static_cast<T*>(a.out) + ((int64_t)(row0 + i) * a.Hq + h * a.rep + rh - i * a.rep) * D;
+      for (int d0 = 0; d0 < D; d0 += 128) {
+        const int d = d0 + lane * 4;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int j = 0; j < pieces; ++j) {
+          const float w = __shfl_sync(0xffffffffu, f, j);
+          if (d >= D) continue;
+          const float4 v = *reinterpret_cast<const float4*>((j ? p1 + 2 * j * slot : p0) + hc * D + d);
+          o.x += v.x * w; o.y += v.y * w; o.z += v.z * w; o.w += v.w * w;
+        }
+        if (d < D) {
+          ka_store2(out + d, o.x * inv, o.y * inv);
+          ka_store2(out + d + 2, o.z * inv, o.w * inv);
+        }
+      }
+    }
+    return;
+  }
   for (int hc = blockIdx.y; hc < HC; hc += gridDim.y) {
     const int rh = cut[4] * HC + hc;
     if (rh >= n * a.rep) break;

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
       for (int n = 0; n < 2 * KK_BLOCKS; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
-#pragma unroll 1
+#pragma unroll 2
       for (int G = 0; G < NG; ++G) {
         float c[2 * KK_BLOCKS][4];
 #pragma unroll
