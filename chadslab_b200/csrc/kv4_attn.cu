@@ -37,7 +37,7 @@ extern "C" {
 int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype, int64_t B, int64_t n_rows) {
   if (!p || p->head_dim <= 0 || p->kv_heads <= 0 || Hq <= 0 || B <= 0 || n_rows < 0) return 0;
   int64_t part = kv4_chunk_part_bytes(p->head_dim);
-  if (!kv4_chunk_supported(p->head_dim, dtype, ka_columns(B, n_rows, Hq / p->kv_heads, dtype))) {
+  if (!kv4_chunk_supported(p->head_dim, dtype, B, p->kv_heads, ka_columns(B, n_rows, Hq / p->kv_heads, dtype))) {
     const int64_t width = KA_MAX_WIDTH / (dtype == BQ_DT_F32 ? 2 : 1);
     int64_t runs = (int64_t)sm_count() * KA_MAX_TEAMS;
     if (runs > KA_MAX_RUNS) runs = KA_MAX_RUNS;
@@ -70,7 +70,7 @@ int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq
   a.slots = slots; a.pos = pos; a.starts = starts; a.status = status_word();
   a.B = (int)B; a.Hq = Hq; a.rep = rep;
   const int64_t cols = ka_columns(B, n_rows, rep, dtype);
-  if (kv4_chunk_supported(p->head_dim, dtype, cols)) return kv4_chunk(a, (cudaStream_t)stream);
+  if (kv4_chunk_supported(p->head_dim, dtype, B, p->kv_heads, cols)) return kv4_chunk(a, (cudaStream_t)stream);
   return dtype == BQ_DT_F32 ? ka_run<float>(a, cols, (cudaStream_t)stream) : ka_run<__nv_bfloat16>(a, cols, (cudaStream_t)stream);
 }
 

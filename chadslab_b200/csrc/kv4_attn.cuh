@@ -1002,9 +1002,8 @@ int ka_launch(KaArgs a, cudaStream_t s) {
   return BQ_OK;
 }
 
-// kv4_chunk.cu: many rows per sequence.  From KK_MIN_COLS (row, head) pairs per sequence and KV head on it is faster
-constexpr int KK_MIN_COLS = 48;
-bool kv4_chunk_supported(int D, int dtype, int64_t cols);
+// kv4_chunk.cu: many rows per sequence; cols = (row, head) pairs of an average sequence and KV head
+bool kv4_chunk_supported(int D, int dtype, int64_t B, int Hkv, int64_t cols);
 int64_t kv4_chunk_part_bytes(int D);
 int kv4_chunk(const KaArgs& a, cudaStream_t s);
 

@@ -378,8 +378,14 @@ static int chunk_launch(KaArgs a, cudaStream_t s) {
   return BQ_OK;
 }
 
-// Head dimensions of whole, even fragments; `cols` = (row, head) pairs of an average sequence and KV head.
-bool kv4_chunk_supported(int D, int dtype, int64_t cols) { return dtype == BQ_DT_BF16 && (D == 64 || D == 128 || D == 256) && cols >= KK_MIN_COLS; }
+// Which calls come here: head dimensions of whole, even fragments, at least 96 (row, head) pairs per sequence and KV head, and
+// 48 segments of 128 of them or more, so that few are cut (a cut leaves 128 pairs' states to be merged).  Both kernels, us, at
+// 8 sequences x 2048 positions, 16 heads of 256 (decode kernel / this one): 64 pairs 143 / 171, 96: 204 / 177, 256: 488 / 330;
+// 32 / 4 heads of 128 (32 segments up to 128 pairs, 64 at 256): 96: 44 / 48, 128: 53 / 54, 256: 80 / 58; 8 heads on one KV
+// head of 256, 256 pairs (16 segments): 51 / 67.
+bool kv4_chunk_supported(int D, int dtype, int64_t B, int Hkv, int64_t cols) {
+  return dtype == BQ_DT_BF16 && (D == 64 || D == 128 || D == 256) && cols >= 96 && B * Hkv * ((cols + KK_ROWS - 1) / KK_ROWS) >= 48;
+}
 int64_t kv4_chunk_part_bytes(int D) { return (int64_t)sm_count() * 2 * KK_ROWS * (D + 4) * (int64_t)sizeof(float); }
 int kv4_chunk(const KaArgs& a, cudaStream_t s) {
   return a.v.D == 64 ? chunk_launch<2>(a, s) : a.v.D == 128 ? chunk_launch<4>(a, s) : chunk_launch<8>(a, s);

@@ -305,13 +305,21 @@ def test_chunk_attention(cuda_lib, D, Hkv, rep, page, dtype):
     check(kv, 0, data, lens, new, Hkv * rep, dtype, rng, strided=True)
 
 
-@pytest.mark.parametrize("D,Hkv,rep,page", [(64, 2, 3, 16), (64, 1, 1, 32), (128, 2, 4, 64), (128, 1, 16, 16), (256, 1, 8, 64), (256, 2, 1, 16)])
+def many_rows(kv, heads, B, n_rows):
+    """Whether a call of these sizes takes the kernel that works on 128 (row, head) pairs at a time (its scratch tells)."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    need = kv._lib.bq_kv4_attention_work_bytes(kv._p, heads, 1, B, n_rows)
+    return need == 1024 * 32 + sms * 2 * 128 * (kv.head_dim + 4) * 4
+
+
+@pytest.mark.parametrize("D,Hkv,rep,page", [(64, 8, 3, 16), (64, 8, 2, 32), (128, 4, 4, 64), (128, 1, 16, 16), (256, 2, 8, 64), (256, 8, 2, 16)])
 def test_many_rows_attention(cuda_lib, D, Hkv, rep, page):
     """Chunks long enough for the kernel that works on 128 (row, head) pairs at a time: odd lengths, whole prompts, sequences
     without rows, several tiles of pairs and of positions, cut segments."""
     rng = np.random.default_rng(D + rep)
     lens, new = [333, 70, 260, 5, 64, 129], [140, 70, 1, 0, 64, 128]
     kv = make(2, Hkv, D, n_pages=80, max_pages=24, page=page)
+    assert many_rows(kv, Hkv * rep, len(lens), sum(new)) and not many_rows(kv, Hkv * rep, 6, 6)
     shuffle(kv, rng)
     data = fill(kv, 1, lens, rng, "bf16", 20.0 if D == 64 else 1.0)
     check(kv, 1, data, lens, new, Hkv * rep, "bf16", rng, strided=True)
@@ -323,14 +331,15 @@ def test_many_rows_ranges_and_bytes_behind(cuda_lib, vscale):
     lens, new, got = [100, 83], [90, 83], []
     for fill_with in (0, 0x7C00, 0x7E00, 0x7BFF, -1):
         rng = np.random.default_rng(8)
-        kv = make(1, 1, 128, page=32)
+        kv = make(1, 24, 128, page=32)
+        assert many_rows(kv, 48, 2, sum(new))
         kv.pages.view(torch.int16).fill_(fill_with)
         data = fill(kv, 0, lens, rng, "bf16", vscale)
-        q = rows(rng, sum(new), 2, 128, "bf16", 6.0)
+        q = rows(rng, sum(new), 48, 128, "bf16", 6.0)
         pos = ints([n - m for n, m in zip(lens, new)])
         got.append(kv.attention(0, q, None, pos, starts_of(new)))
         assert torch.equal(got[-1], got[0])
-    check(kv, 0, data, lens, new, 2, "bf16", np.random.default_rng(3))
+    check(kv, 0, data, lens, new, 48, "bf16", np.random.default_rng(3))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
