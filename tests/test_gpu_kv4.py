@@ -475,3 +475,56 @@ def test_serving_run_in_a_graph(cuda_lib):
     q1 = q[1, [0, 2]].contiguous()
     a, b = (p.attention(1, q1, [0, 2], [38, 38]) for p in (kv, small))
     assert torch.equal(a, b)
+
+
+def test_many_sequences(cuda_lib):
+    """Batches of several hundred sequences (the searches over sequences take more than one pass), some without rows, some
+    refused."""
+    rng = np.random.default_rng(17)
+    B, Hkv, rep, D = 700, 1, 2, 64
+    lens = [int(x) for x in rng.choice([0, 1, 2, 15, 16, 17, 40], B)]
+    kv = make(1, Hkv, D, n_pages=1800, max_seqs=1000, max_pages=4, page=16)
+    shuffle(kv, rng)
+    slots = rng.permutation(1000)[:B]
+    starts = starts_of(lens)
+    k, v = rows(rng, sum(lens), Hkv, D, "bf16"), rows(rng, sum(lens), Hkv, D, "bf16")
+    pos = kv.extend(ints(slots), starts)
+    assert (pos == 0).all()
+    kv.append(0, k, v, ints(slots), pos, starts)
+    gk, gv = kv.gather(0, ints(slots), pos, starts, rows=sum(lens))
+    K, V = okv.held(num(k)), okv.held(num(v))
+    assert np.array_equal(num(gk), K.astype(np.float32)) and np.array_equal(num(gv), V.astype(np.float32))
+    q = rows(rng, sum(lens), Hkv * rep, D, "bf16")
+    refused = rng.random(B) < 0.1
+    some = torch.where(torch.from_numpy(refused).cuda(), -1, pos).int()
+    out = num(kv.attention(0, q, ints(slots), some, starts))
+    at = np.concatenate([[0], np.cumsum(lens)])
+    for b in range(B):
+        one = slice(at[b], at[b + 1])
+        if refused[b]:
+            assert (out[one] == 0).all()
+        elif lens[b]:
+            o, mag, size = okv.attention(num(q)[one], K[one], V[one], 0)
+            assert (np.abs(out[one] - o) <= bound(o, mag, size, V[one], "bf16")).all(), b
+    assert status() == 0
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_pool_past_32_bits(cuda_lib, many):
+    """Pages, layers and tables whose byte offsets pass 2^32, and rows of q and out that do not start at the tensor's start."""
+    rng = np.random.default_rng(4)
+    L, Hkv, rep, D, page = 40, 8, 2, 128, 64
+    from chadslab_b200 import PagedKV4
+    kv = PagedKV4(L, Hkv, D, n_pages=2300, max_seqs=8, max_pages=8, page=page)
+    assert kv.pages.numel() > 2 ** 32 + 2 ** 31
+    kv.refs[:2270] = 1                                # all that is given out lies behind 2^32 bytes
+    lens = [200, 1, 130, 64, 77, 300]
+    data = fill(kv, L - 1, lens, rng)
+    assert int(kv.tables[kv.tables >= 0].min()) >= 2270
+    new = [130, 1, 130, 64, 60, 100] if many else [1] * 6
+    assert many_rows(kv, Hkv * rep, 6, sum(new)) == many
+    check(kv, L - 1, data, lens, new, Hkv * rep, "bf16", rng, strided=True)
+    kv.fork([0, 5], [6, 7])
+    assert kv.extend([6, 7]).tolist() == [200, 300]      # copies of whole pages, all layers
+    a, b = (kv.gather(L - 1, [s], [0], [0, 200], rows=200)[0] for s in (0, 6))
+    assert torch.equal(a, b) and status() == 0
