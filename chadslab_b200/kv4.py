@@ -222,7 +222,7 @@ class PagedKV4:
         heads = q.shape[1]
         q, ldq = self._rows(q, heads, "q")
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() or out.shape != q.shape:
             raise ValueError("out must be a contiguous tensor like q")
         dt = _DT[q.dtype]
