@@ -45,6 +45,13 @@ int kv4_check(const bq_kv4_pool* p, const char* what);                     // kv
 int kv4_view(const bq_kv4_pool* p, int layer, const char* what, Kv4View* out);
 
 #ifdef __CUDACC__
+// The kernels of the cache may start before the kernel that wrote their inputs has finished (pdl_wait orders them), so nothing
+// here is declared __restrict__ or read through the non-coherent path: that is for memory nobody writes while a kernel lives.
+__device__ __forceinline__ uint4 kv4_load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 // The rows of one sequence of a batch call.  n < 0: refused (bad ranges, recorded in the status word); pos < 0: skipped.
 struct Kv4Seq {
   int slot, row0, n, pos;

@@ -27,13 +27,18 @@
 // A, and R moves only when a weight would exceed 2^(A + 4) (A = 11: weights up to 2^15, 2^-24 is the smallest fp16).  A
 // drops when weight * scale overflows, i.e. for values far above one.
 //
-// Work.  The tiles (128 positions, or 64 where two steps of 32 per warp do not fit into shared memory) of all (sequence, KV head, column tile) segments form one list that is cut into equal runs,
-// one per team of four warps: ragged batches and few long sequences fill the machine alike.  The teams of an SM (two to
-// four) are one CTA: as CTAs of their own some found no contiguous registers beside the preceding kernel's and started
-// when the others were done, which doubled the kernel's time (8 of 444 late: 169 us for 100 us of work).  A warp takes 32 (16) positions of every
-// tile through its own ring of bulk copies (no barrier between warps inside a segment).  A segment that lies in one
-// run is finished there; one that is cut leaves partial states in the caller's scratch, which a second kernel merges in run
-// order.  Every result has one order of additions: repeated calls give the same bits.
+// Work.  The tiles (128 positions, or 64 where two steps of 32 per warp do not fit into shared memory) of all (sequence, KV
+// head, column tile) segments form one list that is cut into equal runs, one per team of four warps: ragged batches and few
+// long sequences fill the machine alike.  The teams of an SM (two to four) are one CTA: as CTAs of their own some found no
+// contiguous registers beside the preceding kernel's and started when the others were done, which doubled the kernel's time
+// (8 of 444 late: 169 us for 100 us of work).  A warp takes 32 (16) positions of every tile through its own ring of bulk copies
+// (no barrier between warps inside a segment).  A segment that lies in one run is finished there; one that is cut leaves
+// partial states in the caller's scratch, which a second kernel merges in run order.  Every result has one order of additions:
+// repeated calls give the same bits.
+//
+// Measured (device time of graph replays; short loops, in long ones the power cap lowers the clock): 64 x 2048 positions x 16
+// heads of 256 101 us = 5.96 TB/s, ragged batch of 96 up to 8000 positions with 32 / 4 heads of 128 65 us = 3.5 TB/s, two
+// contexts of 131072 with the same heads 45 us = 3.4 TB/s (eight columns per position block: bound by its instructions).
 #pragma once
 #include "kv4.cuh"
 
@@ -41,7 +46,6 @@ namespace bq {
 
 constexpr int KA_WARPS = 4;                           // of a team: the warps that work on one run
 constexpr int KA_THREADS = KA_WARPS * 32;
-constexpr int KA_MIN_TILES = 1;                       // a run is at least this long
 constexpr uint64_t KA_WAIT_NS = 2000000000ull;        // bound of the wait for a copy
 
 // x / d for 0 <= x < 2^31
@@ -198,7 +202,6 @@ static __device__ bool ka_locate(const KaArgs& a, int runs, int run, int team, K
   }
   *total = (int)sum;
   *per = (int)(((unsigned)sum + runs - 1) / (unsigned)runs);
-  if (*per < KA_MIN_TILES) *per = KA_MIN_TILES;
   const int64_t lo = (int64_t)run * *per;
   if (lo >= sum) return false;
   int64_t before = 0;
@@ -309,7 +312,7 @@ template <typename T, int NG, int NC> struct KaCfg {
   static constexpr int GP = 8 / NC < NG ? 8 / NC : NG; // groups side by side in a fragment
   static_assert(NG % GP == 0, "whole fragments");
   static constexpr int NF = NG / GP;
-  static constexpr int W = NC;                   // columns of a tile
+  static constexpr int W = NC;                        // columns of a tile
   static constexpr int HC = W / SL;
   static_assert(W % SL == 0, "an fp32 row takes two columns");
   static constexpr int J = NC == 1 || SL == 2 ? 1 : 2;  // different (row, head) pairs among a lane's two columns
@@ -994,7 +997,7 @@ int ka_launch(KaArgs a, cudaStream_t s) {
                       (double)((a.n_rows * a.rep * C::SL + C::W - 1) / C::W);
   int64_t grid = sm_count();
   if (grid > KA_MAX_RUNS / C::TEAMS) grid = KA_MAX_RUNS / C::TEAMS;
-  if ((double)grid * KA_MIN_TILES > most) grid = ((int64_t)most + KA_MIN_TILES - 1) / KA_MIN_TILES;
+  if ((double)grid > most) grid = (int64_t)most;
   BQ_CUDA(launch_chain(kv4_attention_kernel<T, NG, NC>, dim3((unsigned)grid), dim3(C::TEAMS * KA_THREADS), C::TEAMS * C::SMEM, s, 1, a));
   BQ_CUDA(launch_chain(kv4_attention_merge_kernel<T>, dim3((unsigned)(grid * C::TEAMS - 1), (unsigned)C::HC), dim3(KA_MERGE_THREADS), 0, s, 1, a));
   count_launch(2);

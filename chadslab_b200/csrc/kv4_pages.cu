@@ -97,8 +97,8 @@ __device__ int kp_list(const int32_t* refs, int64_t n_pages, int want, int32_t* 
 }
 
 // One CTA.  need(b) = pages that sequence b lacks for n more rows, one more if its last page is partly filled and shared.
-__global__ void __launch_bounds__(KP_THREADS) kv4_extend_kernel(KpPool p, const int32_t* __restrict__ slots, const int32_t* __restrict__ starts,
-                                                                int B, int32_t* __restrict__ pos_out, int* __restrict__ status) {
+__global__ void __launch_bounds__(KP_THREADS) kv4_extend_kernel(KpPool p, const int32_t* slots, const int32_t* starts,
+                                                                int B, int32_t* pos_out, int* status) {
   extern __shared__ int owner[];                     // first batch entry that names a slot
   __shared__ int red[32];
   __shared__ int s_copies;
@@ -201,7 +201,7 @@ constexpr int KC_THREADS = 256;
 constexpr int KC_UNROLL = 8;
 constexpr int KC_CHUNK = KC_THREADS * KC_UNROLL * 16;              // bytes of one work unit: 32 KB
 template <bool COMPACT>
-__global__ void __launch_bounds__(KC_THREADS) kv4_copy_kernel(KpPool p, const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
+__global__ void __launch_bounds__(KC_THREADS) kv4_copy_kernel(KpPool p, const uint8_t* src, uint8_t* dst,
                                                               int64_t page_bytes, KpPool q) {
   pdl_launch_dependents();
   pdl_wait();
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_copy_kernel(KpPool p, const ui
 #pragma unroll
     for (int j = 0; j < KC_UNROLL; ++j) {
       const int at = (j * KC_THREADS + (int)threadIdx.x) * 16;
-      if (at < left) v[j] = ldg_stream16(s + at);
+      if (at < left) v[j] = kv4_load16(s + at);
     }
 #pragma unroll
     for (int j = 0; j < KC_UNROLL; ++j) {
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_copy_kernel(KpPool p, const ui
   }
 }
 
-__global__ void __launch_bounds__(KP_THREADS) kv4_compact_plan_kernel(KpPool p, int64_t room, int* __restrict__ status) {
+__global__ void __launch_bounds__(KP_THREADS) kv4_compact_plan_kernel(KpPool p, int64_t room, int* status) {
   __shared__ int red[32];
   pdl_launch_dependents();
   pdl_wait();
@@ -266,8 +266,8 @@ __device__ __forceinline__ void kp_release(const KpPool& p, int32_t* row, int n,
   }
 }
 // first half: every source is read, and its pages counted once more, before any destination changes
-__global__ void __launch_bounds__(KF_THREADS) kv4_fork_read_kernel(KpPool p, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n,
-                                                                   int* __restrict__ status) {
+__global__ void __launch_bounds__(KF_THREADS) kv4_fork_read_kernel(KpPool p, const int32_t* src, const int32_t* dst, int n,
+                                                                   int* status) {
   pdl_launch_dependents();
   pdl_wait();
   const KpWork w = kp_work(p.work, p.n_pages, p.max_seqs);
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(KF_THREADS) kv4_fork_read_kernel(KpPool p, con
   }
   if (threadIdx.x == 0) keep[0] = len;
 }
-__global__ void __launch_bounds__(KF_THREADS) kv4_fork_write_kernel(KpPool p, const int32_t* __restrict__ dst, int* __restrict__ status) {
+__global__ void __launch_bounds__(KF_THREADS) kv4_fork_write_kernel(KpPool p, const int32_t* dst, int* status) {
   pdl_launch_dependents();
   pdl_wait();
   const KpWork w = kp_work(p.work, p.n_pages, p.max_seqs);
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(KF_THREADS) kv4_fork_write_kernel(KpPool p, co
   for (int j = threadIdx.x; j < np; j += KF_THREADS) row[j] = keep[1 + j];
   if (threadIdx.x == 0) p.lens[d] = len;
 }
-__global__ void __launch_bounds__(KF_THREADS) kv4_free_kernel(KpPool p, const int32_t* __restrict__ slots, int* __restrict__ status) {
+__global__ void __launch_bounds__(KF_THREADS) kv4_free_kernel(KpPool p, const int32_t* slots, int* status) {
   __shared__ int s_len;
   pdl_launch_dependents();
   pdl_wait();

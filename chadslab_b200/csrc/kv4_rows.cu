@@ -141,10 +141,10 @@ constexpr int KR_STAGE = 288 * 8;                      // of the largest head_di
 
 // grid: (items, tasks by pairs of warps); a task is (head, K or V)
 template <typename T>
-__global__ void __launch_bounds__(KR_THREADS) kv4_append_kernel(Kv4View v, const T* __restrict__ k, const T* __restrict__ val, int64_t ldk,
-                                                                int64_t ldv, const int32_t* __restrict__ slots,
-                                                                const int32_t* __restrict__ pos, const int32_t* __restrict__ starts, int B,
-                                                                int64_t n_rows, int* __restrict__ status, bool vec) {
+__global__ void __launch_bounds__(KR_THREADS) kv4_append_kernel(Kv4View v, const T* k, const T* val, int64_t ldk,
+                                                                int64_t ldv, const int32_t* slots,
+                                                                const int32_t* pos, const int32_t* starts, int B,
+                                                                int64_t n_rows, int* status, bool vec) {
   __shared__ __align__(16) uint8_t stage[KR_TASKS][KR_STAGE];
   pdl_launch_dependents();
   pdl_wait();
@@ -166,10 +166,10 @@ __global__ void __launch_bounds__(KR_THREADS) kv4_append_kernel(Kv4View v, const
 // The same behind a fused projection: qkv fp32 [n_rows][(Hq + 2 Hkv) * D].  Tasks 0 .. 2 Hkv - 1 are the heads' K and V,
 // the others one query head each (rotated into q_out).
 template <typename T>
-__global__ void __launch_bounds__(KR_THREADS) kv4_rope_append_kernel(Kv4View v, const float* __restrict__ qkv, T* __restrict__ q_out, int Hq,
-                                                                     float rope_base, const int32_t* __restrict__ slots,
-                                                                     const int32_t* __restrict__ pos, const int32_t* __restrict__ starts, int B,
-                                                                     int64_t n_rows, int* __restrict__ status) {
+__global__ void __launch_bounds__(KR_THREADS) kv4_rope_append_kernel(Kv4View v, const float* qkv, T* q_out, int Hq,
+                                                                     float rope_base, const int32_t* slots,
+                                                                     const int32_t* pos, const int32_t* starts, int B,
+                                                                     int64_t n_rows, int* status) {
   extern __shared__ float s_ang[];                     // cos [16][D / 2], sin [16][D / 2]
   __shared__ __align__(16) uint8_t stage[KR_TASKS][KR_STAGE];
   pdl_launch_dependents();
@@ -209,9 +209,9 @@ __global__ void __launch_bounds__(KR_THREADS) kv4_rope_append_kernel(Kv4View v, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(KR_THREADS) kv4_gather_kernel(Kv4View v, T* __restrict__ k, T* __restrict__ val, const int32_t* __restrict__ slots,
-                                                                const int32_t* __restrict__ pos, const int32_t* __restrict__ starts, int B,
-                                                                int64_t n_rows, int* __restrict__ status, bool vec) {
+__global__ void __launch_bounds__(KR_THREADS) kv4_gather_kernel(Kv4View v, T* k, T* val, const int32_t* slots,
+                                                                const int32_t* pos, const int32_t* starts, int B,
+                                                                int64_t n_rows, int* status, bool vec) {
   __shared__ __align__(16) uint8_t all[KR_TASKS][KR_STAGE];
   pdl_launch_dependents();
   pdl_wait();
