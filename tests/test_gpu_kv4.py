@@ -528,3 +528,56 @@ def test_pool_past_32_bits(cuda_lib, many):
     assert kv.extend([6, 7]).tolist() == [200, 300]      # copies of whole pages, all layers
     a, b = (kv.gather(L - 1, [s], [0], [0, 200], rows=200)[0] for s in (0, 6))
     assert torch.equal(a, b) and status() == 0
+
+
+def test_refusals_of_the_c_abi(cuda_lib):
+    """Bad arguments come back as codes and nothing is launched."""
+    from chadslab_b200 import _lib
+    kv = make(2, 2, 64, n_pages=8, max_seqs=4)
+    lib, p = _lib.lib(), kv._p
+    x = torch.zeros(4096, device="cuda")
+    i = ints(range(8))
+    at, ip, s = x.data_ptr(), i.data_ptr(), torch.cuda.current_stream().cuda_stream
+    n0 = lib.bq_launch_count()
+    att = lambda layer=0, q=at, ldq=256, out=at, Hq=4, dt=0, pos=ip, B=2, rows=2, work=at: lib.bq_kv4_attention(
+        p, layer, q, ldq, out, Hq, dt, None, pos, None, B, rows, work, s)
+    app = lambda layer=0, k=at, v=at, ldk=128, ldv=128, dt=0, pos=ip, B=2, rows=2: lib.bq_kv4_append(
+        p, layer, k, v, ldk, ldv, dt, None, pos, None, B, rows, s)
+    rope = lambda Hq=4, q=at, B=2, rows=2, dt=0: lib.bq_kv4_rope_append(p, 0, at, q, Hq, 1e4, dt, None, ip, None, B, rows, s)
+    bad = [att(layer=2), att(layer=-1), att(q=None), att(out=None), att(work=None), att(pos=None), att(Hq=3), att(Hq=0), att(dt=2), att(ldq=255),
+           att(ldq=254), att(B=5, rows=5), att(B=-1), att(rows=3), att(q=at + 4), att(out=at + 4), att(work=at + 8), app(layer=2), app(k=None),
+           app(v=None), app(ldk=127), app(dt=7), app(k=at + 2), app(B=5, rows=5), app(rows=1), app(pos=None), rope(Hq=3), rope(q=None), rope(dt=2),
+           rope(rows=3), lib.bq_kv4_gather(p, 0, None, at, 0, None, ip, None, 2, 2, s), lib.bq_kv4_gather(p, 0, at, at, 0, None, ip, None, 2, 1, s),
+           lib.bq_kv4_extend(p, None, None, 5, ip, s), lib.bq_kv4_extend(p, None, None, 2, None, s), lib.bq_kv4_extend(None, None, None, 1, ip, s),
+           lib.bq_kv4_fork(p, None, ip, 1, s), lib.bq_kv4_fork(p, ip, ip, 5, s), lib.bq_kv4_free(p, None, 1, s), lib.bq_kv4_free(p, ip, -1, s),
+           lib.bq_kv4_compact(p, p, s), lib.bq_kv4_compact(p, make(2, 2, 64, max_seqs=5)._p, s), lib.bq_kv4_compact(p, None, s)]
+    assert bad == [-1] * len(bad) and lib.bq_launch_count() == n0
+    for field, value in (("head_dim", 40), ("page", 48), ("n_pages", 0), ("max_seqs", 9000), ("pages", None), ("refs", at + 4)):
+        q = _lib.Kv4Pool.from_buffer_copy(kv._pool)
+        setattr(q, field, value)
+        assert lib.bq_kv4_free(C.byref(q), ip, 1, s) == -1 and lib.bq_last_error()
+    # nothing to do is not an error
+    assert att(B=0, rows=0) == 0 and app(B=0, rows=0) == 0 and lib.bq_kv4_free(p, ip, 0, s) == 0 and lib.bq_launch_count() == n0
+
+
+def test_refusals_of_the_python_surface(cuda_lib):
+    import chadslab_b200 as cb
+    kv = make(1, 2, 64)
+    k, q = torch.zeros((2, 2, 64), device="cuda"), torch.zeros((2, 4, 64), device="cuda")
+    for call, error in [(lambda: kv.append(0, k.half(), k.half(), [0, 1], [0, 0]), TypeError), (lambda: kv.append(0, k, k.bfloat16(), [0, 1], [0, 0]), ValueError),
+                        (lambda: kv.append(0, k[:, :1], k, [0, 1], [0, 0]), ValueError), (lambda: kv.append(0, k.cpu(), k, [0, 1], [0, 0]), cb.BqError),
+                        (lambda: kv.append(0, k, k, [0], [0, 0]), ValueError), (lambda: kv.append(0, k, k, [0, 1], [0, 0], [0, 1]), ValueError),
+                        (lambda: kv.append(0, k, k, torch.tensor([0, 1], device="cuda"), [0, 0]), cb.BqError),
+                        (lambda: kv.append(1, k, k, [0, 1], [0, 0]), cb.BqError), (lambda: kv.attention(0, q[:, :3], [0, 1], [0, 0]), ValueError),
+                        (lambda: kv.attention(0, q[..., :32], [0, 1], [0, 0]), ValueError), (lambda: kv.attention(0, q, [0, 1], [0, 0], out=q.bfloat16()), ValueError),
+                        (lambda: kv.attention(0, q, [0, 1, 2], [0, 0, 0]), cb.BqError), (lambda: kv.fork([0], [1, 2]), ValueError),
+                        (lambda: kv.extend([0, 1], [0, 1]), ValueError), (lambda: kv.rope_append(0, k.flatten(1), 2, 1e4, [0, 1], [0, 0]), ValueError),
+                        (lambda: kv.rope_append(0, torch.zeros((2, 512), device="cuda").bfloat16(), 4, 1e4, [0, 1], [0, 0]), cb.BqError),
+                        (lambda: kv.compact(kv), cb.BqError), (lambda: kv.gather(0, [0], [0], dtype=torch.float16), TypeError)]:
+        with pytest.raises(error):
+            call()
+    # rows that are not dense, or not aligned, are copied
+    kv.extend([0, 1], [0, 1, 2])
+    odd = torch.randn((2, 64, 2), device="cuda").transpose(1, 2)
+    kv.append(0, odd, odd, [0, 1], [0, 0])
+    assert np.array_equal(num(kv.gather(0, [0, 1], [0, 0])[0]), okv.held(num(odd)).astype(np.float32)) and status() == 0
