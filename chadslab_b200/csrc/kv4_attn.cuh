@@ -276,6 +276,11 @@ __device__ __forceinline__ void ka_mma(float* d, uint32_t a0, uint32_t a1, uint3
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void ka_mma_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {      // d = A x B
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t ka_transpose(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
         float z = sum[f];
         z += __shfl_xor_sync(0xffffffffu, z, 1);
         z += __shfl_xor_sync(0xffffffffu, z, 2);
-        z *= C::SUBNORMAL ? -8.0f / 16777216.0f : 0.0f;
+        z *= -8.0f / 16777216.0f;                              // (SUBNORMAL; else there is nothing to take off)
 #pragma unroll
         for (int j = 0; j < 2; ++j) start[f][j] = __shfl_sync(0xffffffffu, z, (2 * t + j) * 4);
       }
@@ -489,17 +494,15 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
     // ---- the positions ----------------------------------------------------------------------------------------------------
     float acc[2 * NG][4], ref[2], l[2];
     float A = 11.0f;
-    {
 #pragma unroll
-      for (int i = 0; i < 2 * NG; ++i)
+    for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // a column without a row has no weight anywhere: it must not take part in the search for a reference
-        ref[j] = vis[j] == 0x7FFFFFFF ? 3.0e38f : -3.0e38f;
-        l[j] = 0.0f;
-      }
+    for (int j = 0; j < 2; ++j) {
+      // a column without a row has no weight anywhere: it must not take part in the search for a reference
+      ref[j] = vis[j] == 0x7FFFFFFF ? 3.0e38f : -3.0e38f;
+      l[j] = 0.0f;
     }
     for (int i = 0; i < mine; ++i) {
       const uint8_t* stage = ring + take * C::STAGE;
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
 #pragma unroll
           for (int f = 0; f < NF; ++f) {
             float c[4];
-            {
+            if (C::SUBNORMAL) {
               c[0] = c[2] = start[f][0];
               c[1] = c[3] = start[f][1];
             }
@@ -539,7 +542,8 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
                 } else {
                   r0 = ka_code(w); r1 = ka_code16(w); r2 = ka_code(x); r3 = ka_code16(x);
                 }
-                ka_mma(c, r0, r2, r1, r3, bq[2 * G + h][0], bq[2 * G + h][1]);
+                if (!C::SUBNORMAL && gi == 0 && h == 0) ka_mma_new(c, r0, r2, r1, r3, bq[2 * G][0], bq[2 * G][1]);
+                else ka_mma(c, r0, r2, r1, r3, bq[2 * G + h][0], bq[2 * G + h][1]);
               }
             }
             // scales of rows g and g + 8: of the column's group, or (NC == 1) of the two columns' groups
@@ -562,39 +566,36 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
               k0.x = k0.y = __half2float(ks[g * NG + G]);
               k1.x = k1.y = __half2float(ks[(g + 8) * NG + G]);
             }
-            {
-              s[u][0] = f ? fmaf(k0.x, c[0], s[u][0]) : k0.x * c[0];
-              s[u][1] = f ? fmaf(k0.y, c[1], s[u][1]) : k0.y * c[1];
-              s[u][2] = f ? fmaf(k1.x, c[2], s[u][2]) : k1.x * c[2];
-              s[u][3] = f ? fmaf(k1.y, c[3], s[u][3]) : k1.y * c[3];
-            }
+            s[u][0] = f ? fmaf(k0.x, c[0], s[u][0]) : k0.x * c[0];
+            s[u][1] = f ? fmaf(k0.y, c[1], s[u][1]) : k0.y * c[1];
+            s[u][2] = f ? fmaf(k1.x, c[2], s[u][2]) : k1.x * c[2];
+            s[u][3] = f ? fmaf(k1.y, c[3], s[u][3]) : k1.y * c[3];
           }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          {
-            float* z = s[u];
-            if (NC == 1) {
-              z[0] += z[1];
-              z[2] += z[3];
+        for (int u = 0; u < U; ++u) {
+          float* z = s[u];
+          if (NC == 1) {
+            z[0] += z[1];
+            z[2] += z[3];
 #pragma unroll
-              for (int j = 0; j < 4; j += 2) {
-                z[j] += __shfl_xor_sync(0xffffffffu, z[j], 1);
-                z[j] += __shfl_xor_sync(0xffffffffu, z[j], 2);
-                z[j + 1] = z[j];
-              }
-            } else if (NC < 8) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if (NC == 2) z[j] += __shfl_xor_sync(0xffffffffu, z[j], 1);
-                z[j] += __shfl_xor_sync(0xffffffffu, z[j], 2);
-              }
+            for (int j = 0; j < 4; j += 2) {
+              z[j] += __shfl_xor_sync(0xffffffffu, z[j], 1);
+              z[j] += __shfl_xor_sync(0xffffffffu, z[j], 2);
+              z[j + 1] = z[j];
             }
-            if (SL == 2) {
-              z[0] = z[1] = z[0] + z[1] * KA_LO;
-              z[2] = z[3] = z[2] + z[3] * KA_LO;
+          } else if (NC < 8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (NC == 2) z[j] += __shfl_xor_sync(0xffffffffu, z[j], 1);
+              z[j] += __shfl_xor_sync(0xffffffffu, z[j], 2);
             }
           }
+          if (SL == 2) {
+            z[0] = z[1] = z[0] + z[1] * KA_LO;
+            z[2] = z[3] = z[2] + z[3] * KA_LO;
+          }
+        }
         const bool masked = p0 + U * KV4_ROWS - 1 > all_see;   // positions past the end, or past a column's own
         if (masked) {
 #pragma unroll
@@ -704,11 +705,10 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          {
-            l[0] += p[u][0] + p[u][2];
-            if (J == 2) l[1] += p[u][1] + p[u][3];
-          }
+        for (int u = 0; u < U; ++u) {
+          l[0] += p[u][0] + p[u][2];
+          if (J == 2) l[1] += p[u][1] + p[u][3];
+        }
         // values
 #pragma unroll
         for (int u = 0; u < U; ++u)
