@@ -709,19 +709,42 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
           l[0] += p[u][0] + p[u][2];
           if (J == 2) l[1] += p[u][1] + p[u][3];
         }
-        // values
-#pragma unroll
-        for (int u = 0; u < U; ++u)
+        // Values.  The matrix unit truncates its sums, which over a long context adds up to a bias of 2^-25 per step: fp32 rows
+        // add a step's sum to the accumulators themselves, rounded to nearest (4096 positions and more: 3.5e-6 -> 3e-7 off).
+        if (SL == 2) {
 #pragma unroll
           for (int G = 0; G < NG; ++G) {
-            const uint2 w2 = *reinterpret_cast<const uint2*>(blk0 + u * C::BLK + kv4_v_off(D) + G * 256 + lane * 8);
+            float sum[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t w = h ? w2.y : w2.x, x = w >> 8;
-              const uint32_t r0 = ka_code(w), r1 = ka_code16(w), r2 = ka_code(x), r3 = ka_code16(x);
-                ka_mma(acc[2 * G + h], r0, r1, r2, r3, wv[u][G / GP][0], wv[u][G / GP][1]);
+            for (int u = 0; u < U; ++u) {
+              const uint2 w2 = *reinterpret_cast<const uint2*>(blk0 + u * C::BLK + kv4_v_off(D) + G * 256 + lane * 8);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t w = h ? w2.y : w2.x, x = w >> 8;
+                const uint32_t r0 = ka_code(w), r1 = ka_code16(w), r2 = ka_code(x), r3 = ka_code16(x);
+                if (u == 0) ka_mma_new(sum[h], r0, r1, r2, r3, wv[u][G / GP][0], wv[u][G / GP][1]);
+                else ka_mma(sum[h], r0, r1, r2, r3, wv[u][G / GP][0], wv[u][G / GP][1]);
+              }
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[2 * G + h][j] += sum[h][j];
           }
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int G = 0; G < NG; ++G) {
+              const uint2 w2 = *reinterpret_cast<const uint2*>(blk0 + u * C::BLK + kv4_v_off(D) + G * 256 + lane * 8);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t w = h ? w2.y : w2.x, x = w >> 8;
+                const uint32_t r0 = ka_code(w), r1 = ka_code16(w), r2 = ka_code(x), r3 = ka_code16(x);
+                ka_mma(acc[2 * G + h], r0, r1, r2, r3, wv[u][G / GP][0], wv[u][G / GP][1]);
+              }
+            }
+        }
       }
       --flying;
       if (++take == S) { take = 0; phase ^= 1u; }

@@ -353,6 +353,26 @@ def test_long_context_attention(cuda_lib, D, Hkv, rep, dtype):
     check(kv, 0, data, lens, [1, 1, 1], Hkv * rep, dtype, rng)
 
 
+@pytest.mark.parametrize("D,Hkv,rep,lens", [(64, 4, 1, [6000] * 90), (128, 4, 4, [5000] * 70), (256, 2, 2, [4500] * 60)])
+def test_fp32_rows_keep_their_precision_over_long_runs(cuda_lib, D, Hkv, rep, lens):
+    """Many steps of one run into the same sums.  Their errors are to be those of single steps, not of their number: 2-norm of
+    the error over that of the result.  The exponent of a weight, up to 16, is rounded to 2^-21 absolute (a share of 2^-21.5 of
+    the weight, at random), weights and queries are held to 2^-22 of themselves and sums rounded to nearest: below 2^-20
+    together.  Truncated sums would be off by their number of steps, 100 and more here, times 2^-25."""
+    rng = np.random.default_rng(D)
+    kv = make(1, Hkv, D, n_pages=len(lens) * -(-lens[0] // 64), max_seqs=len(lens), max_pages=-(-lens[0] // 64), page=64)
+    starts = starts_of(lens)
+    k = torch.randn((sum(lens), Hkv, D), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    v = torch.randn((sum(lens), Hkv, D), device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    kv.append(0, k, v, None, kv.extend(None, starts), starts)
+    q = rows(rng, len(lens), Hkv * rep, D, "f32")
+    out = num(kv.attention(0, q, None, ints([n - 1 for n in lens])))
+    for b in (0, len(lens) // 2, len(lens) - 1):
+        one = slice(sum(lens[:b]), sum(lens[:b + 1]))
+        o, _, _ = okv.attention(num(q)[b:b + 1], okv.held(num(k[one])), okv.held(num(v[one])), lens[b] - 1)
+        assert np.linalg.norm(out[b] - o[0]) <= 2.0 ** -20 * np.linalg.norm(o), b
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("q_scale,vscale", [(12.0, 1.0), (1e-3, 1e-3), (3.0, 2000.0), (1e4, 1.0), (0.0, 50.0)])
 def test_attention_ranges(cuda_lib, q_scale, vscale, dtype):
