@@ -601,3 +601,48 @@ def test_refusals_of_the_python_surface(cuda_lib):
     odd = torch.randn((2, 64, 2), device="cuda").transpose(1, 2)
     kv.append(0, odd, odd, [0, 1], [0, 0])
     assert np.array_equal(num(kv.gather(0, [0, 1], [0, 0])[0]), okv.held(num(odd)).astype(np.float32)) and status() == 0
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_in_front_of_the_first_sequence(cuda_lib, many):
+    """Row ranges need not begin at row 0: what lies in front is neither read nor written, by any call."""
+    rng = np.random.default_rng(6)
+    Hkv, rep, D, front = 8, 2, 64, 21
+    lens = [70, 33, 90, 64, 1, 80] if many else [20, 3, 0, 17]
+    kv, ref = make(1, Hkv, D, n_pages=64, max_pages=8), make(1, Hkv, D, n_pages=64, max_pages=8)
+    T = front + sum(lens)
+    assert many_rows(kv, Hkv * rep, len(lens), T) == many
+    k, v, q = rows(rng, T, Hkv, D, "bf16"), rows(rng, T, Hkv, D, "bf16"), rows(rng, T, Hkv * rep, D, "bf16")
+    k[:front] = float("nan")
+    starts = starts_of(lens) + front
+    for pool, kk, vv, st in ((kv, k, v, starts), (ref, k[front:], v[front:], starts_of(lens))):
+        pool.pages.zero_()
+        pos = pool.extend(None, st, batch=len(lens))
+        assert pos.tolist() == [0] * len(lens)
+        pool.append(0, kk, vv, None, pos, st)
+    assert torch.equal(kv.pages, ref.pages)
+    out = torch.full((T, Hkv * rep, D), 9.0, dtype=torch.bfloat16, device="cuda")
+    kv.attention(0, q, None, pos, starts, out=out)
+    want = ref.attention(0, q[front:].contiguous(), None, pos, starts_of(lens))
+    # both within half a bf16 step (2^-8) of the same value but for the fp16 weights (2^-10 of values of about one)
+    assert (out[:front] == 9).all() and torch.allclose(out[front:].float(), want.float(), rtol=2 ** -6, atol=1e-3)
+    gk, gv = kv.gather(0, None, pos, starts, rows=T)
+    assert np.array_equal(num(gk)[front:], okv.held(num(k)[front:]).astype(np.float32))
+    qkv = torch.randn((T, (Hkv * rep + 2 * Hkv) * D), device="cuda")
+    q_out = torch.full((T + 2, Hkv * rep, D), 9.0, dtype=torch.bfloat16, device="cuda")[:T]
+    skip = torch.where(torch.arange(len(lens), device="cuda") == 0, -1, pos).int()        # the first sequence takes no part
+    kv.rope_append(0, qkv, Hkv * rep, 1e4, None, skip, starts, q_out=q_out)
+    first = front + lens[0]
+    assert (q_out[:first] == 9).all() and (q_out[first:] != 9).any() and status() == 0
+
+
+@pytest.mark.parametrize("page", [512, 4096])
+def test_large_pages(cuda_lib, page):
+    rng = np.random.default_rng(page)
+    lens = [5000, 511, 513, 1]
+    kv = make(1, 1, 64, n_pages=24, max_seqs=4, max_pages=-(-5120 // page) + 1, page=page)
+    shuffle(kv, rng)
+    data = fill(kv, 0, lens, rng, "bf16")
+    check(kv, 0, data, lens, [1, 3, 1, 1], 2, "bf16", rng)
+    kv.fork([0, 1], [2, 3])
+    assert kv.extend([2, 3]).tolist() == [5000, 511] and kv.lens.tolist() == [5000, 511, 5001, 512] and status() == 0
