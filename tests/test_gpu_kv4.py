@@ -646,3 +646,29 @@ def test_large_pages(cuda_lib, page):
     check(kv, 0, data, lens, [1, 3, 1, 1], 2, "bf16", rng)
     kv.fork([0, 1], [2, 3])
     assert kv.extend([2, 3]).tolist() == [5000, 511] and kv.lens.tolist() == [5000, 511, 5001, 512] and status() == 0
+
+
+def test_bookkeeping_of_thousands_of_sequences(cuda_lib):
+    """More sequences than the planning CTA has threads, more pages than it looks at in one pass."""
+    rng = np.random.default_rng(30)
+    seqs, most, page, n_pages = 3000, 4, 16, 40000
+    kv, model = make(1, 1, 32, n_pages=n_pages, max_seqs=seqs, max_pages=most, page=page), okv.Pool(n_pages, seqs, most, page)
+    taken = rng.random(n_pages) < 0.9                        # pages that belong to somebody else
+    kv.refs[torch.from_numpy(taken).cuda()] = 1
+    model.refs[taken] = 1
+    for _ in range(3):
+        slots = rng.permutation(seqs)[:2700].tolist()
+        n = rng.integers(0, 20, len(slots)).tolist()         # the last ones find no pages left, or outgrow their table
+        pos = kv.extend(slots, np.concatenate([[0], np.cumsum(n)]).tolist())
+        want, _ = model.extend(slots, n)
+        assert pos.tolist() == want
+        same(kv, model)
+    dst = rng.integers(0, seqs, 1500).tolist()
+    src = rng.permutation(seqs)[:1500].tolist()
+    kv.fork(src, dst)
+    model.fork(src, dst)
+    same(kv, model)
+    kv.free(list(range(0, seqs, 2)))
+    model.free(list(range(0, seqs, 2)))
+    same(kv, model)
+    status()
