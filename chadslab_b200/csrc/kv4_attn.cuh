@@ -25,7 +25,11 @@
 //
 // Softmax runs in the exp2 domain with a reference R per column that lags behind the maximum: weights are 2^(s - R), R = max -
 // A, and R moves only when a weight would exceed 2^(A + 4) (A = 11: weights up to 2^15, 2^-24 is the smallest fp16).  A
-// drops when weight * scale overflows, i.e. for values far above one.
+// drops when weight * scale overflows, i.e. for values far above one.  As long as no value scale was above 1/16, the scales
+// of a step are raised in the stage by a power of two (ka_raise): the products would lose in fp16's subnormals what the weights
+// still hold.  What weights and products lose is then at most 2^-31.9 of the largest weight times the largest value
+// per position, however small the values are.  Looking at the first step's scales costs 1 to 2 % (64 x 2048 positions x 16
+// heads of 256: 101.5 -> 103.7 us, ragged batch 66.0 -> 67.1).
 //
 // Work.  The tiles (128 positions, or 64 where two steps of 32 per warp do not fit into shared memory) of all (sequence, KV
 // head, column tile) segments form one list that is cut into equal runs, one per team of four warps: ragged batches and few
@@ -310,6 +314,47 @@ __device__ __forceinline__ void ka_store2(__nv_bfloat16* p, float x, float y) {
 }
 constexpr float KA_LO = 1.0f / 2048.0f;               // weight of the second column of an fp32 row
 
+// `vlim`: a power of two that no value scale so far exceeds, from 2^-15 on; 1 once there was one above 1/16.  Scales are raised by 1 / vlim.
+constexpr float KA_VLIM0 = 1.0f / 32768.0f;
+constexpr float KA_ORDINARY = 1.0f / 16.0f;
+__device__ __forceinline__ float ka_vlim(float vlim, float top) {
+  if (top <= vlim) return vlim;
+  return top > KA_ORDINARY ? 1.0f : __uint_as_float((__float_as_uint(top) + 0x007FFFFFu) & 0x7F800000u);
+}
+__device__ __forceinline__ float ka_inverse(float two_to_the_k) { return __uint_as_float(0x7F000000u - __float_as_uint(two_to_the_k)); }
+// Two value scales of a block, words of the layout (word w of a block: positions r, r + 1 of w % 8), those of positions
+// `live` and behind replaced by zero
+__device__ __forceinline__ uint32_t ka_live_scales(uint32_t x, int w, int live) {
+  const int r = (w >> 1 & 3) * 2 + 8 * (w & 1);
+  return (r < live ? x & 0x0000FFFFu : 0u) | (r + 1 < live ? x & 0xFFFF0000u : 0u);
+}
+// Whether one of the first value scales of a block (D / 32 * 8 words of them) is above 1/16: a warp's first look
+template <int D> __device__ __forceinline__ bool ka_ordinary(const uint8_t* blk, int live) {
+  const int w = (threadIdx.x & 31) % (D / GROUP * 8);
+  const uint32_t x = ka_live_scales(*reinterpret_cast<const uint32_t*>(blk + kv4_vscale_off(D) + w * 4), w, live);
+  return __any_sync(0xffffffffu, __hgt2_mask(ka_half2(x), __floats2half2_rn(KA_ORDINARY, KA_ORDINARY)) != 0u);
+}
+// Raises the value scales of `blocks` blocks (`live` positions) in a warp's stage; returns the new vlim
+template <int D, int BLK>
+__device__ __forceinline__ float ka_raise(uint8_t* stage, int blocks, int live, float vlim) {
+  constexpr int WORDS = D / GROUP * 8;
+  const int lane = threadIdx.x & 31;
+  auto at = [&](int e) { return reinterpret_cast<uint32_t*>(stage + e / WORDS * BLK + kv4_vscale_off(D) + e % WORDS * 4); };
+  auto scales = [&](int e) { return ka_live_scales(*at(e), e % WORDS, live - e / WORDS * KV4_ROWS); };
+  __half2 top2 = __floats2half2_rn(0.0f, 0.0f);
+  for (int e = lane; e < blocks * WORDS; e += 32) top2 = __hmax2(top2, ka_half2(scales(e)));
+  float top = fmaxf(__low2float(top2), __high2float(top2));
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  vlim = ka_vlim(vlim, top);
+  if (vlim == 1.0f) return vlim;
+  const uint32_t up = ka_pack(ka_inverse(vlim), ka_inverse(vlim));
+  for (int e = lane; e < blocks * WORDS; e += 32) *at(e) = ka_mul2(scales(e), up);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the copy that will fill the stage again
+  __syncwarp();
+  return vlim;
+}
+
 // ---- variants ------------------------------------------------------------------------------------------------------------------
 template <typename T, int NG, int NC> struct KaCfg {
   static constexpr int SL = sizeof(T) == 4 ? 2 : 1;
@@ -494,6 +539,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
     // ---- the positions ----------------------------------------------------------------------------------------------------
     float acc[2 * NG][4], ref[2], l[2];
     float A = 11.0f;
+    float vlim = KA_VLIM0;                                     // acc carries the 1 / vlim of the scales
 #pragma unroll
     for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
@@ -511,6 +557,16 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
         *(volatile int*)a.status = (int)BQ_ERR_TIMEOUT;
       }
       const int step0 = ((first + i) * KA_WARPS + warp) * STEP * KV4_ROWS;
+      if (vlim < 1.0f) {
+        const float was = vlim;
+        const int live = end - step0;
+        vlim = ka_ordinary<D>(ring + take * C::STAGE, live) ? 1.0f : ka_raise<D, C::BLK>(ring + take * C::STAGE, live <= KV4_ROWS ? 1 : STEP, live, was);
+        const float lower = was * ka_inverse(vlim);
+#pragma unroll
+        for (int x = 0; x < 2 * NG; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[x][j] *= lower;
+      }
 #pragma unroll 1
       for (int u0 = 0; u0 < STEP; u0 += U) {
         if (U == 1 && u0 && step0 + KV4_ROWS >= end) break;    // no second block
@@ -675,8 +731,8 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
               }
             }
           }
-          const bool over = high > A + 4.0f || fmaxf(__low2float(top), __high2float(top)) > 60000.0f;
-          if (!__any_sync(0xffffffffu, over) || tries == 8) break;
+          const bool large = fmaxf(__low2float(top), __high2float(top)) > 60000.0f;
+          if (!__any_sync(0xffffffffu, high > A + 4.0f || large) || tries == 8) break;
           // The reference moves up to the maximum so far; if that was not enough, a weight times its scale leaves fp16 and
           // all weights become 16 times smaller.
           const float drop = tries ? 4.0f : 0.0f;
@@ -809,7 +865,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
         float r = s_ref[c];
 #pragma unroll
         for (int w = 1; w < KA_WARPS; ++w) r = fmaxf(r, s_ref[w * W + c]);
-        corr[j] = ka_exp2(ref[j] - r) * (SL == 2 && j ? KA_LO : 1.0f);
+        corr[j] = ka_exp2(ref[j] - r) * vlim * (SL == 2 && j ? KA_LO : 1.0f);
       }
     // (row, head) hc = column hc * SL of the tile: its reference and sum, and where its output goes
     float* part = a.part + ((int64_t)run * 2 + (begins ? 1 : 0)) * (HC * (D + 4));

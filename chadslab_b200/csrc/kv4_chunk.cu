@@ -7,8 +7,8 @@
 //   * The fragment words of the cache are B fragments as they lie: for keys (n = position) words r0, r1 and r2, r3 are those
 //     of positions 0-7 and 8-15, for values (n = dimension) r0, r2 and r1, r3 those of dimensions 0-7 and 8-15.
 //   * Codes stay whole numbers (exact in fp16).  A key group's scale multiplies its 32-dimension sum in fp32, a value's scale
-//     multiplies the weight, as in the decode kernel; so do the power-of-two scaling of q, the lagging softmax reference and
-//     the list of tiles that is cut into equal runs (here one per SM) and merged.
+//     multiplies the weight, as in the decode kernel; so do the power-of-two scaling of q, the lagging softmax reference,
+//     the raising of small value scales and the list of tiles that is cut into equal runs (here one per SM) and merged.
 // Bound: shared memory.  Every 512-byte B fragment is read for two matrix instructions (a warp has 16 rows; 32 would need 256
 // accumulator registers at head_dim 256), which is 128 bytes per cycle and SM at the matrix pipe's full rate: 117 TFLOP/s at
 // 512 rows, 8 heads on one KV head of 256.  Unpacking the next tile while this one is multiplied (two buffers, half the tile
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
     }
     const int all_see = seq.pos + a.by_rep(at.ct * KK_ROWS);
 
-    float o[4 * NG][4], ref[2], l[2], A = 11.0f;
+    float o[4 * NG][4], ref[2], l[2], A = 11.0f, vlim = KA_VLIM0;      // o carries the 1 / vlim of the scales
 #pragma unroll
     for (int i = 0; i < 4 * NG; ++i)
 #pragma unroll
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
       }
       --flying;
       // ---- unpack: warp w takes (block, group) units -----------------------------------------------------------------------------
-      const uint8_t* stage = raw + take * KK_BLOCKS * C::BLK;
+      uint8_t* stage = raw + take * KK_BLOCKS * C::BLK;
       const int p0 = tile * KK_TILE;
       float vtop = 0.0f;
 #pragma unroll
@@ -189,11 +189,33 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
           if (p0 + blk * 16 + r < end) vtop = fmaxf(vtop, vs);
         }
       }
-      if (vtop > 1.0f) atomicMax(&sh->vmax[take], __float_as_int(vtop));
+      if (vlim < 1.0f) vtop = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)));
+      if (vlim < 1.0f ? lane == 0 : vtop > 1.0f) atomicMax(&sh->vmax[take], __float_as_int(vtop));
       __syncthreads();
       // values above one: weights stay so far below 2^15 that their product with the largest scale does too
       const float vbig = __int_as_float(sh->vmax[take]);
       const float want = vbig > 1.0f ? 11.0f - (float)((__float_as_int(vbig) >> 23) - 126) : 11.0f;
+      if (vlim < 1.0f) {                                         // no scale above 1/16 before this tile: see kv4_attn.cuh
+        const float was = vlim;
+        vlim = ka_vlim(was, vbig);
+        const float lower = was * ka_inverse(vlim);
+        if (tile > first) {
+#pragma unroll
+          for (int i = 0; i < 4 * NG; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] *= lower;
+        }
+        if (vlim < 1.0f) {
+          constexpr int WORDS = NG * 8;
+          const uint32_t up = ka_pack(ka_inverse(vlim), ka_inverse(vlim));
+          for (int e = tid; e < KK_BLOCKS * WORDS; e += KK_THREADS) {
+            uint32_t* p = reinterpret_cast<uint32_t*>(stage + e / WORDS * C::BLK + kv4_vscale_off(D) + e % WORDS * 4);
+            *p = ka_mul2(ka_live_scales(*p, e % WORDS, end - p0 - e / WORDS * KV4_ROWS), up);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the copy that will fill the stage again
+          __syncthreads();
+        }
+      }
       // ---- scores: rows g, g + 8; positions 8 n + 2t, + 1 -------------------------------------------------------------------------
       float s[2 * KK_BLOCKS][4];
 #pragma unroll
@@ -334,12 +356,12 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
       if (i >= was_seq.n) continue;
       if (whole) {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + ((int64_t)(was_seq.row0 + i) * a.Hq + was.h * a.rep + rh - i * a.rep) * D + 2 * t;
-        const float inv = 1.0f / z;
+        const float inv = vlim / z;
 #pragma unroll
         for (int x = 0; x < 4 * NG; ++x) ka_store2(out + x * 8, o[x][2 * j] * inv, o[x][2 * j + 1] * inv);
       } else {
 #pragma unroll
-        for (int x = 0; x < 4 * NG; ++x) ka_store2(part + hc * D + x * 8 + 2 * t, o[x][2 * j], o[x][2 * j + 1]);
+        for (int x = 0; x < 4 * NG; ++x) ka_store2(part + hc * D + x * 8 + 2 * t, o[x][2 * j] * vlim, o[x][2 * j + 1] * vlim);
         if (t == 0) { part[KK_ROWS * D + 2 * hc] = ref[j]; part[KK_ROWS * D + 2 * hc + 1] = z; }
       }
     }

@@ -1,0 +1,93 @@
+"""Attention over the paged 4-bit KV cache where its operands leave the middle of fp16's range, against 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4 as okv
+from test_gpu_kv4 import DT, ints, make, many_rows, num, rows, starts_of, status
+
+pytestmark = pytest.mark.gpu
+
+
+def limit(o, mag, size, V, dtype):
+    """Per element.  What is lost of small weights and products shrinks with the values.  The largest weight is held as 2^11 or
+    more, the largest value scale as 1/16 or more (2^-15 of it where the scales are below that).  bf16 rows: a weight loses up to
+    half a step of the smallest fp16, 2^-25, which is 2^-36 of the largest weight, times a value; its product with a scale the
+    same 2^-25 times a code of at most 7: 2^-25 / 2^11 * 16 * (7 times the largest scale) = 2^-32 of the largest value.  fp32
+    rows hold both in two halves, the second of them 2^-11 of the first.  The rest as for values around one: roundings to
+    fp16 (twice, 2^-11 each), exponents and sums in fp32 (2^-20), scores (their sum of |q k| times 2^-22 and 16 additions of
+    2^-24, for subnormal keys 2^-18, numerator and denominator)."""
+    most = np.abs(V).max()
+    score = 2.0 * size * (2.0 ** -22 + 16 * 2.0 ** (-24 if dtype == "f32" else -18))
+    lost = len(V) * (2.0 ** -36 * most + max(2.0 ** -32 * most, 7 * 2.0 ** -51))
+    if dtype == "f32":
+        return (2.0 ** -20 + score) * mag + lost * 2.0 ** -11
+    return ((2 * 2.0 ** -11 + 2.0 ** -20 + score) * mag + lost) * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(o)
+
+
+def put(kv, ks, vs, dtype):
+    """Sequences with the given keys and values [len, heads, D] (numpy) -> what the cache holds of each, in 64 bits."""
+    lens = [len(k) for k in ks]
+    starts = starts_of(lens)
+    k, v = (torch.from_numpy(np.concatenate(x).astype(np.float32)).cuda().to(DT[dtype]) for x in (ks, vs))
+    kv.append(0, k, v, None, kv.extend(None, starts), starts)
+    at = np.concatenate([[0], np.cumsum(lens)])
+    K, V = okv.held(num(k)), okv.held(num(v))
+    return [(K[at[b]:at[b + 1]], V[at[b]:at[b + 1]]) for b in range(len(lens))]
+
+
+def compare(kv, data, q, new, dtype):
+    lens = [len(k) for k, _ in data]
+    pos = [n - m for n, m in zip(lens, new)]
+    out = num(kv.attention(0, q, None, ints(pos), None if all(m == 1 for m in new) else starts_of(new)))
+    at = np.concatenate([[0], np.cumsum(new)])
+    for b, (K, V) in enumerate(data):
+        one = slice(at[b], at[b + 1])
+        o, mag, size = okv.attention(num(q)[one], K, V, pos[b])
+        err, tol = np.abs(out[one] - o), limit(o, mag, size, V, dtype)
+        assert (err <= tol).all(), f"sequence {b}: {np.nanmax(err / tol):.3g} x the bound, {np.abs(out[one] - o).max() / np.abs(o).max():.3g} relative"
+    assert status() == 0
+
+
+SHAPES = [("f32", 64, 1, 1, 1), ("f32", 128, 2, 2, 1), ("f32", 256, 1, 8, 3), ("bf16", 64, 1, 1, 1), ("bf16", 64, 1, 2, 1), ("bf16", 96, 2, 2, 1),
+          ("bf16", 128, 1, 4, 1), ("bf16", 128, 1, 8, 5), ("bf16", 256, 2, 1, 1), ("bf16", 256, 1, 8, 1), ("bf16", 64, 24, 2, 60),
+          ("bf16", 128, 24, 2, 60), ("bf16", 256, 24, 2, 60)]
+
+
+def pool(dtype, D, Hkv, rep, rows_each, seqs=2):
+    kv = make(1, Hkv, D, n_pages=64, max_pages=24, page=32)
+    assert many_rows(kv, Hkv * rep, seqs, seqs * rows_each) == (rows_each == 60)
+    return kv
+
+
+@pytest.mark.parametrize("vscale", [1.0, 1e-2, 1e-3, 1e-4, 1e-6])
+@pytest.mark.parametrize("nats", [15, 18])
+@pytest.mark.parametrize("dtype,D,Hkv,rep,rows_each", SHAPES)
+def test_small_values_below_a_position_without_any(cuda_lib, dtype, D, Hkv, rep, rows_each, nats, vscale):
+    """Every sixteenth position takes nearly all the weight and has the value zero: the output is what is left of the others."""
+    rng = np.random.default_rng(nats)
+    kv = pool(dtype, D, Hkv, rep, rows_each)
+    b = np.sign(rng.normal(size=D))
+    ks, vs = [], []
+    for n in (75, 200):
+        k, v = rng.normal(0, 0.05, (n, Hkv, D)), rng.normal(0, vscale, (n, Hkv, D))
+        k[5::16], v[5::16] = b * nats / np.sqrt(D), 0.0
+        ks.append(k), vs.append(v)
+    data = put(kv, ks, vs, dtype)
+    q = torch.from_numpy((b + rng.normal(0, 0.05, (2 * rows_each, Hkv * rep, D))).astype(np.float32)).cuda().to(DT[dtype])
+    compare(kv, data, q, [rows_each] * 2, dtype)
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed", "one large"])
+@pytest.mark.parametrize("dtype,D,Hkv,rep,rows_each", SHAPES)
+def test_values_of_many_magnitudes(cuda_lib, dtype, D, Hkv, rep, rows_each, order):
+    """From 1e-6 to 1e5 within a sequence: the range that products are held in follows the largest one so far."""
+    rng = np.random.default_rng(3)
+    kv = pool(dtype, D, Hkv, rep, rows_each)
+    ks, vs = [], []
+    for n in (130, 333):
+        e = np.linspace(-6, 5, n)
+        e = {"rising": e, "falling": e[::-1], "mixed": rng.permutation(e), "one large": np.where(np.arange(n) == n - 20, 3.0, -4.0)}[order]
+        ks.append(rng.normal(0, 1, (n, Hkv, D))), vs.append(rng.normal(0, 1, (n, Hkv, D)) * 10.0 ** e[:, None, None])
+    data = put(kv, ks, vs, dtype)
+    compare(kv, data, rows(rng, 2 * rows_each, Hkv * rep, D, dtype, 1.5), [rows_each] * 2, dtype)
