@@ -9,6 +9,7 @@
 namespace bq {
 
 constexpr int KP_THREADS = 1024;
+constexpr int KP_LARGE = 1 << 20;                         // pages: 1024 such needs fit into 31 bits
 constexpr int KP_PER = 16;                                // reference counts a thread looks at per pass (four 16-byte loads)
 
 // ---- workspace (int32) -------------------------------------------------------------------------------------------------
@@ -101,14 +102,14 @@ __global__ void __launch_bounds__(KP_THREADS) kv4_extend_kernel(KpPool p, const 
                                                                 int B, int32_t* pos_out, int* status) {
   extern __shared__ int owner[];                     // first batch entry that names a slot
   __shared__ int red[32];
-  __shared__ int s_copies;
+  __shared__ int s_copies, s_large;
   pdl_launch_dependents();
   pdl_wait();
   const KpWork w = kp_work(p.work, p.n_pages, p.max_seqs);
   const int64_t room = (int64_t)p.max_pages << p.page_log2;
   const int page = 1 << p.page_log2;
   for (int i = threadIdx.x; i < p.max_seqs; i += KP_THREADS) owner[i] = B;
-  if (threadIdx.x == 0) s_copies = 0;
+  if (threadIdx.x == 0) s_copies = s_large = 0;
   __syncthreads();
   for (int b = threadIdx.x; b < B; b += KP_THREADS) {
     const int s = slots ? slots[b] : b;
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(KP_THREADS) kv4_extend_kernel(KpPool p, const 
   }
   __syncthreads();
   // what each sequence lacks; pairs[2 b] = pages, pairs[2 b + 1] = pages of the sequences before it (-1: refused)
-  int total = 0;
+  int64_t total = 0;
   for (int b0 = 0; b0 < B; b0 += KP_THREADS) {
     const int b = b0 + (int)threadIdx.x;
     int need = 0, ok = 0;
@@ -138,27 +139,48 @@ __global__ void __launch_bounds__(KP_THREADS) kv4_extend_kernel(KpPool p, const 
       }
       if (!ok) *(volatile int*)status = (int)BQ_ERR_ARG;
     }
+    // what a call asks for can pass 2^31 pages even if the pool cannot: needs of 2^20 and more take the pass below
+    if (need > KP_LARGE) s_large = 1;
+    const int sum = need < KP_LARGE ? need : KP_LARGE;
     int chunk;
-    const int upto = kp_scan(need, red, &chunk);
+    const int64_t before = total + kp_scan(sum, red, &chunk) - sum;
     if (b < B) {
       w.pairs[2 * b] = need;
-      w.pairs[2 * b + 1] = ok ? total + upto - need : -1;
+      w.pairs[2 * b + 1] = !ok ? -1 : before < p.n_pages ? (int)before : (int)p.n_pages;
     }
     total += chunk;
   }
   __syncthreads();
+  if (s_large) total = p.n_pages + 1;
   int found = 0;
-  if (total > 0) found = kp_list<false>(p.refs, p.n_pages, total, w.list, nullptr, red);
+  if (total > 0) found = kp_list<false>(p.refs, p.n_pages, (int)(total < p.n_pages ? total : p.n_pages), w.list, nullptr, red);
   __syncthreads();
-  // a sequence whose pages are not all there is refused and changes nothing
   const int lane = threadIdx.x & 31;
+  if (total > found) {
+    // Not all can be served.  A sequence that needs more than is left is refused and changes nothing; the ones behind it
+    // have what it did not get.
+    if (threadIdx.x < 32) {
+      int taken = 0;
+      for (int b0 = 0; b0 < B; b0 += 32) {
+        const int b = b0 + lane, need = b < B ? w.pairs[2 * b] : 0;
+        int at = b < B ? w.pairs[2 * b + 1] : -1;
+        for (int j = 0; j < 32; ++j) {
+          const int n = __shfl_sync(0xffffffffu, at >= 0 ? need : 0, j);
+          const bool fits = n <= found - taken;
+          if (lane == j && at >= 0) at = fits ? taken : -1;
+          if (fits) taken += n;
+        }
+        if (b < B) w.pairs[2 * b + 1] = at;
+      }
+    }
+    __syncthreads();
+  }
   for (int b0 = 0; b0 < B; b0 += KP_THREADS / 32) {
     const int b = b0 + (int)(threadIdx.x >> 5);
     int from = -1, to = -1;
     if (b < B) {
       const int need = w.pairs[2 * b], at = w.pairs[2 * b + 1];
-      const bool given = at >= 0 && (need == 0 || at + need <= found);
-      if (!given) {
+      if (at < 0) {
         if (lane == 0) pos_out[b] = -1;
       } else {
         const int s = slots ? slots[b] : b;

@@ -138,8 +138,8 @@ class PagedKV4:
 
     # ---- pages --------------------------------------------------------------------------------------------------------
     def extend(self, slots=None, starts=None, batch: int = 0):
-        """Room for every sequence's new rows (starts None: one each) -> pos int32 [B], the length before, -1 where no pages
-        were left.  `batch` gives B when both are None."""
+        """Room for every sequence's new rows (starts None: one each) -> pos int32 [B], the length before, -1 where fewer pages
+        were left than the sequence needs (later ones of the batch are served all the same).  `batch` gives B when both are None."""
         if slots is not None:
             slots = self._ints(slots, "slots")
         if starts is not None:

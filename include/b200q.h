@@ -362,8 +362,9 @@ int64_t bq_kv4_work_bytes(const bq_kv4_pool* p);
  * A slot, row range or position outside the pool records BQ_ERR_ARG in the status word and is treated like pos < 0.       */
 /* Makes room for each sequence's new rows: lens += rows, pages are given out lowest number first in batch order, and a
  * partly filled last page that other sequences hold too is replaced by a copy (every layer).  pos_out[b] = the length
- * before the call, or -1 if the sequence was refused and is unchanged: no pages left, longer than max_pages allows, or its
- * slot already named earlier in the batch (the last two record BQ_ERR_ARG).                                              */
+ * before the call, or -1 if the sequence was refused and is unchanged: it needs more pages than those in front of it have left
+ * (the ones behind it are served from the same pages), is longer than max_pages allows, or its slot was already named
+ * earlier in the batch (the last two record BQ_ERR_ARG).                                                                 */
 int bq_kv4_extend(const bq_kv4_pool* p, const int32_t* slots, const int32_t* starts, int64_t B, int32_t* pos_out,
                   void* stream);
 /* Sequence dst[i] becomes a copy of sequence src[i], all as if at once: it holds the same pages (each counted once more)

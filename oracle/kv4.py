@@ -88,10 +88,10 @@ class Pool:
             had, has = self._count(len_), self._count(len_ + n)
             cow = int(n > 0 and len_ % self.page != 0 and refs[self.tables[s, had - 1]] > 1)
             need, at = has - had + cow, taken
-            taken += need
-            if need and taken > len(free):
+            if need > len(free) - taken:                 # not enough left; the ones behind it are served all the same
                 pos.append(-1)
                 continue
+            taken += need
             new = free[at:at + need]
             if cow:
                 old = int(self.tables[s, had - 1])
