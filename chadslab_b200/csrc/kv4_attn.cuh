@@ -45,12 +45,14 @@
 // contexts of 131072 with the same heads 45 us = 3.4 TB/s (eight columns per position block: bound by its instructions).
 #pragma once
 #include "kv4.cuh"
+#include "kv4_ring.h"
 
 namespace bq {
 
 constexpr int KA_WARPS = 4;                           // of a team: the warps that work on one run
 constexpr int KA_THREADS = KA_WARPS * 32;
-constexpr uint64_t KA_WAIT_NS = 2000000000ull;        // bound of the wait for a copy
+constexpr uint64_t KA_WAIT_NS = 2000000000ull;        // bound of the wait for a copy; a warp runs into it once, and once more for
+                                                      // all that is still under way when it leaves
 
 // x / d for 0 <= x < 2^31
 struct KaDiv {
@@ -256,22 +258,24 @@ __device__ __forceinline__ bool ka_bar_test(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-static __device__ __noinline__ bool ka_bar_wait_long(uint32_t bar, uint32_t parity) {
-  uint64_t t0, t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+__device__ __forceinline__ uint64_t ka_now() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+static __device__ __noinline__ bool ka_bar_wait_long(uint32_t bar, uint32_t parity, uint64_t t0) {
+  if (t0 == 0) t0 = ka_now();
   do {
     for (int i = 0; i < 1024; ++i)
       if (ka_bar_test(bar, parity)) return true;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  } while (t - t0 < KA_WAIT_NS);
+  } while (ka_now() - t0 < KA_WAIT_NS);
   return false;
 }
-// lane 0 polls, the warp follows; false (to lane 0): the copy did not arrive in time
-__device__ __forceinline__ bool ka_bar_wait(uint32_t bar, uint32_t parity, int lane) {
+// lane 0 polls, the warp follows; false: the copy did not arrive in time (counted from t0, 0: from now)
+__device__ __forceinline__ bool ka_bar_wait(uint32_t bar, uint32_t parity, int lane, uint64_t t0 = 0) {
   bool ok = true;
-  if (lane == 0 && !ka_bar_test(bar, parity)) ok = ka_bar_wait_long(bar, parity);
-  __syncwarp();
-  return ok;
+  if (lane == 0 && !ka_bar_test(bar, parity)) ok = ka_bar_wait_long(bar, parity, t0);
+  return __all_sync(0xffffffffu, ok);
 }
 
 // ---- arithmetic --------------------------------------------------------------------------------------------------------------
@@ -422,10 +426,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
   Kv4Seq seq = ka_seq(a, at.b);
   int end = ka_end(a, seq, at.ct), tiles = (end + TILE - 1) / TILE;
   int cts = ka_col_tiles(a, seq);
-  int put = 0, take = 0;
-  uint32_t phase = 0;                                          // stage to fill next, stage to read next and its parity
-  int flying = 0;                                              // copies under way
-  bool dead = false;
+  Kv4Ring<S> copies;
   const int pb = a.v.page_blocks_log2();
   const int32_t* row = a.v.tables + (int64_t)seq.slot * a.v.max_pages;
   // One lane requests this warp's blocks of a tile into stage `st`; `blocks` = blocks of the segment
@@ -448,10 +449,9 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
   };
   // The ring is empty: the first steps of a piece, one lane each
   auto fill = [&](const int32_t* row, int h, int first, int steps, int blocks) {
-    const int n = steps < S ? steps : S;
-    if (lane < n) request(row, h, first + lane, blocks, put + lane >= S ? put + lane - S : put + lane);
-    put = put + n >= S ? put + n - S : put + n;
-    flying += n;
+    const int n = copies.room(steps);
+    if (lane < n) request(row, h, first + lane, blocks, copies.stage(lane));
+    copies.requested(n);
     return n;
   };
   int first = at.tile;
@@ -551,16 +551,17 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
       l[j] = 0.0f;
     }
     for (int i = 0; i < mine; ++i) {
-      const uint8_t* stage = ring + take * C::STAGE;
-      if (!ka_bar_wait(bar0 + take * 8, phase, lane)) {        // a copy did not arrive: record it and go on with what is there
-        dead = true;
+      // a copy that does not arrive: recorded; this warp takes no further part but in the merges
+      if (!copies.arrived([&](int st, uint32_t parity) { return ka_bar_wait(bar0 + st * 8, parity, lane); })) {
         *(volatile int*)a.status = (int)BQ_ERR_TIMEOUT;
+        break;
       }
+      uint8_t* stage = ring + copies.take * C::STAGE;
       const int step0 = ((first + i) * KA_WARPS + warp) * STEP * KV4_ROWS;
       if (vlim < 1.0f) {
         const float was = vlim;
         const int live = end - step0;
-        vlim = ka_ordinary<D>(ring + take * C::STAGE, live) ? 1.0f : ka_raise<D, C::BLK>(ring + take * C::STAGE, live <= KV4_ROWS ? 1 : STEP, live, was);
+        vlim = ka_ordinary<D>(stage, live) ? 1.0f : ka_raise<D, C::BLK>(stage, live <= KV4_ROWS ? 1 : STEP, live, was);
         const float lower = was * ka_inverse(vlim);
 #pragma unroll
         for (int x = 0; x < 2 * NG; ++x)
@@ -802,13 +803,11 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
             }
         }
       }
-      --flying;
-      if (++take == S) { take = 0; phase ^= 1u; }
+      copies.consumed();
       __syncwarp();                                            // the stage has been read by every lane
       if (ahead < mine) {
-        if (lane == 0) request(row, at.h, first + ahead, blocks, put);
-        put = put + 1 == S ? 0 : put + 1;
-        ++flying;
+        if (lane == 0) request(row, at.h, first + ahead, blocks, copies.put);
+        copies.requested(1);
         ++ahead;
       }
     }
@@ -840,7 +839,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
       first = 0;
       last = tiles < left ? tiles : left;
       blocks = (end + KV4_ROWS - 1) / KV4_ROWS;
-      mine = my_steps();
+      mine = copies.dead ? 0 : my_steps();
       ahead = fill(row, at.h, 0, mine, blocks);
     }
 
@@ -939,11 +938,9 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
     }
     if (left <= 0) break;
   }
-  if (__shfl_sync(0xffffffffu, dead, 0)) {                     // do not leave with copies in flight
-    for (; flying > 0; --flying) {
-      ka_bar_wait(bar0 + take * 8, phase, lane);
-      if (++take == S) { take = 0; phase ^= 1u; }
-    }
+  if (copies.dead) {                                           // do not leave with copies in flight
+    const uint64_t t0 = ka_now();
+    copies.drain([&](int st, uint32_t parity) { return ka_bar_wait(bar0 + st * 8, parity, lane, t0); });
   }
 }
 

@@ -22,12 +22,13 @@ constexpr int KK_THREADS = KK_WARPS * 32;
 constexpr int KK_ROWS = KK_WARPS * 16;                // (row, head) pairs of a tile
 constexpr int KK_BLOCKS = 4;                          // 16-position blocks of a tile
 constexpr int KK_TILE = KK_BLOCKS * KV4_ROWS;
+constexpr int KK_LOST = 0x7FFFFFFF;                   // in vmax: the tile's copies did not arrive
 
 struct KkShared {
   KaScan scan;
   KaPlace at;
   int total, per, ok;
-  int vmax[2];                                        // largest value scale of a stage's tile (bits of a float)
+  int vmax[2];                                        // largest value scale of a stage's tile (bits of a float), or KK_LOST
   uint64_t bar[2];
 };
 template <int NG> struct KkCfg {
@@ -82,11 +83,8 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
   const int pb = a.v.page_blocks_log2();
   int first = at.tile, last = tiles - first < left ? tiles : first + left;
   const int32_t* row = a.v.tables + (int64_t)seq.slot * a.v.max_pages;
-  int take = 0;                                                  // stage of the tile at hand; the other one is being filled
-  uint32_t phase = 0;
-  bool dead = false;
-  int flying = 0;
-  // warp 0 requests a tile's blocks, one lane each
+  Kv4Ring<2> copies;                                             // the same in every warp; warp 0 requests
+  // a tile's blocks, one lane each
   auto request = [&](int tile, int st) {
     const int blocks = (end + KV4_ROWS - 1) / KV4_ROWS, b0 = tile * KK_BLOCKS, n = blocks - b0 < KK_BLOCKS ? blocks - b0 : KK_BLOCKS;
     if (lane == 0) ka_bar_expect(bar0 + st * 8, n * C::BLK);
@@ -102,9 +100,9 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
       ka_bulk_load(ka_smem(raw + (st * KK_BLOCKS + lane) * C::BLK), a.v.pages + (int64_t)id * a.v.page_bytes + (a.v.layer_off + (int64_t)in * C::BLK),
                    C::BLK, bar0 + st * 8);
     }
-    ++flying;
   };
-  if (warp == 0) request(first, take);
+  if (warp == 0) request(first, copies.put);
+  copies.requested(1);
 
   while (true) {
     // ---- this warp's 16 pairs: rows g and g + 8 of its A fragments ---------------------------------------------------------------
@@ -159,15 +157,19 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
       l[j] = 0.0f;
     }
     for (int tile = first; tile < last; ++tile) {
-      if (warp == 0 && tile + 1 < last) request(tile + 1, take ^ 1);
-      if (!ka_bar_wait(bar0 + take * 8, phase, lane)) {          // a copy did not arrive: record it and go on with what is there
-        dead = true;
-        *(volatile int*)a.status = (int)BQ_ERR_TIMEOUT;
+      if (tile + 1 < last) {
+        if (warp == 0) request(tile + 1, copies.put);
+        copies.requested(1);
       }
-      --flying;
-      // ---- unpack: warp w takes (block, group) units -----------------------------------------------------------------------------
+      // a copy that does not arrive: recorded, and all warps leave behind the next barrier
+      if (!copies.arrived([&](int st, uint32_t parity) { return ka_bar_wait(bar0 + st * 8, parity, lane); })) {
+        *(volatile int*)a.status = (int)BQ_ERR_TIMEOUT;
+        if (lane == 0) atomicMax(&sh->vmax[copies.take], KK_LOST);
+      }
+      const int take = copies.take;
       uint8_t* stage = raw + take * KK_BLOCKS * C::BLK;
       const int p0 = tile * KK_TILE;
+      // ---- unpack: warp w takes (block, group) units -----------------------------------------------------------------------------
       float vtop = 0.0f;
 #pragma unroll
       for (int u = warp; u < KK_BLOCKS * NG; u += KK_WARPS) {
@@ -192,8 +194,13 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
       if (vlim < 1.0f) vtop = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)));
       if (vlim < 1.0f ? lane == 0 : vtop > 1.0f) atomicMax(&sh->vmax[take], __float_as_int(vtop));
       __syncthreads();
+      const int vbits = sh->vmax[take];
+      if (vbits == KK_LOST) {
+        copies.dead = true;
+        break;
+      }
       // values above one: weights stay so far below 2^15 that their product with the largest scale does too
-      const float vbig = __int_as_float(sh->vmax[take]);
+      const float vbig = __int_as_float(vbits);
       const float want = vbig > 1.0f ? 11.0f - (float)((__float_as_int(vbig) >> 23) - 126) : 11.0f;
       if (vlim < 1.0f) {                                         // no scale above 1/16 before this tile: see kv4_attn.cuh
         const float was = vlim;
@@ -313,9 +320,9 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
       }
       __syncthreads();                                           // the tile has been read by every warp
       if (tid == 0) sh->vmax[take] = 0;
-      take ^= 1;
-      if (take == 0) phase ^= 1u;
+      copies.consumed();
     }
+    if (copies.dead) break;
 
     // ---- where this run goes next: its first tile travels while this piece is stored -----------------------------------------------
     const KaPlace was = at;
@@ -343,7 +350,8 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
       tiles = (end + KK_TILE - 1) / KK_TILE;
       first = 0;
       last = tiles < left ? tiles : left;
-      if (warp == 0) request(0, take);
+      if (warp == 0) request(0, copies.put);
+      copies.requested(1);
     }
     // ---- this warp's rows --------------------------------------------------------------------------------------------------------------
     float* part = a.part + ((int64_t)run * 2 + (begins ? 1 : 0)) * (KK_ROWS * (D + 4));
@@ -372,12 +380,9 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
     }
     if (left <= 0) break;
   }
-  if (warp == 0 && __shfl_sync(0xffffffffu, dead, 0)) {          // do not leave with copies in flight
-    for (; flying > 0; --flying) {
-      ka_bar_wait(bar0 + take * 8, phase, lane);
-      take ^= 1;
-      if (take == 0) phase ^= 1u;
-    }
+  if (warp == 0 && copies.dead) {                                // do not leave with copies in flight
+    const uint64_t t0 = ka_now();
+    copies.drain([&](int st, uint32_t parity) { return ka_bar_wait(bar0 + st * 8, parity, lane, t0); });
   }
 }
 
