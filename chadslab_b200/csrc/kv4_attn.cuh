@@ -25,7 +25,8 @@
 //
 // Softmax runs in the exp2 domain with a reference R per column that lags behind the maximum: weights are 2^(s - R), R = max -
 // A, and R moves only when a weight would exceed 2^(A + 4) (A = 11: weights up to 2^15, 2^-24 is the smallest fp16).  A
-// drops when weight * scale overflows, i.e. for values far above one.  As long as no value scale was above 1/16, the scales
+// drops when weight * scale overflows, i.e. for values far above one.  Weights end at 2^(A + 4): where scores are so large that
+// fp32 has steps of 16 and more (2^27), R cannot be set closer to their maximum; it is rounded down.  As long as no value scale was above 1/16, the scales
 // of a step are raised in the stage by a power of two (ka_raise): the products would lose in fp16's subnormals what the weights
 // still hold.  What weights and products lose is then at most 2^-31.9 of the largest weight times the largest value
 // per position, however small the values are.  Looking at the first step's scales costs 1 to 2 % (64 x 2048 positions x 16
@@ -299,6 +300,11 @@ __device__ __forceinline__ float ka_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float ka_min(float a, float b) {              // NaN stays
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 __device__ __forceinline__ uint32_t ka_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 ka_half2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ uint32_t ka_pack(float lo, float hi) { return ka_bits(__floats2half2_rn(lo, hi)); }
@@ -491,8 +497,10 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
       for (int off = 1; off < 32; off <<= 1)
         if (off < 4 || off >= 4 * NC) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
       int k2 = 13 - ((int)(__float_as_uint(big) >> 23) - 127);          // big * 2^k2 is in [2^13, 2^14)
-      k2 = k2 > 100 ? 100 : k2 < -100 ? -100 : k2;
+      k2 = k2 > 100 ? 100 : k2 < -114 ? -114 : k2;
       const float up = __uint_as_float((uint32_t)(127 + k2) << 23);
+      // queries past 2^113: scores of that size are all or nothing, so they may come out 2^-14 of what they are
+      k2 = k2 < -100 ? -100 : k2;
       const bool second = SL == 2 && (col & 1);
       float sum[NF];
 #pragma unroll
@@ -678,7 +686,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
                 if (J == 1 && (j & 1)) { w[j] = w[j - 1]; continue; }
                 w[j] = fmaf(s[u][j], kappa[j & 1], -ref[j & 1]);
                 high = fmaxf(high, w[j]);
-                w[j] = ka_exp2(w[j]);
+                w[j] = ka_exp2(ka_min(w[j], A + 4.0f));
               }
               uint32_t m0, m1;                                 // rows g, g + 8: columns 2t, 2t + 1
               if (SL == 1) {
@@ -734,8 +742,9 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
           }
           const bool large = fmaxf(__low2float(top), __high2float(top)) > 60000.0f;
           if (!__any_sync(0xffffffffu, high > A + 4.0f || large) || tries == 8) break;
-          // The reference moves up to the maximum so far; if that was not enough, a weight times its scale leaves fp16 and
-          // all weights become 16 times smaller.
+          // The reference moves up to the maximum so far; if after that a weight times its scale leaves fp16, all weights become
+          // 16 times smaller.
+          if (tries && !__any_sync(0xffffffffu, large)) break;        // (the limit above holds the weights)
           const float drop = tries ? 4.0f : 0.0f;
           A -= drop;
 #pragma unroll
@@ -747,7 +756,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
               float m = -INFINITY;
 #pragma unroll
               for (int u = 0; u < U; ++u) m = fmaxf(m, fmaxf(s[u][j], s[u][j + 2]));
-              m *= kappa[j];
+              m = __fmul_rd(m, kappa[j]);
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));

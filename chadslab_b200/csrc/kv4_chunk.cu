@@ -126,8 +126,9 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         int k2 = 13 - ((int)(__float_as_uint(big) >> 23) - 127);
-        k2 = k2 > 100 ? 100 : k2 < -100 ? -100 : k2;
+        k2 = k2 > 100 ? 100 : k2 < -114 ? -114 : k2;
         up[j] = __uint_as_float((uint32_t)(127 + k2) << 23);
+        k2 = k2 < -100 ? -100 : k2;                              // as in the decode kernel
         kappa[j] = __uint_as_float((uint32_t)(127 - k2) << 23) * 1.4426950408889634f * rsqrtf((float)D);
         vis[j] = ok[j] ? seq.pos + i : 0x7FFFFFFF;
       }
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
         A = low;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float m = high[j] * kappa[j];
+          float m = __fmul_rd(high[j], kappa[j]);
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
           const float r = fmaxf(ref[j] + drop, m - A), corr = ka_exp2(ref[j] - r);
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(KK_THREADS, 1) kv4_chunk_kernel(const __grid_c
         float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          w[j] = ka_exp2(fmaf(s[n][j], kappa[j >> 1], -ref[j >> 1]));
+          w[j] = ka_exp2(ka_min(fmaf(s[n][j], kappa[j >> 1], -ref[j >> 1]), A + 4.0f));
           l[j >> 1] += w[j];
         }
         p[n >> 1][(n & 1) * 2] = ka_pack(w[0], w[1]);

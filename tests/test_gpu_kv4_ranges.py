@@ -91,3 +91,26 @@ def test_values_of_many_magnitudes(cuda_lib, dtype, D, Hkv, rep, rows_each, orde
         ks.append(rng.normal(0, 1, (n, Hkv, D))), vs.append(rng.normal(0, 1, (n, Hkv, D)) * 10.0 ** e[:, None, None])
     data = put(kv, ks, vs, dtype)
     compare(kv, data, rows(rng, 2 * rows_each, Hkv * rep, D, dtype, 1.5), [rows_each] * 2, dtype)
+
+
+@pytest.mark.parametrize("size", [1e4, 1e7, 1e9, 1e12, 1e20, 1e30, 1e35])
+@pytest.mark.parametrize("dtype,D,Hkv,rep,rows_each", SHAPES)
+def test_queries_of_any_size(cuda_lib, dtype, D, Hkv, rep, rows_each, size):
+    """Scores up to 1e37, one position far above the others: its value.  Its weight is rounded to fp16 alone and times the scale
+    (2^-11 each) in bf16 calls, and the result to bf16 (2^-8); fp32 calls hold 22 bits of both and add in fp32 (2^-20)."""
+    rng = np.random.default_rng(7)
+    kv = pool(dtype, D, Hkv, rep, rows_each)
+    b = np.sign(rng.normal(size=D))
+    ks, vs, at = [], [], (3, 77)
+    for n, w in zip((75, 333), at):
+        ks.append(rng.normal(0, 0.05, (n, Hkv, D))), vs.append(rng.normal(0, 1, (n, Hkv, D)))
+        ks[-1][w] = 2.0 * b
+    data = put(kv, ks, vs, dtype)
+    q = b * rng.uniform(0.5, 1.0, (2 * rows_each, Hkv * rep, D)) * size
+    q = torch.from_numpy(q.astype(np.float32)).cuda().to(DT[dtype])
+    out = num(kv.attention(0, q, None, ints([75 - rows_each, 333 - rows_each]), None if rows_each == 1 else starts_of([rows_each] * 2)))
+    for s in range(2):
+        want = np.repeat(data[s][1][at[s]], rep, axis=0)
+        err = np.abs(out[s * rows_each:(s + 1) * rows_each] - want)
+        assert (err <= (2.0 ** -20 if dtype == "f32" else 2 * 2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) * np.abs(want)).all(), err.max()
+    assert status() == 0
