@@ -43,6 +43,10 @@ struct Kv4View {
 
 int kv4_check(const bq_kv4_pool* p, const char* what);                     // kv4_pages.cu: 0, or BQ_ERR_* with the message set
 int kv4_view(const bq_kv4_pool* p, int layer, const char* what, Kv4View* out);
+// element addresses: a pointer that is not a multiple of its elements' size would fault on the device
+inline bool kv4_misaligned(size_t size, const void* a, const void* b = nullptr, const void* c = nullptr) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & (size - 1)) != 0;
+}
 
 #ifdef __CUDACC__
 // The kernels of the cache may start before the kernel that wrote their inputs has finished (pdl_wait orders them), so nothing

@@ -59,6 +59,7 @@ int bq_kv4_attention(const bq_kv4_pool* p, int layer, const void* q, int64_t ldq
     return fail(BQ_ERR_ARG, "bq_kv4_attention: bad number of rows (one per sequence without row ranges)");
   if (B == 0 || n_rows == 0) return BQ_OK;
   if (!q || !out || !pos || !work) return fail(BQ_ERR_ARG, "bq_kv4_attention: null pointer");
+  if (kv4_misaligned(4, slots, starts, pos)) return fail(BQ_ERR_ARG, "bq_kv4_attention: slots, pos and starts must be aligned to their elements");
   const uintptr_t pair = dtype == BQ_DT_F32 ? 7 : 3;
   if (ldq < (int64_t)Hq * p->head_dim || (ldq & 1) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & pair) ||
       (reinterpret_cast<uintptr_t>(work) & 15))

@@ -395,6 +395,7 @@ int kv4_check(const bq_kv4_pool* p, const char* what) {
   if (!p->pages || !p->tables || !p->lens || !p->refs || !p->work) return fail(BQ_ERR_ARG, w + ": null pointer in the pool");
   if ((reinterpret_cast<uintptr_t>(p->pages) | reinterpret_cast<uintptr_t>(p->refs) | reinterpret_cast<uintptr_t>(p->work)) & 15)
     return fail(BQ_ERR_ARG, w + ": pages, refs and work must be 16-byte aligned");
+  if (kv4_misaligned(4, p->tables, p->lens)) return fail(BQ_ERR_ARG, w + ": tables and lens must be aligned to their elements");
   int cur = -1;
   BQ_CUDA(cudaGetDevice(&cur));
   if (cur != device_id()) return fail(BQ_ERR_STATE, w + ": the current device is not the one bq_init() selected");
@@ -445,6 +446,7 @@ int bq_kv4_extend(const bq_kv4_pool* p, const int32_t* slots, const int32_t* sta
   if (B < 0 || B > p->max_seqs) return fail(BQ_ERR_ARG, "bq_kv4_extend: more sequences than the pool holds");
   if (B == 0) return BQ_OK;
   if (!pos_out) return fail(BQ_ERR_ARG, "bq_kv4_extend: null pointer");
+  if (kv4_misaligned(4, slots, starts, pos_out)) return fail(BQ_ERR_ARG, "bq_kv4_extend: slots, starts and pos_out must be aligned to their elements");
   cudaStream_t s = (cudaStream_t)stream;
   const int64_t bytes = kv4_page_bytes(p);
   BQ_CUDA(launch_chain(kv4_extend_kernel, dim3(1), dim3(KP_THREADS), (size_t)p->max_seqs * sizeof(int), s, 1, kp_pool(p), slots, starts, (int)B,
@@ -462,6 +464,7 @@ int bq_kv4_fork(const bq_kv4_pool* p, const int32_t* src, const int32_t* dst, in
   if (n < 0 || n > p->max_seqs) return fail(BQ_ERR_ARG, "bq_kv4_fork: more pairs than the pool holds sequences");
   if (n == 0) return BQ_OK;
   if (!src || !dst) return fail(BQ_ERR_ARG, "bq_kv4_fork: null pointer");
+  if (kv4_misaligned(4, src, dst)) return fail(BQ_ERR_ARG, "bq_kv4_fork: src and dst must be aligned to their elements");
   cudaStream_t s = (cudaStream_t)stream;
   if (n <= KF_PAIRS && n * p->max_pages <= KF_ONE) {
     BQ_CUDA(launch_chain(kv4_fork_kernel, dim3(1), dim3(KP_THREADS), 0, s, 1, kp_pool(p), src, dst, (int)n, status_word()));
@@ -482,6 +485,7 @@ int bq_kv4_free(const bq_kv4_pool* p, const int32_t* slots, int64_t n, void* str
   if (n < 0 || n > p->max_seqs) return fail(BQ_ERR_ARG, "bq_kv4_free: more slots than the pool holds sequences");
   if (n == 0) return BQ_OK;
   if (!slots) return fail(BQ_ERR_ARG, "bq_kv4_free: null pointer");
+  if (kv4_misaligned(4, slots)) return fail(BQ_ERR_ARG, "bq_kv4_free: slots must be aligned to its elements");
   BQ_CUDA(launch_chain(kv4_free_kernel, dim3((unsigned)n), dim3(KF_THREADS), 0, (cudaStream_t)stream, 1, kp_pool(p), slots, status_word()));
   count_launch();
   BQ_CUDA(cudaGetLastError());

@@ -253,13 +253,15 @@ __global__ void __launch_bounds__(KR_THREADS) kv4_gather_kernel(Kv4View v, T* k,
 
 // work items that cover every block which n_rows rows of B sequences can touch (kv4_item_base)
 static int64_t kr_items(int64_t B, int64_t n_rows, bool ragged) { return ragged ? (n_rows >> 4) + 2 * B : B; }
-static int kr_check(const bq_kv4_pool* p, int64_t B, int64_t n_rows, const int32_t* starts, const int32_t* pos, int dtype, const char* what) {
+static int kr_check(const bq_kv4_pool* p, int64_t B, int64_t n_rows, const int32_t* slots, const int32_t* starts, const int32_t* pos, int dtype,
+                    const char* what) {
   const std::string w(what);
   if (dtype != BQ_DT_F32 && dtype != BQ_DT_BF16) return fail(BQ_ERR_ARG, w + ": dtype must be BQ_DT_F32 or BQ_DT_BF16");
   if (B < 0 || B > p->max_seqs) return fail(BQ_ERR_ARG, w + ": more sequences than the pool holds");
   if (n_rows < 0 || n_rows > (int64_t)1 << 30 || (!starts && n_rows != B))
     return fail(BQ_ERR_ARG, w + ": bad number of rows (one per sequence without row ranges)");
   if (B && !pos) return fail(BQ_ERR_ARG, w + ": null pointer");
+  if (kv4_misaligned(4, slots, starts, pos)) return fail(BQ_ERR_ARG, w + ": slots, pos and starts must be aligned to their elements");
   return BQ_OK;
 }
 
@@ -273,7 +275,7 @@ int bq_kv4_append(const bq_kv4_pool* p, int layer, const void* k, const void* v,
                   const int32_t* pos, const int32_t* starts, int64_t B, int64_t n_rows, void* stream) {
   Kv4View view;
   int rc = kv4_view(p, layer, "bq_kv4_append", &view);
-  if (rc || (rc = kr_check(p, B, n_rows, starts, pos, dtype, "bq_kv4_append"))) return rc;
+  if (rc || (rc = kr_check(p, B, n_rows, slots, starts, pos, dtype, "bq_kv4_append"))) return rc;
   if (B == 0 || n_rows == 0) return BQ_OK;
   if (!k || !v) return fail(BQ_ERR_ARG, "bq_kv4_append: null pointer");
   const int64_t row = (int64_t)p->kv_heads * p->head_dim;
@@ -298,10 +300,13 @@ int bq_kv4_rope_append(const bq_kv4_pool* p, int layer, const float* qkv, void* 
                        const int32_t* pos, const int32_t* starts, int64_t B, int64_t n_rows, void* stream) {
   Kv4View view;
   int rc = kv4_view(p, layer, "bq_kv4_rope_append", &view);
-  if (rc || (rc = kr_check(p, B, n_rows, starts, pos, dtype, "bq_kv4_rope_append"))) return rc;
-  if (Hq <= 0 || Hq % p->kv_heads) return fail(BQ_ERR_ARG, "bq_kv4_rope_append: query heads must be a multiple of the KV heads");
+  if (rc || (rc = kr_check(p, B, n_rows, slots, starts, pos, dtype, "bq_kv4_rope_append"))) return rc;
+  if (Hq <= 0 || Hq > 65536 || Hq % p->kv_heads)
+    return fail(BQ_ERR_ARG, "bq_kv4_rope_append: query heads must be a multiple of the KV heads, 65536 at most");
   if (B == 0 || n_rows == 0) return BQ_OK;
   if (!qkv || !q_out) return fail(BQ_ERR_ARG, "bq_kv4_rope_append: null pointer");
+  if (kv4_misaligned(4, qkv) || kv4_misaligned(dtype == BQ_DT_F32 ? 4 : 2, q_out))
+    return fail(BQ_ERR_ARG, "bq_kv4_rope_append: qkv and q_out must be aligned to their elements");
   const dim3 grid((unsigned)kr_items(B, n_rows, starts != nullptr), (unsigned)((2 * p->kv_heads + Hq + KR_TASKS - 1) / KR_TASKS));
   const size_t smem = (size_t)KV4_ROWS * p->head_dim * sizeof(float);
   cudaStream_t s = (cudaStream_t)stream;
@@ -320,9 +325,10 @@ int bq_kv4_gather(const bq_kv4_pool* p, int layer, void* k, void* v, int dtype, 
                   int64_t B, int64_t n_rows, void* stream) {
   Kv4View view;
   int rc = kv4_view(p, layer, "bq_kv4_gather", &view);
-  if (rc || (rc = kr_check(p, B, n_rows, starts, pos, dtype, "bq_kv4_gather"))) return rc;
+  if (rc || (rc = kr_check(p, B, n_rows, slots, starts, pos, dtype, "bq_kv4_gather"))) return rc;
   if (B == 0 || n_rows == 0) return BQ_OK;
   if (!k || !v) return fail(BQ_ERR_ARG, "bq_kv4_gather: null pointer");
+  if (kv4_misaligned(dtype == BQ_DT_F32 ? 4 : 2, k, v)) return fail(BQ_ERR_ARG, "bq_kv4_gather: k and v must be aligned to their elements");
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
   const dim3 grid((unsigned)kr_items(B, n_rows, starts != nullptr), (unsigned)((2 * p->kv_heads + KR_TASKS - 1) / KR_TASKS));
   cudaStream_t s = (cudaStream_t)stream;

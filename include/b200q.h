@@ -344,7 +344,7 @@ int bq_ep_combine(bq_ep_t ep, const float* out_rows, const int32_t* inv, const f
  * the low or high nibble (by e again) of byte G * 256 + ((e % 8) * 4 + r % 8 / 2) * 8 + 4 i + r / 8 + 2 * (r % 2); scale of K
  * number r * head_dim / 32 + G, of V number G * 16 + r % 8 / 2 * 4 + r / 8 * 2 + r % 2.
  * Limits: head_dim a multiple of 32 up to 256, page a power of two from 16 to 4096, max_seqs <= 8192, max_pages * page
- * <= 2^30, n_pages < 2^30; pages, refs and work 16-byte aligned.  The CUDA device must be the one bq_init() selected.  */
+ * <= 2^30, n_pages < 2^30; pages, refs and work 16-byte aligned, all else aligned to its elements.  The CUDA device must be the one bq_init() selected.  */
 typedef struct {
   void* pages;         /* n_pages * bq_kv4_page_bytes() bytes                                                       */
   int32_t* tables;     /* [max_seqs][max_pages] page numbers, -1 behind a sequence's last page                      */
