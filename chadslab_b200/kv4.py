@@ -199,12 +199,14 @@ class PagedKV4:
                                                 _DT[q_out.dtype], at_slots, at_pos, at_starts, B, qkv.shape[0], self._stream()))
         return q_out
 
-    def gather(self, layer: int, slots, pos, starts=None, rows: int = 0, dtype=torch.float32):
+    def gather(self, layer: int, slots, pos, starts=None, rows: int | None = None, dtype=torch.float32):
         """What the pages hold (code * scale) of the positions that the rows stand for -> k, v [n_rows, kv_heads, head_dim];
-        `rows` gives n_rows where `starts` is given.  Rows of refused sequences, or of none, are left as allocated."""
+        where `starts` is given, `rows` has to say how many they are (it is on the device).  Rows of refused sequences, or of none, are left as allocated."""
         keep, at_slots, at_pos, at_starts, B = self._batch(slots, pos, starts)
         if dtype not in _DT:
             raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+        if starts is not None and rows is None:
+            raise ValueError("gather with starts needs rows, the number of rows they stand for")
         n_rows = int(rows) if starts is not None else B
         shape = (n_rows, self.kv_heads, self.head_dim)
         k, v = self.lens.new_empty(shape, dtype=dtype), self.lens.new_empty(shape, dtype=dtype)

@@ -1,5 +1,36 @@
-"""Paged 4-bit KV cache without a GPU: what the restated pool serves."""
+"""Paged 4-bit KV cache without a GPU: what the restated pool serves, and what the Python surface does before it calls."""
+import pytest
+import torch
+
 from oracle import kv4 as okv
+
+
+class Recorder:
+    """In place of the library: every call succeeds and is kept."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+def surface(seqs=4):
+    """A PagedKV4 whose tensors lie on the CPU and whose calls go to a Recorder."""
+    from chadslab_b200 import PagedKV4
+    kv = object.__new__(PagedKV4)
+    kv.layers, kv.kv_heads, kv.head_dim, kv.page, kv.n_pages, kv.max_seqs, kv.max_pages = 1, 2, 64, 16, 8, seqs, 4
+    kv.device, kv._index, kv._lib, kv._pool, kv._p, kv._attn_ints = torch.device("cpu"), 0, Recorder(), None, None, {}
+    kv.lens, kv.refs = torch.zeros(seqs, dtype=torch.int32), torch.zeros(8, dtype=torch.int32)
+    kv._stream = lambda: 0
+    return kv
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
 
 
 def test_restated_pool_serves_whoever_fits():
@@ -10,3 +41,14 @@ def test_restated_pool_serves_whoever_fits():
     p.free([1])
     # page 0 is not shared any more; the copy of page 4 that sequences 2 and 3 want does not exist
     assert p.extend([0, 2, 3], [3, 1, 4]) == ([1, -1, -1], [])
+
+
+def test_gather_of_ranges_needs_their_rows():
+    kv = surface()
+    with pytest.raises(ValueError):
+        kv.gather(0, i32(0, 1), i32(0, 0), i32(0, 3, 5))
+    assert not kv._lib.calls
+    k, v = kv.gather(0, i32(0, 1), i32(0, 0), i32(0, 3, 5), rows=5)
+    assert k.shape == v.shape == (5, 2, 64) and kv._lib.calls[-1][1][9] == 5
+    assert kv.gather(0, i32(0, 1), i32(0, 0), i32(0, 0, 0), rows=0)[0].shape == (0, 2, 64)
+    assert kv.gather(0, i32(0, 1), i32(0, 0))[0].shape == (2, 2, 64)
