@@ -137,13 +137,17 @@ class PagedKV4:
         return x, s0
 
     # ---- pages --------------------------------------------------------------------------------------------------------
-    def extend(self, slots=None, starts=None, batch: int = 0):
+    def extend(self, slots=None, starts=None, batch: int | None = None):
         """Room for every sequence's new rows (starts None: one each) -> pos int32 [B], the length before, -1 where fewer pages
-        were left than the sequence needs (later ones of the batch are served all the same).  `batch` gives B when both are None."""
+        were left than the sequence needs (later ones of the batch are served all the same).  `batch` has to give B when both are None."""
+        if slots is None and starts is None and batch is None:
+            raise ValueError("extend needs slots, starts or batch")
         if slots is not None:
             slots = self._ints(slots, "slots")
         if starts is not None:
             starts = self._ints(starts, "starts")
+            if starts.numel() == 0:
+                raise ValueError("starts must have one entry more than there are sequences")
         B = slots.numel() if slots is not None else starts.numel() - 1 if starts is not None else int(batch)
         if starts is not None and starts.numel() != B + 1:
             raise ValueError(f"starts must have one entry more than slots ({B}), got {starts.numel()}")

@@ -52,3 +52,14 @@ def test_gather_of_ranges_needs_their_rows():
     assert k.shape == v.shape == (5, 2, 64) and kv._lib.calls[-1][1][9] == 5
     assert kv.gather(0, i32(0, 1), i32(0, 0), i32(0, 0, 0), rows=0)[0].shape == (0, 2, 64)
     assert kv.gather(0, i32(0, 1), i32(0, 0))[0].shape == (2, 2, 64)
+
+
+def test_extend_needs_to_know_the_batch():
+    kv = surface()
+    with pytest.raises(ValueError):
+        kv.extend()
+    with pytest.raises(ValueError):
+        kv.extend(None, i32())
+    assert not kv._lib.calls
+    assert kv.extend(batch=3).shape == (3,) and kv.extend(i32(1, 2)).shape == (2,) and kv.extend(None, i32(0, 4)).shape == (1,)
+    assert [c[1][3] for c in kv._lib.calls] == [3, 2, 1] and kv.extend(batch=0).shape == (0,)
