@@ -9,9 +9,10 @@
 
 Token rows are [n_rows, heads, head_dim]; `starts` (int32 [B + 1]) gives the rows of every sequence of the batch, None means
 one row per sequence.  `slots` (int32 [B], None: 0 .. B-1) are rows of the page table, `pos` (int32 [B]) the position of every
-sequence's first row, as `extend` returns it (-1: refused, no pages left).  All three are CUDA tensors, or sequences of ints that
-are copied to the device.  Nothing here waits for the GPU; every call can be captured in a graph.  Calls that change a pool
-are to be ordered on the device, like the library's other calls.
+sequence's first row, as `extend` returns it (-1: refused, no pages left).  All three are CUDA tensors, or sequences of ints, which
+are copied to the device.  Nothing here waits for the GPU.  Calls whose arguments are tensors can be captured in a graph; a
+sequence of ints is refused during capture, since a replay would read host memory that is gone.  Calls that change a pool are to
+be ordered on the device, like the library's other calls; compact counts as one for both pools.
 """
 from __future__ import annotations
 
@@ -87,7 +88,11 @@ class PagedKV4:
     def _ints(self, t, what: str):
         """-> int32 CUDA tensor on the pool's device (a sequence of ints is copied there)."""
         if not isinstance(t, torch.Tensor):
-            return torch.tensor(t, dtype=torch.int32).to(self.device)
+            if self.device.type != "cuda":
+                return torch.tensor(t, dtype=torch.int32)
+            if torch.cuda.is_current_stream_capturing():
+                raise BqError(_lib.ERR_STATE, f"{what} must be an int32 tensor on {self.device} during stream capture")
+            return torch.tensor(t, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True)      # the host does not wait
         if t.dtype is not torch.int32 or t.device != self.device or t.dim() != 1:
             raise BqError(_lib.ERR_ARG, f"{what} must be a 1-D int32 tensor on {self.device}")
         return t if t.is_contiguous() else t.contiguous()

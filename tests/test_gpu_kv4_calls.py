@@ -35,3 +35,45 @@ def test_addresses_between_elements_are_refused(cuda_lib):
         bad.append(lib.bq_kv4_free(C.byref(q), i, 1, s))
     assert bad == [-1] * len(bad) and lib.bq_launch_count() == n0
     assert status() == 0
+
+
+def test_ints_do_not_make_the_host_wait(cuda_lib):
+    kv = make(1, 2, 64, max_seqs=4)
+    q = torch.zeros((1, 2, 64), device="cuda")
+    calls = [lambda: kv.extend([0], [0, 1]), lambda: kv.attention(0, q, [0], [0]), lambda: kv.append(0, q, q, [0], [0]), lambda: kv.gather(0, [0], [0]),
+             lambda: kv.fork([0], range(1, 2)), lambda: kv.free([1])]
+    for call in calls * 2:                                   # the allocators have seen these sizes
+        call()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)                           # about 0.2 s of the stream
+    done = torch.cuda.Event()
+    done.record()
+    for call in calls:
+        call()
+    assert not done.query()
+    torch.cuda.synchronize()
+    assert kv.lens.tolist() == [3, 0, 0, 0] and status() == 0
+
+
+def test_ints_are_refused_during_capture(cuda_lib):
+    """... before anything is issued: the capture goes on and the graph replays."""
+    import chadslab_b200 as cb
+    kv = make(1, 2, 64, max_seqs=4)
+    q, slots, starts = torch.ones((1, 2, 64), device="cuda"), ints([1]), ints([0, 1])
+    at = kv.extend(slots)
+    kv.append(0, q, q, slots, at)
+    kv.attention(0, q, slots, at)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: kv.extend([1]), lambda: kv.extend(slots, [0, 1]), lambda: kv.attention(0, q, [1], at), lambda: kv.attention(0, q, slots, [0]),
+                     lambda: kv.append(0, q, q, slots, at, [0, 1]), lambda: kv.free(range(1)), lambda: kv.fork([1], slots)):
+            with pytest.raises(cb.BqError):
+                call()
+        at = kv.extend(slots, starts)
+        kv.append(0, q, q, slots, at, starts)
+        out = kv.attention(0, q, slots, at, starts)
+    for _ in range(3):
+        graph.replay()
+    assert kv.lens.tolist() == [0, 4, 0, 0] and at.tolist() == [3] and status() == 0
+    assert np.allclose(num(out), okv.held(np.ones((1, 2, 64), np.float32)), rtol=1e-5)
