@@ -240,6 +240,8 @@ class PagedKV4:
         sizes = (heads, dt, B, q.shape[0])
         need = self._attn_ints.get(sizes)
         if need is None:
+            if len(self._attn_ints) >= 256:              # a server's chunks come in any size
+                self._attn_ints.clear()
             need = self._attn_ints[sizes] = int(self._lib.bq_kv4_attention_work_bytes(self._p, *sizes)) // 4
         work = self.refs.new_empty(need)                       # of this call alone: calls may overlap
         _lib.check(self._lib.bq_kv4_attention(self._p, int(layer), q.data_ptr(), ldq, out.data_ptr(), heads, dt, at_slots, at_pos, at_starts, B,

@@ -63,3 +63,14 @@ def test_extend_needs_to_know_the_batch():
     assert not kv._lib.calls
     assert kv.extend(batch=3).shape == (3,) and kv.extend(i32(1, 2)).shape == (2,) and kv.extend(None, i32(0, 4)).shape == (1,)
     assert [c[1][3] for c in kv._lib.calls] == [3, 2, 1] and kv.extend(batch=0).shape == (0,)
+
+
+def test_scratch_sizes_do_not_pile_up():
+    kv = surface()
+    for n in range(2000):
+        kv.attention(0, torch.zeros((n, 2, 64)), i32(0), i32(0), i32(0, n))
+    assert len(kv._attn_ints) <= 256 and sum(name == "bq_kv4_attention" for name, _ in kv._lib.calls) == 2000
+    kv._lib.calls.clear()
+    for _ in range(10):                                      # a size that repeats is asked for once
+        kv.attention(0, torch.zeros((7, 2, 64)), i32(0), i32(0), i32(0, 7))
+    assert sum(name == "bq_kv4_attention_work_bytes" for name, _ in kv._lib.calls) <= 1
