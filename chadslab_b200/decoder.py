@@ -86,11 +86,13 @@ class QuantDecoder:
             raise ValueError(f"kv_bits={kv_bits}: the cache is held in the activation type (0) or in 4 bits (4)")
         c, dev = self.cfg, self.embed.device
         self.max_batch, self.max_seq, self.pos, self.kv = max_batch, max_seq, 0, None
+        self._lens, self._lens_of = [], None           # lengths of the paged cache's sequences, as of kv.changes == _lens_of
         if kv_bits == 4:
             per_seq = -(-max_seq // kv_page)
             # one page more per sequence: a shared last page is copied by all that share it before it is given up
             self.kv = PagedKV4(c.layers, self.kv_local, c.head_dim, n_pages=max_batch * (per_seq + 1), max_seqs=max_batch, max_pages=per_seq,
                                page=kv_page, device=dev)
+            self._lens, self._lens_of = [0] * max_batch, self.kv.changes
             return
         self.k_cache = [torch.zeros((max_batch, max_seq, self.kv_local, c.head_dim), dtype=self.act_dtype, device=dev)
                         for _ in range(c.layers)]
@@ -170,6 +172,7 @@ class QuantDecoder:
         self.pos = 0
         if self.kv is not None:
             self.kv.free(range(self.max_batch))
+            self._lens, self._lens_of = [0] * self.max_batch, self.kv.changes
 
     def share_prefix(self, batch: int):
         """After a prompt run alone (batch 1): sequences 0 .. batch-1 all continue it.  They share its pages until they write."""
@@ -178,7 +181,10 @@ class QuantDecoder:
         if not 1 <= batch <= self.max_batch:
             raise ValueError(f"the cache holds {self.max_batch} sequences, asked for {batch}")
         if batch > 1:
+            known = self._lens_of == self.kv.changes
             self.kv.fork([0] * (batch - 1), range(1, batch))
+            if known:
+                self._lens[1:batch], self._lens_of = [self._lens[0]] * (batch - 1), self.kv.changes
 
     def _cached_attention(self, l, q, k, v, rows, b0: int = 0):
         """Appends k, v [B, T, heads, d] at self.pos of sequences b0 .. b0+B-1 of layer l and attends q to them and everything
@@ -205,9 +211,17 @@ class QuantDecoder:
         return o.transpose(1, 2)
 
     def _new_rows(self, B: int, T: int, b0: int = 0):
-        """Room for T more rows of sequences b0 .. b0+B-1 of the paged cache -> (slots, pos, starts)."""
+        """Room for T more rows of sequences b0 .. b0+B-1 of the paged cache -> (slots, pos, starts).  The cache puts them behind
+        what each sequence holds, the rotation at self.pos: they have to agree."""
         if self.kv is None:
             return None
+        if self._lens_of != self.kv.changes:           # changed by other hands, or by a captured step: ask the device
+            self._lens, self._lens_of = self.kv.lens.tolist(), self.kv.changes
+        if any(n != self.pos for n in self._lens[b0:b0 + B]):
+            raise ValueError(f"sequences {b0}..{b0 + B - 1} hold {self._lens[b0:b0 + B]} positions, the pass is at position {self.pos}: "
+                             "reset(), or share_prefix(), first")
+        self._lens[b0:b0 + B] = [self.pos + T] * B
+        self._lens_of += 1                             # the extend below
         slots = torch.arange(b0, b0 + B, dtype=torch.int32, device=self.embed.device)
         starts = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device=self.embed.device)
         return slots, self.kv.extend(slots, starts), starts
@@ -389,6 +403,7 @@ class QuantDecoder:
                 raise ValueError(f"KV cache is full ({S} positions): the next token has no row to be written to")
             graph.replay()
             self.pos += 1
+            self._lens_of = None
         return step, tokens
 
     def linear_bytes_per_token(self) -> float:

@@ -82,6 +82,7 @@ class PagedKV4:
         self._work = torch.empty(int(lib.bq_kv4_work_bytes(self._p)) // 4, dtype=torch.int32, device=device)
         p = self._pool
         p.pages, p.tables, p.lens, p.refs, p.work = (t.data_ptr() for t in (pages, tables, lens, refs, self._work))
+        self.changes = 0                     # calls that may have changed the sequences, replays of captured ones apart
         self._attn_ints = {}                 # scratch of an attention call by (heads, dtype, sequences, rows)
 
     # ---- arguments --------------------------------------------------------------------------------------------------
@@ -156,6 +157,7 @@ class PagedKV4:
         B = slots.numel() if slots is not None else starts.numel() - 1 if starts is not None else int(batch)
         if starts is not None and starts.numel() != B + 1:
             raise ValueError(f"starts must have one entry more than slots ({B}), got {starts.numel()}")
+        self.changes += 1
         pos = self.lens.new_empty(B)
         _lib.check(self._lib.bq_kv4_extend(self._p, self._ptr(slots), self._ptr(starts), B, pos.data_ptr(), self._stream()))
         return pos
@@ -165,17 +167,20 @@ class PagedKV4:
         src, dst = self._ints(src, "src"), self._ints(dst, "dst")
         if src.numel() != dst.numel():
             raise ValueError(f"{src.numel()} sources for {dst.numel()} destinations")
+        self.changes += 1
         _lib.check(self._lib.bq_kv4_fork(self._p, src.data_ptr(), dst.data_ptr(), src.numel(), self._stream()))
 
     def free(self, slots) -> None:
         """Empties sequences; pages that no other sequence holds become free."""
         slots = self._ints(slots, "slots")
+        self.changes += 1
         _lib.check(self._lib.bq_kv4_free(self._p, slots.data_ptr(), slots.numel(), self._stream()))
 
     def compact(self, to: "PagedKV4") -> "PagedKV4":
         """Moves a copy of all live pages, in ascending order, and the sequences into pool `to`; returns it."""
         if to.device != self.device:
             raise BqError(_lib.ERR_ARG, f"both pools must be on {self.device}")
+        to.changes += 1
         _lib.check(self._lib.bq_kv4_compact(self._p, to._p, self._stream()))
         return to
 

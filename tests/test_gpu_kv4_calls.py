@@ -77,3 +77,52 @@ def test_ints_are_refused_during_capture(cuda_lib):
         graph.replay()
     assert kv.lens.tolist() == [0, 4, 0, 0] and at.tolist() == [3] and status() == 0
     assert np.allclose(num(out), okv.held(np.ones((1, 2, 64), np.float32)), rtol=1e-5)
+
+
+def test_decoder_refuses_positions_that_the_pages_do_not_have(cuda_lib):
+    """Rows go behind what a sequence holds; a pass at another position would rotate them wrongly without a word."""
+    from chadslab_b200.decoder import DecoderConfig, MoEDecoder, QuantDecoder
+    from oracle import model as omodel
+    from test_gpu_decoder_kv4 import MOE_SMALL, SMALL
+    cfg = dict(SMALL, fmt=1)
+    w = omodel.random_weights(cfg, seed=5)
+    dec = QuantDecoder.from_numpy(DecoderConfig(**cfg), w, act_dtype=torch.float32, max_seq=48, max_batch=3, kv_bits=4, kv_page=16)
+    prompt = torch.from_numpy(np.random.default_rng(1).integers(0, cfg["vocab"], (3, 9))).cuda()
+
+    def refused(tokens):
+        before = [t.clone() for t in (dec.kv.lens, dec.kv.refs, dec.kv.tables, dec.kv.pages)]
+        with pytest.raises(ValueError):
+            dec.hidden_states(tokens)
+        assert all(torch.equal(a, b) for a, b in zip(before, (dec.kv.lens, dec.kv.refs, dec.kv.tables, dec.kv.pages)))
+
+    dec.hidden_states(prompt[:1])
+    refused(prompt)                                          # sequences 1 and 2 are empty
+    dec.share_prefix(3)
+    want = dec.logits(prompt[:, :2])
+    dec.pos -= 1                                             # a position once more
+    refused(prompt[:, :1])
+    dec.pos += 1
+    dec.hidden_states(prompt[:2, :1])
+    refused(prompt[:, :1])                                   # sequence 2 stayed behind
+    dec.kv.free([1])
+    refused(prompt[:2, :1])                                  # gone behind the decoder's back
+    dec.reset()
+    dec.hidden_states(prompt[:1])
+    dec.share_prefix(3)
+    assert torch.equal(dec.logits(prompt[:, :2]), want)
+    # a captured step moves the sequences on, and eager passes go on from there
+    eager = dec.next_tokens(prompt[:, 2:3])
+    dec.reset()
+    dec.hidden_states(prompt[:, :5])
+    step, tokens = dec.make_graph_stepper(3, prompt[:, 5], start_pos=5)
+    step()
+    step()
+    assert dec.logits(tokens[:, None]).shape[0] == 3 and dec.kv.lens.tolist() == [8] * 3 and eager.shape == (3,)
+    refused(torch.zeros((3, 48), dtype=torch.int64, device="cuda"))
+    moe = MoEDecoder.from_numpy(DecoderConfig(**MOE_SMALL), omodel.random_weights(MOE_SMALL, seed=11), act_dtype=torch.float32, max_seq=32, max_batch=2,
+                                kv_bits=4, kv_page=16)
+    moe.prefill(prompt[:2, :5] % MOE_SMALL["vocab"], 1)
+    moe.pos = 3
+    with pytest.raises(ValueError):
+        moe.hidden_states(prompt[:2, :1] % MOE_SMALL["vocab"])
+    assert status() == 0

@@ -24,6 +24,7 @@ def surface(seqs=4):
     kv = object.__new__(PagedKV4)
     kv.layers, kv.kv_heads, kv.head_dim, kv.page, kv.n_pages, kv.max_seqs, kv.max_pages = 1, 2, 64, 16, 8, seqs, 4
     kv.device, kv._index, kv._lib, kv._pool, kv._p, kv._attn_ints = torch.device("cpu"), 0, Recorder(), None, None, {}
+    kv.changes = 0
     kv.lens, kv.refs = torch.zeros(seqs, dtype=torch.int32), torch.zeros(8, dtype=torch.int32)
     kv._stream = lambda: 0
     return kv
