@@ -177,7 +177,9 @@ class PagedKV4:
         _lib.check(self._lib.bq_kv4_free(self._p, slots.data_ptr(), slots.numel(), self._stream()))
 
     def compact(self, to: "PagedKV4") -> "PagedKV4":
-        """Moves a copy of all live pages, in ascending order, and the sequences into pool `to`; returns it."""
+        """Moves a copy of all live pages, in ascending order, and the sequences into pool `to`; returns it.  How many pages are
+        live is known on the device alone: if `to` has fewer, it stays as it was and BQ_ERR_STATE is recorded in the
+        status word (bq_status_poll)."""
         if to.device != self.device:
             raise BqError(_lib.ERR_ARG, f"both pools must be on {self.device}")
         to.changes += 1
@@ -197,8 +199,11 @@ class PagedKV4:
 
     def rope_append(self, layer: int, qkv, heads: int, rope_base: float, slots, pos, starts=None, q_out=None, dtype=torch.bfloat16):
         """qkv fp32 [n_rows, (heads + 2 kv_heads) head_dim] of a fused projection: rotates q and k by each row's position,
-        quantises k and v into the pages -> q [n_rows, heads, head_dim] in `dtype` (or q_out)."""
+        quantises k and v into the pages -> q [n_rows, heads, head_dim] in `dtype` (or q_out).  Rows of refused sequences, or
+        of none, are not written: as allocated, or as they were in q_out."""
         keep, at_slots, at_pos, at_starts, B = self._batch(slots, pos, starts)
+        if q_out is None and dtype not in _DT:
+            raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
         if not qkv.is_cuda or qkv.device != self.device or qkv.dtype != torch.float32 or not qkv.is_contiguous():
             raise BqError(_lib.ERR_ARG, f"qkv must be a contiguous fp32 tensor on {self.device}")
         width = (heads + 2 * self.kv_heads) * self.head_dim

@@ -75,3 +75,10 @@ def test_scratch_sizes_do_not_pile_up():
     for _ in range(10):                                      # a size that repeats is asked for once
         kv.attention(0, torch.zeros((7, 2, 64)), i32(0), i32(0), i32(0, 7))
     assert sum(name == "bq_kv4_attention_work_bytes" for name, _ in kv._lib.calls) <= 1
+
+
+def test_rope_append_names_a_type_it_does_not_have():
+    kv = surface()
+    with pytest.raises(TypeError):
+        kv.rope_append(0, torch.zeros((2, 8 * 64)), 4, 1e4, None, i32(0, 0), dtype=torch.float16)
+    assert not kv._lib.calls
