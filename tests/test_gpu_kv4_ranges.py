@@ -114,3 +114,32 @@ def test_queries_of_any_size(cuda_lib, dtype, D, Hkv, rep, rows_each, size):
         err = np.abs(out[s * rows_each:(s + 1) * rows_each] - want)
         assert (err <= (2.0 ** -20 if dtype == "f32" else 2 * 2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) * np.abs(want)).all(), err.max()
     assert status() == 0
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype,D,Hkv,rep,rows_each", SHAPES)
+def test_rows_that_are_not_finite_keep_to_themselves(cuda_lib, dtype, D, Hkv, rep, rows_each, bad):
+    """A query row with a NaN or an infinity gives NaN; every other row has the bits that it has without it.  A value that is NaN
+    shows in its group of 32 dimensions only, in the rows that see it."""
+    rng = np.random.default_rng(9)
+    kv = pool(dtype, D, Hkv, rep, rows_each)
+    ks, vs = ([rng.normal(0, 1, (n, Hkv, D)) for n in (75, 200)] for _ in range(2))
+    put(kv, ks, vs, dtype)
+    pos, starts = ints([75 - rows_each, 200 - rows_each]), None if rows_each == 1 else starts_of([rows_each] * 2)
+    q = rows(rng, 2 * rows_each, Hkv * rep, D, dtype)
+    ref = kv.attention(0, q, None, pos, starts)
+    hit, head = rows_each - 1, Hkv * rep - 1
+    broken = q.clone()
+    broken[hit, head, 5] = bad
+    out = kv.attention(0, broken, None, pos, starts)
+    keep = torch.ones(ref.shape[:2], dtype=torch.bool, device="cuda")
+    keep[hit, head] = False
+    assert torch.isnan(out[hit, head]).all() and torch.equal(out[keep], ref[keep]) and torch.isfinite(ref).all()
+    # sequence 0's last position: its value becomes NaN in one group of head 0
+    k, v = (torch.from_numpy(x[0][-1:].astype(np.float32)).cuda() for x in (ks, vs))
+    v[0, 0, 3] = float("nan")
+    kv.append(0, k.to(DT[dtype]), v.to(DT[dtype]), [0], [74])
+    out = kv.attention(0, q, None, pos, starts)
+    sees = torch.zeros_like(out, dtype=torch.bool)
+    sees[hit, :rep, :32] = True                              # only the last row of sequence 0 sees position 74
+    assert torch.isnan(out[sees]).all() and torch.isfinite(out[~sees]).all() and status() == 0
