@@ -270,11 +270,15 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
 
 // element d of a head taken from the fp32 projection output, rotated like rope_kv_append_kernel does
 template <typename T>
-__device__ __forceinline__ float rope_elem(const float* __restrict__ src, int d, int D, const float* cs, const float* sn, bool rotate) {
+__device__ __forceinline__ float rope_elem_of(const float* src, int d, int D, const float* cs, const float* sn, bool rotate) {
   if (!rotate) return to_float<T>(from_float<T>(src[d]));
   const int half = D / 2, j = d < half ? d : d - half;
   const float x1 = to_float<T>(from_float<T>(src[j])), x2 = to_float<T>(from_float<T>(src[j + half]));
   return to_float<T>(from_float<T>(d < half ? x1 * cs[j] - x2 * sn[j] : x2 * cs[j] + x1 * sn[j]));
+}
+template <typename T>
+__device__ __forceinline__ float rope_elem(const float* __restrict__ src, int d, int D, const float* cs, const float* sn, bool rotate) {
+  return rope_elem_of<T>(src, d, D, cs, sn, rotate);
 }
 
 // Exact integer-code -> fp32 conversions without the (slow) I2F pipe.

@@ -62,7 +62,7 @@ template <typename T> struct KrRope {
   bool rotate;
   __device__ __forceinline__ void eight(int r, int d, float* x) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = rope_elem<T>(base + r * ld, d + j, D, cs + r * (D / 2), sn + r * (D / 2), rotate);
+    for (int j = 0; j < 8; ++j) x[j] = rope_elem_of<T>(base + r * ld, d + j, D, cs + r * (D / 2), sn + r * (D / 2), rotate);
   }
 };
 
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(KR_THREADS) kv4_rope_append_kernel(Kv4View v, 
     for (int e = threadIdx.x & 63; e < (it.r_hi - it.r_lo) * D; e += 64) {
       const int r = it.r_lo + e / D, d = e % D;
       q_out[((int64_t)(it.first + r) * Hq + h) * D + d] =
-          from_float<T>(rope_elem<T>(rows + r * ld + (int64_t)h * D, d, D, cs + r * half, sn + r * half, true));
+          from_float<T>(rope_elem_of<T>(rows + r * ld + (int64_t)h * D, d, D, cs + r * half, sn + r * half, true));
     }
     return;
   }
