@@ -93,9 +93,9 @@ __device__ __forceinline__ int kv4_item_seq(const int32_t* starts, int B, int it
   return lo;
 }
 // scale and code of one group: scale = fp16(min(absmax * (1/7), 65504)), code = clip(rint(x / scale), +-7).  The weight
-// quantiser's rule but for two things: absmax is multiplied by the fp32 reciprocal of 7 (no division in the append path; the
-// fp16 scale differs from the quotient's in about one group of 10^4), and a NaN makes its whole group NaN instead of
-// vanishing in the maximum.
+// quantiser's rule but for two things: absmax is multiplied by the fp32 reciprocal of 7, and a NaN makes its whole group NaN
+// instead of vanishing in the maximum.  The reciprocal is what torch computes for a CUDA tensor divided by the number 7 (a
+// quotient would differ from it in the last bit of about one scale in 10^4): a cache written by torch code has the same bytes.
 __device__ __forceinline__ float kv4_absmax(float a, float b) {       // fmaxf that keeps NaN (bits of |x| order like |x|)
   const uint32_t x = __float_as_uint(a) & 0x7FFFFFFFu, y = __float_as_uint(b) & 0x7FFFFFFFu;
   return __uint_as_float(x > y ? x : y);

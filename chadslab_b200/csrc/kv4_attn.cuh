@@ -26,11 +26,13 @@
 // Softmax runs in the exp2 domain with a reference R per column that lags behind the maximum: weights are 2^(s - R), R = max -
 // A, and R moves only when a weight would exceed 2^(A + 4) (A = 11: weights up to 2^15, 2^-24 is the smallest fp16).  A
 // drops when weight * scale overflows, i.e. for values far above one.  Weights end at 2^(A + 4): where scores are so large that
-// fp32 has steps of 16 and more (2^27), R cannot be set closer to their maximum; it is rounded down.  As long as no value scale was above 1/16, the scales
-// of a step are raised in the stage by a power of two (ka_raise): the products would lose in fp16's subnormals what the weights
-// still hold.  What weights and products lose is then at most 2^-31.9 of the largest weight times the largest value
-// per position, however small the values are.  Looking at the first step's scales costs 1 to 2 % (64 x 2048 positions x 16
-// heads of 256: 101.5 -> 103.7 us, ragged batch 66.0 -> 67.1).
+// fp32 has steps of 16 and more (2^27), R cannot be set closer to their maximum; it is rounded down.
+//
+// Small values.  As long as no value scale was above 1/16, the scales of a step are raised in the stage by a power of two
+// (ka_raise): the products would lose in fp16's subnormals what the weights still hold.  What weights and products lose is
+// then at most 2^-31.9 of the largest weight times the largest value per position, however small the values are.  Looking at
+// the first step's scales costs 1 to 2 % (64 x 2048 positions x 16 heads of 256: 101.5 -> 103.7 us, ragged batch 66.0 -> 67.1),
+// raising those of every step a quarter (values around 0.01: 105 -> 131 us; 32 / 4 heads of 128 28 -> 32).
 //
 // Work.  The tiles (128 positions, or 64 where two steps of 32 per warp do not fit into shared memory) of all (sequence, KV
 // head, column tile) segments form one list that is cut into equal runs, one per team of four warps: ragged batches and few
@@ -42,8 +44,9 @@
 // repeated calls give the same bits.
 //
 // Measured (device time of graph replays; short loops, in long ones the power cap lowers the clock): 64 x 2048 positions x 16
-// heads of 256 101 us = 5.96 TB/s, ragged batch of 96 up to 8000 positions with 32 / 4 heads of 128 65 us = 3.5 TB/s, two
-// contexts of 131072 with the same heads 45 us = 3.4 TB/s (eight columns per position block: bound by its instructions).
+// heads of 256 105 us = 5.75 TB/s (calls in a loop of seconds 121), ragged batch of 96 up to 8000 positions with 32 / 4 heads
+// of 128 68.5 us = 3.3 TB/s, two contexts of 131072 with the same heads 46.4 us = 3.25 TB/s (eight columns per position block:
+// bound by its instructions, 342 per block).
 #pragma once
 #include "kv4.cuh"
 #include "kv4_ring.h"
@@ -382,7 +385,8 @@ template <typename T, int NG, int NC> struct KaCfg {
   static constexpr int OSTR = QG * 32 + 4;            // row pitch of the merge buffer: a quad's columns hit different banks
   // teams of an SM, by the registers that a thread needs: 8 NG accumulators, 4 NG of q, and with eight columns 4 NG more for
   // starts and weights.  One team more at the price of spills is slower: 32 / 4 heads of 128 take 79 us with four teams of
-  // 128 registers (200 bytes spilled) and 70 with three of 168 (ragged batch of 96)
+  // 128 registers (200 bytes spilled) and 70 with three of 168 (ragged batch of 96).  That was measured with eight columns; with
+  // two and four the same rule leaves 16 to 112 bytes spilled, which is not measured against fewer teams
   static constexpr int TEAMS = NG <= (NC == 8 ? 3 : 4) ? 4 : NG <= (NC == 8 ? 5 : 8) ? 3 : 2;
   static constexpr int FIXED = KA_WARPS * HC * OSTR * 4 + 2 * KA_WARPS * W * 4 + HC * 12 + (int)sizeof(KaScan) + 128;
   // a warp's step, one stage of its ring: two blocks if the ring then has two stages, else one
@@ -955,7 +959,7 @@ __global__ void __launch_bounds__((KaCfg<T, NG, NC>::TEAMS * KA_THREADS), 1) kv4
 
 // Segments that were cut, merged in run order.  grid: (runs, (row, head) pairs of a tile); a run that begins a segment and
 // does not finish it has left its place in `cut`, the others have nothing to do.  Few pieces: a warp per pair; many: a CTA per
-// pair, whose threads share the pieces (two contexts of 131072 positions have 73; one warp would read them one by one).
+// pair, whose threads share the pieces (two contexts of 131072 positions with 32 / 4 heads of 128 have 56; one warp would read them one by one).
 constexpr int KA_MERGE_THREADS = 256, KA_MAX_RUNS = 1024, KA_FEW = 4;
 template <typename T>
 __global__ void __launch_bounds__(KA_MERGE_THREADS) kv4_attention_merge_kernel(const __grid_constant__ KaArgs a) {

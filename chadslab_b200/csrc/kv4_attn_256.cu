@@ -1,5 +1,6 @@
 // Attention over the 4-bit KV cache, head_dim 256: the narrowest variant that holds a sequence's columns
-// (see kv4_attn.cuh); more than eight go eight at a time (sixteen per pass spilled: chunks of 512 rows took 333 us against 293).
+// (see kv4_attn.cuh); more than eight go eight at a time: sixteen per pass spilled (chunks of 512 rows, which kv4_chunk.cu has
+// taken since, 333 us against 293).
 #include "kv4_attn.cuh"
 
 namespace bq {

@@ -9,9 +9,10 @@
 //   * Codes stay whole numbers (exact in fp16).  A key group's scale multiplies its 32-dimension sum in fp32, a value's scale
 //     multiplies the weight, as in the decode kernel; so do the power-of-two scaling of q, the lagging softmax reference,
 //     the raising of small value scales and the list of tiles that is cut into equal runs (here one per SM) and merged.
-// Bound: shared memory.  Every 512-byte B fragment is read for two matrix instructions (a warp has 16 rows; 32 would need 256
-// accumulator registers at head_dim 256), which is 128 bytes per cycle and SM at the matrix pipe's full rate: 117 TFLOP/s at
-// 512 rows, 8 heads on one KV head of 256.  Unpacking the next tile while this one is multiplied (two buffers, half the tile
+// Bound: shared memory and its latency.  Every 512-byte B fragment is read for two matrix instructions (a warp has 16 rows; 32
+// would need 256 accumulator registers at head_dim 256), which is 128 bytes per cycle and SM at the matrix pipe's full rate:
+// 117 TFLOP/s at 512 rows, 8 heads on one KV head of 256; the shared-memory pipe is busy in 68 % of the cycles, the matrix pipe
+// in 38 %, with two warps per scheduler to cover the rest.  Unpacking the next tile while this one is multiplied (two buffers, half the tile
 // at head_dim 256) changed nothing at head_dim 128 (272 -> 270 us) and lost at 256 (132 -> 159 us).
 #include "kv4_attn.cuh"
 

@@ -359,7 +359,9 @@ int64_t bq_kv4_work_bytes(const bq_kv4_pool* p);
 /* Batch calls below take, in DEVICE memory: slots int32[B] (NULL: slot b), starts int32[B + 1], ascending (NULL: one row per
  * sequence): sequence b owns rows starts[b] .. starts[b + 1] - 1 of the n_rows token rows, and pos int32[B]: the position
  * of its first row.  Rows that belong to no sequence are neither read nor written.  A sequence with pos < 0 takes no part.
- * A slot, row range or position outside the pool records BQ_ERR_ARG in the status word and is treated like pos < 0.       */
+ * A slot, row range or position outside the pool records BQ_ERR_ARG in the status word and is treated like pos < 0.  So
+ * does a position inside the pool for which the table holds no page, for append, rope_append and gather, which leave it out;
+ * attention records it too, and what the rows that see it come out as is undefined.                                       */
 /* Makes room for each sequence's new rows: lens += rows, pages are given out lowest number first in batch order, and a
  * partly filled last page that other sequences hold too is replaced by a copy (every layer).  pos_out[b] = the length
  * before the call, or -1 if the sequence was refused and is unchanged: it needs more pages than those in front of it have left
@@ -374,7 +376,8 @@ int bq_kv4_fork(const bq_kv4_pool* p, const int32_t* src, const int32_t* dst, in
 int bq_kv4_free(const bq_kv4_pool* p, const int32_t* slots, int64_t n, void* stream);
 /* Fills pool `to` (same shape but for n_pages, its own memory) with the pages that are held, in ascending order from 0, and
  * with the tables, lengths and counts that go with them; `p` is unchanged, and so are the bytes of free pages of `to`.  If
- * `to` has too few pages BQ_ERR_STATE is recorded and `to` is unchanged.                                                 */
+ * `to` has too few pages BQ_ERR_STATE is recorded and `to` is unchanged.  The scratch of `p` is used: not at the same time
+ * as another extend, fork or compact of `p`.                                                                             */
 int bq_kv4_compact(const bq_kv4_pool* p, const bq_kv4_pool* to, void* stream);
 /* Quantises rows k, v (n_rows rows of kv_heads * head_dim elements, ldk / ldv elements apart; fastest when every row is
  * 16-byte aligned) into the pages of `layer`: scale = fp16(min(absmax * fp32(1/7), 65504)), code = clip(rint(x / scale), +-7)
@@ -392,7 +395,8 @@ int bq_kv4_gather(const bq_kv4_pool* p, int layer, void* k, void* v, int dtype, 
                   const int32_t* starts, int64_t B, int64_t n_rows, void* stream);
 /* out[n_rows, Hq, head_dim] = softmax(q . K^T / sqrt(head_dim)) . V over positions 0 .. own position of every row
  * (causal), grouped-query heads.  Rows of q are ldq elements apart (even; q and out
- * aligned to two elements).  Rows of a sequence with pos < 0 are set to zero.
+ * aligned to two elements).  Rows of a sequence with pos < 0 are set to zero.  A copy that does not arrive within two seconds
+ * records BQ_ERR_TIMEOUT, a call of more than 2^31 tiles of positions BQ_ERR_UNSUPPORTED; out is then undefined.
  * work: bq_kv4_attention_work_bytes() of device scratch for a call of these sizes, 16-byte aligned, contents do not
  * matter; calls that may overlap on the device need scratch of their own.                                                */
 int64_t bq_kv4_attention_work_bytes(const bq_kv4_pool* p, int Hq, int dtype, int64_t B, int64_t n_rows);
