@@ -42,7 +42,8 @@ def test_ints_do_not_make_the_host_wait(cuda_lib):
     q = torch.zeros((1, 2, 64), device="cuda")
     calls = [lambda: kv.extend([0], [0, 1]), lambda: kv.attention(0, q, [0], [0]), lambda: kv.append(0, q, q, [0], [0]), lambda: kv.gather(0, [0], [0]),
              lambda: kv.fork([0], range(1, 2)), lambda: kv.free([1])]
-    for call in calls * 2:                                   # the allocators have seen these sizes
+    torch.cuda._sleep(20_000_000)
+    for call in calls * 2:                                   # the allocators have seen these sizes, this many at a time
         call()
     torch.cuda.synchronize()
     torch.cuda._sleep(400_000_000)                           # about 0.2 s of the stream

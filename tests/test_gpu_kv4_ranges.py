@@ -143,3 +143,30 @@ def test_rows_that_are_not_finite_keep_to_themselves(cuda_lib, dtype, D, Hkv, re
     sees = torch.zeros_like(out, dtype=torch.bool)
     sees[hit, :rep, :32] = True                              # only the last row of sequence 0 sees position 74
     assert torch.isnan(out[sees]).all() and torch.isfinite(out[~sees]).all() and status() == 0
+
+
+@pytest.mark.parametrize("dtype,D,Hkv,rep,rows_each", SHAPES)
+def test_bytes_behind_small_values_do_not_matter(cuda_lib, dtype, D, Hkv, rep, rows_each):
+    """The rest of a last block can hold anything, also where the scales in front of it are raised."""
+    got = []
+    for fill_with in (0, 0x7C00, 0x7E00, 0x7BFF, -0x8000 + 0x7C00, -1):
+        rng = np.random.default_rng(21)
+        kv = pool(dtype, D, Hkv, rep, rows_each)
+        kv.pages.view(torch.int16).fill_(fill_with)
+        data = put(kv, [rng.normal(0, 1, (n, Hkv, D)) for n in (61, 131)], [rng.normal(0, 1e-3, (n, Hkv, D)) for n in (61, 131)], dtype)
+        q = rows(rng, 2 * rows_each, Hkv * rep, D, dtype)
+        got.append(kv.attention(0, q, None, ints([61 - rows_each, 131 - rows_each]), None if rows_each == 1 else starts_of([rows_each] * 2)))
+        assert torch.equal(got[-1], got[0])
+    compare(kv, data, q, [rows_each] * 2, dtype)
+
+
+@pytest.mark.parametrize("vscale", [1e-1, 1e-3])
+@pytest.mark.parametrize("dtype,D,Hkv,rep", [("bf16", 64, 1, 2), ("bf16", 128, 1, 8), ("bf16", 256, 2, 1), ("bf16", 96, 1, 3), ("f32", 128, 1, 2)])
+def test_small_values_over_long_and_short_contexts(cuda_lib, dtype, D, Hkv, rep, vscale):
+    """Segments that are cut and joined, whose pieces raise their scales by different powers of two; and sequences of a few positions."""
+    rng = np.random.default_rng(D)
+    kv = make(1, Hkv, D, n_pages=300, max_seqs=6, max_pages=160, page=64)
+    lens = [9001, 1, 2, 16, 17, 4000]
+    vs = [rng.normal(0, vscale, (n, Hkv, D)) * np.where(np.arange(n) > n // 2, 1.0, 0.03)[:, None, None] for n in lens]
+    data = put(kv, [rng.normal(0, 1, (n, Hkv, D)) for n in lens], vs, dtype)
+    compare(kv, data, rows(rng, len(lens), Hkv * rep, D, dtype, 1.5), [1] * len(lens), dtype)
